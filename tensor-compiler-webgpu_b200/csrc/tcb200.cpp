@@ -359,12 +359,14 @@ int encode_maps(int n_maps, const uint64_t* d, TmaBlock* blk) {
     uint64_t addr = v[0], cols = v[1], rows = v[2], batches = v[3], rs = v[4], bs = v[5], bc = v[6] & 0xFFFFFFFFull,
              br = v[7];
     const bool atom32 = (v[6] >> 32) & 1;  // 128-byte swizzle of 32-byte chunks (MN-major tf32 tiles)
-    if (atom32 && bc * 4 != 128) return fail(TC_ERR_INVALID, "tensor map %d: 32-byte-atom swizzle needs 128-byte rows", m);
+    const bool half = (v[6] >> 33) & 1;    // fp16 elements
+    const uint64_t row = bc * (half ? 2 : 4);   // bytes of a box row
+    if (atom32 && (half || row != 128)) return fail(TC_ERR_INVALID, "tensor map %d: 32-byte-atom swizzle needs 128-byte rows of floats", m);
     if (addr % 16) return fail(TC_ERR_INVALID, "tensor map %d: address not 16-byte aligned", m);
     if (rs % 16 || bs % 16) return fail(TC_ERR_INVALID, "tensor map %d: strides must be multiples of 16 bytes", m);
-    if ((bc * 4 != 128 && bc * 4 != 64 && bc * 4 != 32) || br == 0 || br > 256)
-      return fail(TC_ERR_INVALID, "tensor map %d: box of %llu x %llu floats", m, (unsigned long long)bc,
-                  (unsigned long long)br);
+    if ((row != 128 && row != 64 && row != 32) || br == 0 || br > 256)
+      return fail(TC_ERR_INVALID, "tensor map %d: box of %llu x %llu %s", m, (unsigned long long)bc,
+                  (unsigned long long)br, half ? "halves" : "floats");
     if (cols == 0 || rows == 0 || batches == 0) return fail(TC_ERR_INVALID, "tensor map %d: empty", m);
     cuuint64_t dims[3] = {cols, rows, batches};
     cuuint64_t strides[2] = {rs, bs};
@@ -372,10 +374,10 @@ int encode_maps(int n_maps, const uint64_t* d, TmaBlock* blk) {
     cuuint32_t estr[3] = {1, 1, 1};
     // the swizzle spans one box row: 128, 64 or 32 bytes
     CUtensorMapSwizzle sw = atom32 ? CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B
-                            : bc * 4 == 128 ? CU_TENSOR_MAP_SWIZZLE_128B
-                            : bc * 4 == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B;
-    CUresult r = CU(cuTensorMapEncodeTiled)(&blk->maps[m], CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, (void*)addr, dims, strides,
-                                        box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
+                            : row == 128 ? CU_TENSOR_MAP_SWIZZLE_128B
+                            : row == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B;
+    CUresult r = CU(cuTensorMapEncodeTiled)(&blk->maps[m], half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32,
+                                        3, (void*)addr, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
                                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(TC_ERR_INVALID, "cuTensorMapEncodeTiled (map %d): %s", m, cu_name(r));
   }
