@@ -59,6 +59,21 @@ def _max_rule(G, n, gy):
     raise GradientError("max has no gradient; wrap it in stopGradient where its gradient is zero (as softmax does)")
 
 
+def _linear_nll_rule(G, n, gy, need):
+    names = ("h", "w", "b") if n.attrs["bias"] else ("h", "w")
+    ins = [*n.inputs, n.id, gy]
+    return [G.emit("linearNllGrad", ins, {**n.attrs, "wrt": k}) if want else None
+            for k, want in zip(names, need)] + [None]
+
+
+def _head_norm_rope_rule(G, n, gy, need):
+    return [G.emit("headNormRopeGrad", [*n.inputs, gy], {**n.attrs, "wrt": k}) if want else None
+            for k, want in zip(("x", "gain"), need)] + [None]
+
+
+# Rules told which inputs' gradients are wanted: one launch computes all of a node's, and only those.
+SELECTIVE = (_linear_nll_rule, _head_norm_rope_rule)
+
 RULES = {
     "add": lambda G, n, gy: [gy, gy],
     "sub": lambda G, n, gy: [gy, G.neg(gy)],
@@ -78,6 +93,8 @@ RULES = {
     "step": lambda G, n, gy: [None],
     "stopGradient": lambda G, n, gy: [None],
     "max": _max_rule,
+    "linearNll": _linear_nll_rule,
+    "headNormRope": _head_norm_rope_rule,
 }
 
 
@@ -129,7 +146,10 @@ def grad(graph, outputs, wrt, rules=None, prefix="d"):
         rule = rules.get(node.op)
         if rule is None:
             raise GradientError(f"no gradient rule for '{node.op}'")
-        contributions = rule(G, node, cot[nid])
+        if rule in SELECTIVE:
+            contributions = rule(G, node, cot[nid], [depends[i] for i in node.inputs])
+        else:
+            contributions = rule(G, node, cot[nid])
         for k, inp in enumerate(node.inputs):
             if contributions[k] is not None and depends[inp]:
                 accumulate(inp, contributions[k])

@@ -22,7 +22,8 @@ from __future__ import annotations
 import math
 import struct
 
-from .ir import size, strides, f32
+from .ir import TRAINING_OPS, size, strides, f32
+from .training_ops import siblings, training_launch
 
 MAX_RANK = 6  # src/gpu/codegen.js:16, kept for the gather rank limit of the interface
 WG = 256  # threads per CTA of the 1-D templates (the reference's WG = 64, src/gpu/codegen.js:12)
@@ -1208,12 +1209,18 @@ def lower(graph, matmul="naive", sabotage=None, fold=False, keep=()):
     folds = foldable_transposes(graph, matmul, keep) if fold else set()
     tprods = transposed_products(graph, matmul, keep, folds) if fold else {}
     tmats = set(tprods.values())
+    groups = siblings(graph)
     launches = []
     for node in graph.nodes:
         if node.op in ("input", "const") or node.id in folds or node.id in tmats:
             continue
         if node.id in tprods:
             launches.append(_transposed_product_launch(graph, node, graph.nodes[tprods[node.id]], matmul, folds))
+            continue
+        if node.op in TRAINING_OPS:
+            lau = training_launch(graph, node, groups)
+            if lau is not None:
+                launches.append(lau)
             continue
         if folds and _matmul_operands(graph, node) and set(_matmul_operands(graph, node)) & folds:
             lau = _folded_launch(graph, node, matmul, sabotage, folds)
@@ -1536,6 +1543,7 @@ def lower_fused(graph, matmul="naive", sabotage=None, fold=False, keep=(), colfu
     producer_of = {p: (sid, w, f) for sid, (p, w, f) in sums.items()}
     mos = mo_fusions(graph, keep, exclude=set(sums) | set(producer_of) | folds | set(tprods) | tmats) if mofuse else {}
     readers = set(mos.values())
+    groups = siblings(graph)
     launches = []
     for node in graph.nodes:
         if node.op in ("input", "const") or node.id in folds or node.id in readers or node.id in tmats:
@@ -1555,6 +1563,11 @@ def lower_fused(graph, matmul="naive", sabotage=None, fold=False, keep=(), colfu
             pid, write, make = sums[node.id]
             if not write:
                 launches.append(make(graph, graph.nodes[pid], node, False))
+            continue
+        if node.op in TRAINING_OPS:
+            lau = training_launch(graph, node, groups)
+            if lau is not None:
+                launches.append(lau)
             continue
         ops = _matmul_operands(graph, node) if folds else None
         if ops and set(ops) & folds:

@@ -19,6 +19,12 @@ BINARY = ("add", "sub", "mul", "div")
 REDUCE = ("sum", "max")
 # src/ir/shapes.js:51-52 (same order)
 OPS = ("input", "const") + BINARY + UNARY + ("matmul",) + REDUCE + ("broadcast", "reshape", "transpose")
+# Operators of a decoder's training step that the backend has whole kernels for (the reference has none of
+# them; its composites would hold the logits, or pass over the values several times).
+TRAINING_OPS = ("linearNll", "linearNllGrad", "headNormRope", "headNormRopeGrad", "orthogonalize")
+OPS += TRAINING_OPS
+MAX_CLASSES = 1 << 24    # class indices and positions are whole numbers in float32
+MAX_HEAD = 512
 
 
 class ShapeError(ValueError):
@@ -84,6 +90,8 @@ def infer_shape(op, shapes, attrs):
     """The result shape of ``op`` (src/ir/shapes.js:55-114)."""
     if op not in OPS:
         raise ShapeError(f"unknown op '{op}'")
+    if op in TRAINING_OPS:
+        return _infer_training(op, shapes, attrs)
     want = {"input": 0, "const": 0, "matmul": 2}.get(op, 2 if op in BINARY else 1)
     if len(shapes) != want:
         raise ShapeError(f"{op}: takes {want} inputs, got {len(shapes)}")
@@ -138,6 +146,140 @@ def infer_shape(op, shapes, attrs):
             raise ShapeError(f"transpose: {p!r} is not a permutation of rank {len(x)}")
         return [x[i] for i in p]
     raise ShapeError(f"no shape rule for '{op}'")
+
+
+def _number(v):
+    return isinstance(v, (int, float)) and not isinstance(v, bool) and math.isfinite(v)
+
+
+def _infer_nll(op, shapes, attrs):
+    bias = attrs.get("bias")
+    if not isinstance(bias, bool):
+        raise ShapeError(f"{op}: bias must be true or false")
+    back = op == "linearNllGrad"
+    want = 3 + bias + 2 * back
+    if len(shapes) != want:
+        raise ShapeError(f"{op}: takes {want} inputs, got {len(shapes)}")
+    h, w = shapes[0], shapes[1]
+    if len(h) != 2 or len(w) != 2 or h[1] != w[0]:
+        raise ShapeError(f"{op}: rows {fmt(h)} and weight {fmt(w)} must be [R,d] and [d,V]")
+    if w[1] > MAX_CLASSES:
+        raise ShapeError(f"{op}: {w[1]} classes, at most {MAX_CLASSES} (a class index is a float32)")
+    if bias and list(shapes[2]) != [w[1]]:
+        raise ShapeError(f"{op}: bias {fmt(shapes[2])} for {w[1]} classes")
+    for what, s in zip(("targets", "loss", "cotangent"), shapes[2 + bias:]):
+        if list(s) != [h[0]]:
+            raise ShapeError(f"{op}: {what} {fmt(s)} for {h[0]} rows")
+    if not back:
+        return [h[0]]
+    wrt = attrs.get("wrt")
+    if wrt not in ("h", "w", "b") or (wrt == "b" and not bias):
+        raise ShapeError(f"{op}: no gradient with respect to {wrt!r}")
+    return list(h) if wrt == "h" else list(w) if wrt == "w" else [w[1]]
+
+
+def _infer_head(op, shapes, attrs):
+    back = op == "headNormRopeGrad"
+    want = 3 + back
+    if len(shapes) != want:
+        raise ShapeError(f"{op}: takes {want} inputs, got {len(shapes)}")
+    x, gain, pos = shapes[:3]
+    if len(x) != 4:
+        raise ShapeError(f"{op}: x must be [B,T,H,D], got {fmt(x)}")
+    B, T, H, D = x
+    if D > MAX_HEAD:
+        raise ShapeError(f"{op}: a head of {D} values, at most {MAX_HEAD}")
+    if list(gain) != [D]:
+        raise ShapeError(f"{op}: gain {fmt(gain)} for heads of {D}")
+    if list(pos) not in ([T], [B, T]):
+        raise ShapeError(f"{op}: positions {fmt(pos)} must be {fmt([T])} or {fmt([B, T])}")
+    r = attrs.get("rotary")
+    if not _is_int(r) or r < 0 or r > D or r % 2:
+        raise ShapeError(f"{op}: rotary must be an even number of a head's {D} values, got {r!r}")
+    for name in ("interleaved", "headsFirst"):
+        if not isinstance(attrs.get(name), bool):
+            raise ShapeError(f"{op}: {name} must be true or false")
+    if not _number(attrs.get("eps")) or f32(attrs["eps"]) < 0 or not math.isfinite(f32(attrs["eps"])):
+        raise ShapeError(f"{op}: eps must be a number of at least 0")
+    if not _number(attrs.get("base")) or attrs["base"] <= 0:
+        raise ShapeError(f"{op}: base must be a number above 0")
+    out = [B, H, T, D] if attrs["headsFirst"] else [B, T, H, D]
+    if not back:
+        return out
+    if list(shapes[3]) != out:
+        raise ShapeError(f"{op}: cotangent {fmt(shapes[3])} of a value {fmt(out)}")
+    wrt = attrs.get("wrt")
+    if wrt not in ("x", "gain"):
+        raise ShapeError(f"{op}: no gradient with respect to {wrt!r}")
+    return list(x) if wrt == "x" else [D]
+
+
+NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)   # the Muon optimiser's quintic
+F16_ROOM = 60000.0    # largest scaled value held in fp16, a little below its limit
+
+
+def newton_schulz_scales(steps, coeffs):
+    """Exponents (x, s, p) of the powers of two that scale X, S and P of every Newton-Schulz step into fp16.
+
+    Singular values start in [0, 1] (the Frobenius norm is divided out) and every step maps them by
+    a t + b t^3 + c t^5, so the largest singular value after each step, and with it the largest entry that
+    X, S = X X^T and P = b S + c S S can have, follow from the extrema of polynomials.  1 % is left for the
+    rounding of the products."""
+    a, b, c = coeffs
+    top, mx, ms, mp = 1.0, 0.0, 0.0, 0.0
+    for _ in range(steps):
+        s = top * top
+        mx, ms = max(mx, top), max(ms, s)
+        mp = max(mp, abs(b * s + c * s * s))
+        if c != 0 and 0 < -b / (2 * c) < s:
+            mp = max(mp, abs(b * b / (4 * c)))
+        nxt = abs(a * top + b * top * s + c * top * s * s)
+        if c != 0:
+            disc = 9 * b * b - 20 * a * c
+            roots = [(-3 * b + math.sqrt(disc)) / (10 * c), (-3 * b - math.sqrt(disc)) / (10 * c)] if disc >= 0 else []
+        else:
+            roots = [-a / (3 * b)] if b != 0 else []
+        for t in roots:
+            if 0 < t < s:
+                q = math.sqrt(t)
+                nxt = max(nxt, abs(a * q + b * q * t + c * q * t * t))
+        top = nxt * 1.01
+    out = []
+    for bound in (mx, ms, mp):
+        k = 0
+        while k < 15 and bound * 1.01 * (2 << k) <= F16_ROOM:
+            k += 1
+        if not bound * 1.01 * (1 << k) <= F16_ROOM:
+            raise ShapeError(f"orthogonalize: coefficients {tuple(coeffs)} let the values grow beyond fp16 in {steps} steps")
+        out.append(k)
+    return tuple(out)
+
+
+def _infer_orthogonalize(op, shapes, attrs):
+    if len(shapes) != 1:
+        raise ShapeError(f"{op}: takes 1 input, got {len(shapes)}")
+    x = shapes[0]
+    if len(x) < 2:
+        raise ShapeError(f"{op}: needs rank >= 2, got {fmt(x)}")
+    if size(x[:-2]) > 65535:
+        raise ShapeError(f"{op}: {size(x[:-2])} matrices in {fmt(x)}, at most 65535")
+    steps, co, eps = attrs.get("steps"), attrs.get("coeffs"), attrs.get("eps")
+    if not _is_int(steps) or not 1 <= steps <= 32:
+        raise ShapeError(f"{op}: steps must be 1 to 32, got {steps!r}")
+    if not isinstance(co, (list, tuple)) or len(co) != 3 or not all(_number(v) for v in co):
+        raise ShapeError(f"{op}: coeffs must be three numbers, got {co!r}")
+    if not _number(eps) or eps < 0:
+        raise ShapeError(f"{op}: eps must be a number of at least 0, got {eps!r}")
+    newton_schulz_scales(steps, co)
+    return list(x)
+
+
+def _infer_training(op, shapes, attrs):
+    if op in ("linearNll", "linearNllGrad"):
+        return _infer_nll(op, shapes, attrs)
+    if op in ("headNormRope", "headNormRopeGrad"):
+        return _infer_head(op, shapes, attrs)
+    return _infer_orthogonalize(op, shapes, attrs)
 
 
 class Node:
@@ -267,6 +409,32 @@ class Graph:
     def log_softmax(self, x, axis=-1):
         z = self._shifted(x, axis)
         return self.sub(z, self.log(self.sum(self.exp(z), axis, True)))
+
+    # ---- operators of a decoder's training step ----
+    def linear_nll(self, h, w, bias, targets):
+        """-log softmax(h w + bias)[target] of every row, [R]: the cross entropy of a linear head without
+        its logits (h [R,d], w [d,V], bias [V] or None, targets [R]: class indices held in float32).
+
+        A row whose target is not in 0 .. V-1 (-1, say, for padding) has loss 0 and no gradient, and
+        nothing of its row of h is used.  Gradients: h, w and bias."""
+        ins = [h, w] + ([] if bias is None else [bias]) + [targets]
+        return self.emit("linearNll", ins, {"bias": bias is not None})
+
+    def head_norm_rope(self, x, gain, pos, base=10000.0, eps=1e-6, rotary=None, interleaved=False,
+                       heads_first=True):
+        """RMS norm over every head of x [B,T,H,D] times gain [D], its first `rotary` values (all of them
+        when None) turned by position: pair i by pos * base^(-2i/rotary), pairs being halves apart or, with
+        `interleaved`, neighbours.  pos is [T] or [B,T].  The result is [B,H,T,D], what attention reads, or
+        x's shape without `heads_first`.  Gradients: x and gain."""
+        return self.emit("headNormRope", [x, gain, pos],
+                         {"base": base, "eps": eps, "rotary": self.shape(x)[-1] if rotary is None else rotary,
+                          "interleaved": interleaved, "headsFirst": heads_first})
+
+    def orthogonalize(self, x, steps=5, coeffs=NEWTON_SCHULZ, eps=1e-7):
+        """Newton-Schulz orthogonalisation of the matrix (or every matrix of the stack) x [..., m, n]:
+        x / (|x|_F + eps), then `steps` times X = a X + (b S + c S S) X with S = X X^T.  No gradient: it is
+        an optimiser's."""
+        return self.emit("orthogonalize", [x], {"steps": steps, "coeffs": list(coeffs), "eps": eps})
 
 
 def strides(shape):

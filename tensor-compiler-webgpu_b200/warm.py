@@ -114,6 +114,18 @@ def full_size_sources():
     return codes
 
 
+def training_sources():
+    """The modules of the training operators: sizes are run-time parameters, so these serve every shape of
+    the usual head layouts and the default Newton-Schulz coefficients."""
+    from . import training_ops as to
+    from .ir import NEWTON_SCHULZ
+    codes = {to.nll_source(bias) for bias in (False, True)}
+    codes |= {to.orth_source(steps, NEWTON_SCHULZ, 1e-7) for steps in (1, 2, 5)}
+    for D in (16, 32, 48, 64, 80, 96, 128, 192, 256):
+        codes |= {to.head_source(D, rot, pairs) for rot in (D, D // 2) for pairs in (False, True)}
+    return codes
+
+
 def graph_sources(graphs):
     """Kernels of (graph, keep) pairs on both matmul paths, fused and unfused."""
     codes = set()
@@ -130,7 +142,7 @@ def warm(full=True, prune=True, extra=()):
     import os
     codes = standard_sources(full) | set(extra)
     if full:
-        codes |= sweep_sources() | fuzz_sources(10) | full_size_sources()
+        codes |= sweep_sources() | fuzz_sources(10) | full_size_sources() | training_sources()
     n = rt.precompile(codes)
     if prune and full and os.path.isdir(rt.CACHE_DIR):
         keep = {os.path.basename(rt._cache_path(c)) for c in codes}
