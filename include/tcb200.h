@@ -112,7 +112,7 @@ int tc_launch(tc_module* mod, const char* kernel, const uint32_t grid[3], const 
  * swizzle of 32-byte chunks instead: the shared-memory layout the tensor cores
  * read an MN-major tf32 operand tile in.
  * Bit 33 of box_cols says that the elements are fp16: cols, rows and the box count halves, and
- * box_cols * 2 is one of 128, 64 or 32 bytes. */
+ * box_cols * 2 is one of 128, 64 or 32 bytes.  Bit 34 makes a box two planes (batches) deep. */
 int tc_launch_tma(tc_module* mod, const char* kernel, const uint32_t grid[3], const uint32_t block[3],
                   uint32_t smem_bytes, int n_maps, const uint64_t* map_desc /* 8 per map */,
                   const tc_args* args);

@@ -60,10 +60,13 @@ def _max_rule(G, n, gy):
 
 
 def _linear_nll_rule(G, n, gy, need):
+    if n.attrs["out"] != "loss":
+        raise GradientError("linearNll: the saved value has no gradient")
+    (_, d), V = G.shape(n.inputs[0]), G.shape(n.inputs[1])[1]
+    saved = G.emit("linearNll", n.inputs, {**n.attrs, "out": "saved"})   # by the loss's own launch
     names = ("h", "w", "b") if n.attrs["bias"] else ("h", "w")
-    ins = [*n.inputs, n.id, gy]
-    return [G.emit("linearNllGrad", ins, {**n.attrs, "wrt": k}) if want else None
-            for k, want in zip(names, need)] + [None]
+    return [G.emit("linearNllGrad", [n.inputs[-1], saved, gy], {"bias": n.attrs["bias"], "d": d, "V": V, "wrt": k})
+            if want else None for k, want in zip(names, need)] + [None]
 
 
 def _head_norm_rope_rule(G, n, gy, need):

@@ -360,6 +360,7 @@ int encode_maps(int n_maps, const uint64_t* d, TmaBlock* blk) {
              br = v[7];
     const bool atom32 = (v[6] >> 32) & 1;  // 128-byte swizzle of 32-byte chunks (MN-major tf32 tiles)
     const bool half = (v[6] >> 33) & 1;    // fp16 elements
+    const uint32_t depth = 1 + ((v[6] >> 34) & 1);   // planes a box takes
     const uint64_t row = bc * (half ? 2 : 4);   // bytes of a box row
     if (atom32 && (half || row != 128)) return fail(TC_ERR_INVALID, "tensor map %d: 32-byte-atom swizzle needs 128-byte rows of floats", m);
     if (addr % 16) return fail(TC_ERR_INVALID, "tensor map %d: address not 16-byte aligned", m);
@@ -370,7 +371,7 @@ int encode_maps(int n_maps, const uint64_t* d, TmaBlock* blk) {
     if (cols == 0 || rows == 0 || batches == 0) return fail(TC_ERR_INVALID, "tensor map %d: empty", m);
     cuuint64_t dims[3] = {cols, rows, batches};
     cuuint64_t strides[2] = {rs, bs};
-    cuuint32_t box[3] = {(cuuint32_t)bc, (cuuint32_t)br, 1};
+    cuuint32_t box[3] = {(cuuint32_t)bc, (cuuint32_t)br, depth};
     cuuint32_t estr[3] = {1, 1, 1};
     // the swizzle spans one box row: 128, 64 or 32 bytes
     CUtensorMapSwizzle sw = atom32 ? CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B

@@ -13,20 +13,34 @@
 // The tensor core truncates its float32 accumulator after every instruction, so a long chain drifts
 // towards zero: by 3e-9 of the result a K index, measured (2.5e-5 at K = 8192).  A chain therefore ends
 // after CHUNK indices; the epilogue warps add the chunks in registers, rounded to nearest, while the next
-// one runs in the other TMEM accumulator.  With 256 the drift is below 1e-6; shorter chains leave the
-// epilogue less time behind the products (K = 1024, exponentials in the epilogue: 10.8 ms with 256, 11.8
-// with 128, 13.2 with 64).
+// one runs in the other TMEM buffer.  With 256 the drift is below 1e-6; shorter chains leave the epilogue
+// less time behind the products (K = 1024, exponentials in the epilogue: 10.8 ms with 256, 11.8 with 128,
+// 13.2 with 64).  Tiles narrower than 256 have TMEM to spare: their mixed terms go to accumulators of
+// their own, which keeps the drift of the main one to a third and breaks up the chain of dependent
+// instructions (a 64-wide product takes about 100 clocks in a chain, 32 by its size).
 //
 // Persistent, one CTA per SM, warps specialised: warp 0 loads the stage's four tiles by TMA, one lane of
 // warp 1 issues three tcgen05.mma.kind::f16 (M = 128, N = BN, K = 16) per K step into one of two TMEM
-// accumulators, warps 4-11 collect the other: a quarter of the rows and half of the columns each, up to
-// 128 sums a thread, on which the epilogue then runs 32 columns at a time.  They need more registers than
-// an even share (168), so the first warpgroup gives up most of its own: 40 + 2 x 232 = 3 x 168.  Either operand may
-// be K-major (64-byte rows) or MN-major (rows of 64 M or N values, 128 bytes), so no operand is ever
-// transposed in memory.  A symmetric product (SYM) computes the tiles on or above the diagonal only and
-// its epilogue mirrors them.
+// buffers, warps 4-11 collect the other: a quarter of the rows and half of the columns each, up to 128
+// sums a thread, on which the epilogue then runs 32 columns at a time.  They need more registers than an
+// even share (168), so the first warpgroup gives up most of its own: 40 + 2 x 232 = 3 x 168.  Either
+// operand may be K-major (64-byte rows) or MN-major (rows of 64 M or N values, 128 bytes), so no operand is
+// ever transposed in memory.  A symmetric product (SYM) computes the tiles on or above the diagonal only
+// and its epilogue mirrors them.
 //
-// p[0] = M, p[1] = N, p[2] = K, p[3] = batch, p[15] = error word; the rest is the epilogue's.
+// Work: the first `full` tiles go whole to the CTAs in turn, in grouped raster order.  The others, where a
+// last wave would leave SMs idle or there are fewer tiles than SMs, are one line of units of `quantum`
+// chunks, cut into equal runs, one a CTA.  A run that holds a part of a tile only leaves its sums in
+// scratch; the warp that arrives last at its part of the tile adds them all, in order, and goes on to the
+// epilogue: no CTA waits for another, and the result does not depend on which came last.
+//
+// p[0] = M | N << 32, p[1] = K | batch << 32, p[2] = full | quantum << 32, p[3] = byte offset in scratch of
+// the partial sums (two 128 x BN slots a CTA), p[15] = control block: the error word, 16 bytes on a
+// counter per warp and tile, zero between launches.  Maps: A, B ({cols, rows, 2 batch}: each matrix's hi
+// plane, then its lo plane, a box taking both) and the epilogue's.  BLOCKED operands (no batch) are stored in
+// blocks of 256 columns, a block's planes of 512-byte rows in the place of a batch: with rows as long as a
+// vocabulary every row of a K-major box lies in a page of its own (dh at 8192 x 1024 x 50001: 1.34 us a stage
+// of 32 K indices, the same product of short rows 0.70).
 #pragma once
 #include "tcb/sm100.cuh"
 
@@ -67,26 +81,34 @@ template <int BN> struct F16x3 {
   static constexpr u32 STAGING = 8 * 4096;                           // a 4 KB block per epilogue warp
   static constexpr u32 FIT = (227 * 1024 - 2048 - STAGING) / STAGE;  // 1 KB of barriers, 1 KB to align
   static constexpr u32 STAGES = FIT > 8 ? 8 : FIT;
+  static constexpr u32 ACCS = BN == 256 ? 1 : BN == 128 ? 2 : 3;     // accumulators of a TMEM buffer
+  static constexpr u32 TMEM = 512;                                   // columns allocated: 2 ACCS BN, a power of 2
 };
 
 // Shared-memory matrix descriptors.  K-major: 64-byte rows, 64-byte swizzle, 8-row groups 512 bytes
 // apart.  MN-major: rows of 64 values along M or N, one per K index, 128-byte swizzle; 8-row groups 1 KB
-// apart and the next 64 M or N values HG_K rows on.
-__device__ __forceinline__ u64 f16_kdesc(u32 saddr) {
-  return (u64)((saddr >> 4) & 0x3FFF) | (u64)1 << 16 | (u64)(512 >> 4) << 32 | (u64)1 << 46 | (u64)4 << 61;
+// apart and the next 64 M or N values 2 HG_K rows on (their lo plane lies between).  Only the address in the
+// low word changes.
+template <bool MN> __device__ __forceinline__ u32 f16_desc_lo(u32 saddr) {
+  return (saddr >> 4) | (MN ? (2 * HG_K * 128) >> 4 : 1) << 16;
 }
-__device__ __forceinline__ u64 f16_mndesc(u32 saddr) {
-  return (u64)((saddr >> 4) & 0x3FFF) | (u64)((HG_K * 128) >> 4) << 16 | (u64)(1024 >> 4) << 32 | (u64)1 << 46 |
-         (u64)2 << 61;
+template <bool MN> __host__ __device__ constexpr u32 f16_desc_hi() {
+  return MN ? 1024u >> 4 | 1u << 14 | 2u << 29 : 512u >> 4 | 1u << 14 | 4u << 29;
 }
 // D f32, A and B f16, M = 128, N = n
 __host__ __device__ constexpr u32 idesc_f16(u32 n, u32 a_mn, u32 b_mn) {
   return (1u << 4) | (a_mn << 15) | (b_mn << 16) | ((n >> 3) << 17) | ((u32)(HG_M >> 4) << 24);
 }
-__device__ __forceinline__ void mma_f16(u32 tmem, u64 a, u64 b, u32 idesc, u32 accumulate) {
-  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-               " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
-               :: "r"(tmem), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+__device__ __forceinline__ bool elect_one() {
+  u32 p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(p));
+  return p != 0;
+}
+template <u32 ID, u32 AH, u32 BH>
+__device__ __forceinline__ void mma_f16(u32 tmem, u32 a, u32 b, bool accumulate) {
+  asm volatile("{\n .reg .pred p;\n .reg .b64 x, y;\n setp.ne.b32 p, %3, 0;\n mov.b64 x, {%1, %5};\n mov.b64 y, {%2, %6};\n"
+               " tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %4, p;\n}"
+               :: "r"(tmem), "r"(a), "r"(b), "r"((u32)accumulate), "n"(ID), "n"(AH), "n"(BH) : "memory");
 }
 __device__ __forceinline__ void tmem_ld32(u32 taddr, float (&r)[32]) {
   u32 v[32];
@@ -102,41 +124,76 @@ __device__ __forceinline__ void tmem_ld32(u32 taddr, float (&r)[32]) {
   for (int j = 0; j < 32; ++j) r[j] = __uint_as_float(v[j]);
 }
 
-struct F16Tile { int m0, n0, bz; u32 mt, nt; };
+struct F16Tile { int m0, n0, bz; };
 
-// Unit u -> output tile.  Grouped raster (8 tile rows per group) so the CTAs running together share
-// operand panels in L2; a symmetric product walks the tiles that reach the diagonal, row by row.
+// Tile u.  Grouped raster (8 tile rows per group) so the CTAs running together share operand panels in L2;
+// a symmetric product walks the tiles that reach the diagonal, row by row.
 template <int BN, bool SYM>
 __device__ __forceinline__ F16Tile f16_tile(u32 u, u32 tm, u32 tn, u32 per) {
   F16Tile T;
   T.bz = (int)(u / per);
-  u32 r = u % per;
+  u32 r = u % per, mt, nt;
   if (SYM) {
     u32 i = 0;
     for (;; ++i) {
       const u32 first = i * HG_M / BN, n = tn - first;
-      if (r < n) { T.nt = first + r; break; }
+      if (r < n) { nt = first + r; break; }
       r -= n;
     }
-    T.mt = i;
+    mt = i;
   } else {
     const u32 g = r / (8 * tn), first = g * 8;
     const u32 gsz = tm - first < 8 ? tm - first : 8;
     const u32 w = r - first * tn;
-    T.mt = first + w % gsz;
-    T.nt = w / gsz;
+    mt = first + w % gsz;
+    nt = w / gsz;
   }
-  T.m0 = (int)(T.mt * HG_M);
-  T.n0 = (int)(T.nt * BN);
+  T.m0 = (int)(mt * HG_M);
+  T.n0 = (int)(nt * BN);
   return T;
 }
 template <int BN, bool SYM>
-__device__ __forceinline__ u32 f16_units(u32 tm, u32 tn) {
+__device__ __forceinline__ u32 f16_tiles(u32 tm, u32 tn) {
   if (!SYM) return tm * tn;
   u32 n = 0;
   for (u32 i = 0; i < tm; ++i) n += tn - i * HG_M / BN;
   return n;
 }
+
+// The work of one CTA, in order: whole tiles, then its run of the divided ones.
+struct F16Work {
+  u32 tiles, full, chunks, quantum, per;   // per: units of a divided tile
+  u32 u;                                   // next whole tile
+  u64 at, end, total;                      // the run, in units over the divided tiles
+  u32 tile, c0, c1;                        // the current piece: chunks c0 .. c1 of a tile
+  __device__ __forceinline__ F16Work(u32 tiles_, u32 full_, u32 chunks_, u32 quantum_)
+      : tiles(tiles_), full(full_), chunks(chunks_), quantum(quantum_), per((chunks_ + quantum_ - 1) / quantum_),
+        u(blockIdx.x) {
+    total = (u64)(tiles - full) * per;
+    at = blockIdx.x * total / gridDim.x;
+    end = (blockIdx.x + 1) * total / gridDim.x;
+  }
+  __device__ __forceinline__ bool next() {
+    if (u < full) {
+      tile = u;
+      c0 = 0;
+      c1 = chunks;
+      u += gridDim.x;
+      return true;
+    }
+    if (at >= end) return false;
+    const u32 t = (u32)(at / per), k = (u32)(at - (u64)t * per);
+    const u32 n = (u32)(end - at < per - k ? end - at : per - k);
+    tile = full + t;
+    c0 = k * quantum;
+    c1 = (k + n) * quantum < chunks ? (k + n) * quantum : chunks;
+    at += n;
+    return true;
+  }
+  __device__ __forceinline__ bool whole() const { return c0 == 0 && c1 == chunks; }
+  // the CTA whose run holds unit x
+  __device__ __forceinline__ u32 owner(u64 x) const { return (u32)(((x + 1) * gridDim.x - 1) / total); }
+};
 
 // An epilogue warp's view of one tile: rows 32 q .. of it, columns from c0, this lane's row.
 struct F16Epi {
@@ -148,14 +205,54 @@ struct F16Epi {
 };
 
 // Written out block by block, so that every index into the sums is a constant and they stay in registers.
-template <int I, int NB>
+template <int BN, int I, int NB>
 __device__ __forceinline__ void f16_collect(float (&v)[NB][32], u32 t) {
   if constexpr (I < NB) {
+    constexpr int ACCS = (int)F16x3<BN>::ACCS;
     float w[32];
-    tmem_ld32(t + 32 * I, w);
+    if constexpr (ACCS > 1) {   // the mixed terms, 2^-11 of the main ones, first
+      tmem_ld32(t + BN + 32 * I, w);
+      if constexpr (ACCS > 2) {
+        float x[32];
+        tmem_ld32(t + 2 * BN + 32 * I, x);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) w[i] = __fadd_rn(w[i], x[i]);
+      }
+      float x[32];
+      tmem_ld32(t + 32 * I, x);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) w[i] = __fadd_rn(w[i], x[i]);
+    } else {
+      tmem_ld32(t + 32 * I, w);
+    }
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[I][i] = __fadd_rn(v[I][i], w[i]);
-    f16_collect<I + 1>(v, t);
+    f16_collect<BN, I + 1>(v, t);
+  }
+}
+// A warp's sums to or from a partial slot: 32 lanes side by side, 64 loads in flight.
+template <bool ADD, int NB>
+__device__ __forceinline__ void f16_partial_load(float (&v)[NB][32], const float* p) {
+  constexpr int STEP = NB > 1 ? 2 : 1;
+#pragma unroll
+  for (int b = 0; b < NB; b += STEP) {
+    float w[STEP][32];
+#pragma unroll
+    for (int k = 0; k < STEP; ++k)
+#pragma unroll
+      for (int i = 0; i < 32; ++i) w[k][i] = __ldcg(p + ((b + k) * 32 + i) * 32);
+#pragma unroll
+    for (int k = 0; k < STEP; ++k)
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[b + k][i] = ADD ? __fadd_rn(v[b + k][i], w[k][i]) : w[k][i];
+  }
+}
+template <int I, int NB>
+__device__ __forceinline__ void f16_partial_store(const float (&v)[NB][32], float* p) {
+  if constexpr (I < NB) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) __stcg(p + (I * 32 + i) * 32, v[I][i]);
+    f16_partial_store<I + 1>(v, p);
   }
 }
 template <int I, int NB, class EPI>
@@ -166,35 +263,42 @@ __device__ __forceinline__ void f16_blocks(EPI& epi, const F16Epi& e, float (&v)
   }
 }
 
-// EPI: struct with begin(e), block(e, c0, v) for each 32 columns (from column c0 of the tile) that reach into
+// EPI: struct with start(staging) once, by all 256 epilogue threads, begin(e), block(e, c0, v) for each 32 columns (from column c0 of the tile) that reach into
 // the output, end(e), and done(e) once after the last tile.
-template <int BN, bool A_MN, bool B_MN, bool SYM, int CHUNK, class EPI>
+template <int BN, bool A_MN, bool B_MN, bool SYM, bool BLOCKED, int CHUNK, class EPI>
 __device__ __forceinline__ void gemm_f16x3(const GemmParams& P, EPI& epi) {
   using S = F16x3<BN>;
-  constexpr int STAGES = (int)S::STAGES;
+  constexpr u32 STAGES = S::STAGES;
   extern __shared__ unsigned char smem_raw[];
   u32* err = reinterpret_cast<u32*>(P.a.p[15]);
   const u32 raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
   unsigned char* gbase = smem_raw + (base - raw);
   const u32 bars = base + STAGES * S::STAGE, staging = bars + 1024;
   u32* tmem_slot = reinterpret_cast<u32*>(gbase + STAGES * S::STAGE + (2 * STAGES + 4) * 8);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  auto full = [&](int s) { return bars + 8u * s; };
-  auto empty = [&](int s) { return bars + 8u * (STAGES + s); };
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  auto full = [&](u32 s) { return bars + 8u * s; };
+  auto empty = [&](u32 s) { return bars + 8u * (STAGES + s); };
   auto accf = [&](u32 b) { return bars + 8u * (2 * STAGES + b); };
   auto acce = [&](u32 b) { return bars + 8u * (2 * STAGES + 2 + b); };
-  const u32 M = (u32)P.a.p[0], N = (u32)P.a.p[1], K = (u32)P.a.p[2], batch = (u32)P.a.p[3];
+  const u32 M = (u32)P.a.p[0], N = (u32)((u64)P.a.p[0] >> 32), K = (u32)P.a.p[1], batch = (u32)((u64)P.a.p[1] >> 32);
   const u32 tm = (M + HG_M - 1) / HG_M, tn = (N + BN - 1) / BN, kbs = (K + HG_K - 1) / HG_K;
-  const u32 per = f16_units<BN, SYM>(tm, tn), units = per * batch;
+  constexpr u32 CK = CHUNK / HG_K;   // stages of a chunk
+  const u32 per = f16_tiles<BN, SYM>(tm, tn);
+  F16Work work(per * batch, (u32)P.a.p[2], (kbs + CK - 1) / CK, (u32)((u64)P.a.p[2] >> 32));
 
+  if (threadIdx.x == 32 * 3) {
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+      asm volatile("prefetch.tensormap [%0];" :: "l"(reinterpret_cast<u64>(&P.maps[m])) : "memory");
+  }
   if (threadIdx.x == 0) {
-    for (int s = 0; s < STAGES; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
+    for (u32 s = 0; s < STAGES; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
     for (u32 b = 0; b < 2; ++b) { mbar_init(accf(b), 1); mbar_init(acce(b), 8); }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(tmem_slot)),
-                 "r"((u32)(2 * BN)) : "memory");
+                 "r"(S::TMEM) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   tc_fence_before();
@@ -205,65 +309,88 @@ __device__ __forceinline__ void gemm_f16x3(const GemmParams& P, EPI& epi) {
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-    if (warp == 0 && lane == 0) {
-      u32 it = 0;
+    // Both warps run their loops whole and one elected lane issues: the operands of the copies and products are
+    // then the warp's, held in uniform registers.  Issued from a one-lane branch each product cost some 120
+    // clocks to issue, whatever its size; a wait's outcome is voted on so that the branches stay uniform too.
+    const bool leader = elect_one();
+    auto wait = [&](u32 bar, u32 parity, u32 code) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, code)) != 0; };
+    if (warp == 0) {
+      u32 it = 0, s = 0, phase = 0;
       bool ok = true;
-      for (u32 u = blockIdx.x; ok && u < units; u += gridDim.x) {
-        const F16Tile T = f16_tile<BN, SYM>(u, tm, tn, per);
-        for (u32 kb = 0; kb < kbs; ++kb, ++it) {
-          const int s = it % STAGES;
-          if (it >= (u32)STAGES && !mbar_wait(empty(s), ((it / STAGES) - 1) & 1, err, 1)) { ok = false; break; }
-          const u32 st = base + s * S::STAGE;
+      while (ok && work.next()) {
+        const F16Tile T = f16_tile<BN, SYM>(work.tile, tm, tn, per);
+        const u32 kend = work.c1 * CK < kbs ? work.c1 * CK : kbs;
+        for (u32 kb = work.c0 * CK; kb < kend; ++kb, ++it) {
+          if (it >= STAGES && !wait(empty(s), phase ^ 1, 1)) { ok = false; break; }
+          const u32 st = base + s * S::STAGE, sb = st + 2 * S::A_BYTES;
           const int kc = (int)(kb * HG_K);
-          mbar_expect_tx(full(s), S::STAGE);
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const u32 a = st + h * S::A_BYTES, b = st + 2 * S::A_BYTES + h * S::B_BYTES;
+          auto load = [&](u32 dst, const TmaDesc* map, int col, int row) {
+            if (BLOCKED) tma_load_3d(dst, map, full(s), col & 255, row, 2 * (col >> 8));
+            else tma_load_3d(dst, map, full(s), col, row, 2 * T.bz);
+          };
+          if (leader) {
+            mbar_expect_tx(full(s), S::STAGE);
+            // a box holds a tile's hi plane and, behind it, its lo plane
             if (A_MN) {
 #pragma unroll
-              for (int c = 0; c < HG_M / 64; ++c) tma_load_3d(a + c * HG_K * 128, &P.maps[h], full(s), T.m0 + 64 * c, kc, T.bz);
+              for (int c = 0; c < HG_M / 64; ++c) load(st + c * HG_K * 256, &P.maps[0], T.m0 + 64 * c, kc);
             } else {
-              tma_load_3d(a, &P.maps[h], full(s), kc, T.m0, T.bz);
+              load(st, &P.maps[0], kc, T.m0);
             }
             if (B_MN) {
 #pragma unroll
-              for (int c = 0; c < BN / 64; ++c) tma_load_3d(b + c * HG_K * 128, &P.maps[2 + h], full(s), T.n0 + 64 * c, kc, T.bz);
+              for (int c = 0; c < BN / 64; ++c) load(sb + c * HG_K * 256, &P.maps[1], T.n0 + 64 * c, kc);
             } else {
-              tma_load_3d(b, &P.maps[2 + h], full(s), kc, T.n0, T.bz);
+              load(sb, &P.maps[1], kc, T.n0);
             }
           }
+          __syncwarp();
+          if (++s == STAGES) { s = 0; phase ^= 1; }
         }
       }
       // wait (bounded) for the copies still in flight before this CTA may exit
-      for (u32 i = it > (u32)STAGES ? it - STAGES : 0; i < it; ++i) mbar_wait(full(i % STAGES), (i / STAGES) & 1, err, 2);
-    } else if (warp == 1 && lane == 0) {
-      constexpr u32 ID = idesc_f16(BN, A_MN ? 1u : 0u, B_MN ? 1u : 0u);
-      auto da = [&](u32 t, int k) { return A_MN ? f16_mndesc(t + 2048 * k) : f16_kdesc(t + 32 * k); };
-      auto db = [&](u32 t, int k) { return B_MN ? f16_mndesc(t + 2048 * k) : f16_kdesc(t + 32 * k); };
-      u32 it = 0, j = 0;   // stages, chunks
+      for (u32 i = it > STAGES ? it - STAGES : 0; i < it; ++i) mbar_wait(full(i % STAGES), (i / STAGES) & 1, err, 2);
+    } else if (warp == 1) {
+      constexpr u32 ID = idesc_f16(BN, A_MN ? 1u : 0u, B_MN ? 1u : 0u), AH = f16_desc_hi<A_MN>(), BH = f16_desc_hi<B_MN>();
+      // hi to lo plane, and one K step on, in descriptor units of 16 bytes
+      constexpr u32 AL = (A_MN ? HG_K * 128 : S::A_BYTES) >> 4, AK = (A_MN ? 2048 : 32) >> 4;
+      constexpr u32 BL = (B_MN ? HG_K * 128 : S::B_BYTES) >> 4, BK = (B_MN ? 2048 : 32) >> 4;
+      const u32 a0 = f16_desc_lo<A_MN>(base), b0 = f16_desc_lo<B_MN>(base + 2 * S::A_BYTES);
+      u32 j = 0, s = 0, phase = 0, da = a0, db = b0;   // j counts chunks
       bool ok = true;
-      for (u32 u = blockIdx.x; ok && u < units; u += gridDim.x) {
-        for (u32 k0 = 0; ok && k0 < kbs; k0 += CHUNK / HG_K, ++j) {
-          const u32 k1 = k0 + CHUNK / HG_K < kbs ? k0 + CHUNK / HG_K : kbs, buf = j & 1;
-          if (j >= 2 && !mbar_wait(acce(buf), ((j >> 1) - 1) & 1, err, 5)) { ok = false; break; }
+      while (ok && work.next()) {
+        for (u32 c = work.c0; ok && c < work.c1; ++c, ++j) {
+          const u32 k1 = (c + 1) * CK < kbs ? CK : kbs - c * CK, buf = j & 1;
+          if (j >= 2 && !wait(acce(buf), ((j >> 1) - 1) & 1, 5)) { ok = false; break; }
           tc_fence_after();
-          const u32 acc = tmem + buf * BN;
-          for (u32 kb = k0; kb < k1; ++kb, ++it) {
-            const int s = it % STAGES;
-            if (!mbar_wait(full(s), (it / STAGES) & 1, err, 3)) { ok = false; break; }
+          const u32 acc = tmem + buf * S::ACCS * BN;
+          for (u32 kb = 0; kb < k1; ++kb) {
+            if (!wait(full(s), phase, 3)) { ok = false; break; }
             tc_fence_after();
-            const u32 st = base + s * S::STAGE;
+            if (leader) {
 #pragma unroll
-            for (int k = 0; k < HG_K / 16; ++k) {
-              const u64 ah = da(st, k), al = da(st + S::A_BYTES, k);
-              const u64 bh = db(st + 2 * S::A_BYTES, k), bl = db(st + 2 * S::A_BYTES + S::B_BYTES, k);
-              mma_f16(acc, al, bh, ID, ((kb - k0) | k) != 0);
-              mma_f16(acc, ah, bl, ID, 1);
-              mma_f16(acc, ah, bh, ID, 1);
+              for (int k = 0; k < HG_K / 16; ++k) {
+                const u32 ah = da + AK * k, al = ah + AL, bh = db + BK * k, bl = bh + BL;
+                const bool on = k > 0 || kb != 0;
+                if (S::ACCS == 1) {
+                  mma_f16<ID, AH, BH>(acc, al, bh, on);
+                  mma_f16<ID, AH, BH>(acc, ah, bl, true);
+                  mma_f16<ID, AH, BH>(acc, ah, bh, true);
+                } else {
+                  mma_f16<ID, AH, BH>(acc + BN, al, bh, on);
+                  mma_f16<ID, AH, BH>(acc, ah, bh, on);
+                  mma_f16<ID, AH, BH>(acc + (S::ACCS - 1) * BN, ah, bl, S::ACCS == 2 || on);
+                }
+              }
+              mma_commit(empty(s));
             }
-            mma_commit(empty(s));
+            __syncwarp();
+            da += S::STAGE >> 4;
+            db += S::STAGE >> 4;
+            if (++s == STAGES) { s = 0; phase ^= 1; da = a0; db = b0; }
           }
-          if (ok) mma_commit(accf(buf));
+          if (ok && leader) mma_commit(accf(buf));
+          __syncwarp();
         }
       }
     }
@@ -271,33 +398,57 @@ __device__ __forceinline__ void gemm_f16x3(const GemmParams& P, EPI& epi) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
     constexpr int NB = BN / 64;   // 32-column blocks a warp
     F16Epi e;
+    const int w = warp - 4;
     e.q = warp & 3;
-    e.c0 = (warp - 4) / 4 * (BN / 2);
+    e.c0 = w / 4 * (BN / 2);
     e.lane = lane;
-    e.stage = staging + (u32)(warp - 4) * 4096;
+    e.stage = staging + (u32)w * 4096;
     e.gstage = gbase + (e.stage - base);
+    epi.start(e.gstage - w * 4096);
     u32 j = 0;
     bool ok = true;
-    for (u32 u = blockIdx.x; ok && u < units; u += gridDim.x) {
-      e.T = f16_tile<BN, SYM>(u, tm, tn, per);
+    while (ok && work.next()) {
+      e.T = f16_tile<BN, SYM>(work.tile, tm, tn, per);
       e.row = (u64)e.T.m0 + 32 * e.q + lane;
       float v[NB][32];
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[b][i] = 0.0f;
-      for (u32 k0 = 0; k0 < kbs; k0 += CHUNK / HG_K, ++j) {
+      for (u32 c = work.c0; c < work.c1; ++c, ++j) {
         const u32 buf = j & 1;
         if (!mbar_wait(accf(buf), (j >> 1) & 1, err, 4)) { ok = false; break; }
         tc_fence_after();
-        const u32 t = tmem + buf * BN + ((u32)(32 * e.q) << 16) + (u32)e.c0;
-        f16_collect<0>(v, t);
+        f16_collect<BN, 0>(v, tmem + buf * S::ACCS * BN + ((u32)(32 * e.q) << 16) + (u32)e.c0);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(acce(buf)) : "memory");
       }
       // this warp's part of the tile reaches into the output
-      if (ok && (u32)e.T.m0 + 32 * e.q < M && (u32)(e.T.n0 + e.c0) < N) {
+      bool mine = ok && (u32)e.T.m0 + 32 * e.q < M && (u32)(e.T.n0 + e.c0) < N;
+      if (mine && !work.whole()) {
+        // CTA c's slots: 2 c + 1 for the beginning of a tile, 2 c for a later part of one
+        constexpr u64 SLOT = (u64)8 * NB * 1024;
+        float* part = reinterpret_cast<float*>(P.a.scratch + (u64)P.a.p[3]) + (u64)w * NB * 1024 + lane;
+        f16_partial_store<0>(v, part + (2 * blockIdx.x + (work.c0 == 0)) * SLOT);
+        __threadfence();
+        __syncwarp();
+        const u64 first = (u64)(work.tile - work.full) * work.per;
+        const u32 ca = work.owner(first), cb = work.owner(first + work.per - 1);
+        u32* count = reinterpret_cast<u32*>(P.a.p[15]) + 4 + (work.tile - work.full) * 8 + w;
+        u32 old = 0;
+        if (lane == 0) old = atomicAdd(count, 1u);
+        old = __shfl_sync(0xffffffffu, old, 0);
+        mine = old == cb - ca;
+        if (mine) {
+          __threadfence();
+          f16_partial_load<false>(v, part + (2 * ca + 1) * SLOT);
+#pragma unroll 1
+          for (u32 c = ca + 1; c <= cb; ++c) f16_partial_load<true>(v, part + 2 * c * SLOT);
+          if (lane == 0) *count = 0u;   // every part has arrived: zero for the next launch
+        }
+      }
+      if (mine) {
         epi.begin(e);
         f16_blocks<0>(epi, e, v, N);
         epi.end(e);
@@ -309,16 +460,22 @@ __device__ __forceinline__ void gemm_f16x3(const GemmParams& P, EPI& epi) {
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"((u32)(2 * BN)) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(S::TMEM) : "memory");
   }
 }
 
-// ---- what epilogues share ----
+// ---- what the operators share ----
+
+// Clears a launch's control block of n words (its first kernel does).
+__device__ __forceinline__ void f16_clear(const Args& a, u32 n) {
+  if (blockIdx.x == 0 && blockIdx.y == 0 && a.p[15])
+    for (u32 i = threadIdx.x; i < n; i += blockDim.x) reinterpret_cast<u32*>(a.p[15])[i] = 0u;
+}
+constexpr u32 F16_CTRL = 4 + 8 * 2 * 148;   // words: the error word, 8 counters for each of up to 2 tiles an SM
 
 // 32 columns of hi / lo pairs through the warp's staging block to two planes of an fp16 array by TMA
-// store (map 4: {cols, rows, planes}, boxes of 32 x 32, 64-byte swizzle).
-__device__ __forceinline__ void store_split32(const F16Epi& e, const TmaDesc* map, const float (&v)[32], int col,
-                                              int row, int plane_hi, int plane_lo) {
+// store (map: {cols, rows, planes}, boxes of 32 x 32 x 2, 64-byte swizzle).
+__device__ __forceinline__ void store_split32(const F16Epi& e, const TmaDesc* map, const float (&v)[32], int col, int row, int matrix) {
   if (e.lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");   // the last store has read it
   __syncwarp();
   uint4* sp = reinterpret_cast<uint4*>(e.gstage);
@@ -336,8 +493,7 @@ __device__ __forceinline__ void store_split32(const F16Epi& e, const TmaDesc* ma
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   __syncwarp();
   if (e.lane == 0) {
-    tma_store_3d(map, e.stage, col, row, plane_hi);
-    tma_store_3d(map, e.stage + 2048, col, row, plane_lo);
+    tma_store_3d(map, e.stage, col, row, 2 * matrix);
     bulk_commit();
   }
 }

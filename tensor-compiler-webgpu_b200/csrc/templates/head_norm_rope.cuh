@@ -233,21 +233,26 @@ extern "C" __global__ void __launch_bounds__(256) tcb_head_norm_rope_grad(const 
   tcb::head_norm_rope<1, true>(a);
 }
 
-// dgain: the blocks' shares added up, 32 columns a block, warp k the shares k, k + 32, ...  p[0]: the shares.
+// dgain: the blocks' shares added up, 8 columns a block; thread row k takes the shares k, k + 128, ...
+// p[0]: the shares.
 extern "C" __global__ void __launch_bounds__(1024) tcb_head_gain_finish(const tcb::Args a) {
   tcb::grid_dependency_sync();
-  __shared__ float sh[32][33];
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
+  __shared__ float sh[32][8];
+  const int c = threadIdx.x & 7, row = threadIdx.x >> 3, col = blockIdx.x * 8 + c;
   const float* p = reinterpret_cast<const float*>(a.scratch);
   float s = 0.0f;
   if (col < TCB_D) {
-#pragma unroll 4
-    for (u32 k = w; k < (u32)a.p[0]; k += 32) s += p[(u64)k * TCB_D + col];
+#pragma unroll 10
+    for (u32 k = row; k < (u32)a.p[0]; k += 128) s += p[(u64)k * TCB_D + col];
   }
-  sh[w][lane] = s;
+  s += __shfl_xor_sync(0xffffffffu, s, 8);
+  s += __shfl_xor_sync(0xffffffffu, s, 16);
+  if ((threadIdx.x & 31) < 8) sh[threadIdx.x >> 5][c] = s;
   __syncthreads();
-  if (w == 0 && col < TCB_D) {
-    for (int k = 1; k < 32; ++k) s += sh[k][lane];
+  if (threadIdx.x < 8 && col < TCB_D) {
+    s = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 32; ++k) s += sh[k][c];
     reinterpret_cast<float*>(a.out)[col] = s;
   }
 }

@@ -8,23 +8,27 @@
 // A row whose target is not one of 0 .. V-1 (a negative one marks padding) is left out: its loss is 0, it
 // takes and gives no gradient, and what its row of h holds is never used.
 //
-// Forward: one matrix product (tcb/gemm_f16x3.cuh) whose epilogue keeps, per row and half tile of columns, the
-// running maximum and the sum of exponentials; tcb_nll_finish joins a row's tiles.  The logits exist in
-// tensor memory only.
-// Backward: the vocabulary is walked in pieces of TCB's host's choosing (a bounded workspace).  A piece's
-// logits are computed again, turned into dz in the epilogue -- as fp16 hi / lo, what the two products
-// after it read; |dz| <= |g_i|, so its scale is known before -- and dh += dz W_piece^T and
-// dW_piece = h^T dz follow.  db's column sums are taken in the dz epilogue.  lse_i is nll_i + z_i,t_i,
-// with the target's logit as a dot product in double, so the forward hands over no more than its loss.
+// Forward: one matrix product (tcb/gemm_f16x3.cuh) whose epilogue keeps, per row and half tile of columns,
+// the running maximum and the sum of exponentials; tcb_nll_finish joins a row's tiles.  The logits exist in
+// tensor memory and registers only, in units of log 2: z2 = log2(e) z is one fma from the sums, its
+// exponential one ex2 (2^-22 relative, as far off as the operands' split).
+// What the backward needs of it is saved in one opaque value (NllSaved): the scales, b log2(e), each
+// row's log2 of the sum, and h and W as split for the tensor core, 4 bytes a value.
+// Backward: the vocabulary is walked in pieces (a bounded workspace).  A piece's logits are computed
+// again, turned into dz in the epilogue -- as fp16 hi / lo, what the two products after it read;
+// |dz| <= |g_i|, so its scale is known before -- and dh += dz W_piece^T and dW_piece = h^T dz follow.
+// db's column sums are taken in the dz epilogue.
 //
 // dz below 2^-40 of the largest |g_i| rounds to zero, and keeps fewer than 22 bits below 2^-18 of it: the
 // gradient of a class whose probability is that small in every row has that absolute accuracy, which is
 // beneath the float32 rounding of the sums it enters.
 //
-// p[] of every kernel: [0..3] the product's M, N, K, batch (amax / split / finish: [0] the blocks of the
-// amax launch), [4] R, [5] d, [6] V, [7..11] byte offsets in scratch of h's split, W's split, the row
-// statistics, dz, the column-sum partials, [12] first column of the piece, [13] flags.
-// in[]: h, W, (b), t, then in the backward nll and the loss's cotangent.
+// p[] of every kernel: [0..3] the product's (split: [0] blocks of the amax launch; finish: [0] half tiles of a
+// row), [4] R, [5] d, [6] V, [7] byte offset of the saved value in scratch (a forward whose backward nobody
+// asks for), [8..10] byte offsets in it of the row sums, h and W, [11] byte offset in scratch of the targets'
+// logits (backward: of the column-sum partials), [12] of the row partials (backward: the piece's first
+// column), [13] 1 to add to dh, [14] address of the saved value or 0.
+// in[]: h, W, (b), t forward; t, saved, the loss's cotangent backward.
 #pragma once
 #include "tcb/gemm_f16x3.cuh"
 
@@ -34,35 +38,46 @@
 
 namespace tcb {
 
-constexpr int NLL_T = TCB_BIAS ? 3 : 2;
-constexpr u32 NLL_BACKWARD = 1, NLL_ADD = 2;
+constexpr float NLL_LOG2E = 1.44269504f, NLL_LN2 = 0.693147181f, NLL_MAX = 3.402823466e38f;
+#define TCB_MINUS_INF bits(0xff800000u)
 
-struct NllScales { float up_h, up_w, up_g, down_h, down_w, down_g; };   // at the start of scratch
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
 
-struct Nll {
+// At the start of the saved value; b log2(e) follows at 256 bytes, -inf beyond V up to a multiple of 256.
+struct NllScales { float down_h, down_w, z2; };
+
+template <bool BACK> struct Nll {
   const Args& a;
-  __device__ explicit Nll(const Args& args) : a(args) {}
-  __device__ u64 R() const { return (u64)a.p[4]; }
-  __device__ u64 d() const { return (u64)a.p[5]; }
-  __device__ u64 V() const { return (u64)a.p[6]; }
-  __device__ const float* h() const { return reinterpret_cast<const float*>(a.in[0]); }
-  __device__ const float* w() const { return reinterpret_cast<const float*>(a.in[1]); }
-  __device__ float bias(u64 v) const { return TCB_BIAS ? ld1(reinterpret_cast<const float*>(a.in[2]) + v) : 0.0f; }
+  __device__ __forceinline__ explicit Nll(const Args& args) : a(args) {}
+  __device__ __forceinline__ u64 R() const { return (u64)a.p[4]; }
+  __device__ __forceinline__ u64 d() const { return (u64)a.p[5]; }
+  __device__ __forceinline__ u64 V() const { return (u64)a.p[6]; }
+  __device__ __forceinline__ const float* h() const { return reinterpret_cast<const float*>(a.in[0]); }
+  __device__ __forceinline__ const float* w() const { return reinterpret_cast<const float*>(a.in[1]); }
   // the row's class, or -1 when it takes no part
-  __device__ int target(u64 row) const {
-    const float t = ld1(reinterpret_cast<const float*>(a.in[NLL_T]) + row);
+  __device__ __forceinline__ int target(u64 row) const {
+    const float t = ld1(reinterpret_cast<const float*>(a.in[BACK ? 0 : TCB_BIAS ? 3 : 2]) + row);
     return t >= 0.0f && t < (float)V() ? (int)t : -1;
   }
-  template <class X> __device__ X* at(u64 off) const { return reinterpret_cast<X*>(a.scratch + off); }
-  __device__ NllScales* scales() const { return at<NllScales>(0); }
-  __device__ float* amax() const { return at<float>(512); }
-  __device__ u32* h_split() const { return at<u32>((u64)a.p[7]); }
-  __device__ u32* w_split() const { return at<u32>((u64)a.p[8]); }
+  __device__ __forceinline__ float cotangent(u64 row) const { return ld1(reinterpret_cast<const float*>(a.in[2]) + row); }
+  template <class X> __device__ __forceinline__ X* scratch(u64 off) const { return reinterpret_cast<X*>(a.scratch + off); }
+  template <class X> __device__ __forceinline__ X* saved(u64 off) const {
+    return reinterpret_cast<X*>((BACK ? a.in[1] : a.p[14] ? (u64)a.p[14] : a.scratch + (u64)a.p[7]) + off);
+  }
+  __device__ __forceinline__ NllScales* scales() const { return saved<NllScales>(0); }
+  __device__ __forceinline__ float* bias2() const { return saved<float>(256); }
+  __device__ __forceinline__ float* lse2() const { return saved<float>((u64)a.p[8]); }
+  __device__ __forceinline__ float* amax() const { return scratch<float>(0); }
+  __device__ __forceinline__ float2* g_scale() const { return scratch<float2>(0); }   // up, down (backward)
 };
 
 __device__ __forceinline__ float finite_abs(float x) {
   const float m = fabsf(x);
-  return m <= 3.402823466e38f ? m : 0.0f;   // an infinity or a NaN does not set the scale
+  return m <= NLL_MAX ? m : 0.0f;   // an infinity or a NaN does not set the scale
 }
 __device__ __forceinline__ float max4(float m, const float4& q) {
   return fmaxf(fmaxf(m, fmaxf(finite_abs(q.x), finite_abs(q.y))), fmaxf(finite_abs(q.z), finite_abs(q.w)));
@@ -89,155 +104,176 @@ __device__ __forceinline__ void load4(float (&x)[4], const float* row, u64 c, u6
   }
 }
 
-// A row-major [rows, n] matrix's hi and lo planes, row pitch n rounded up to 8 (the values between n and
-// the pitch are never read).  use(row) false: the row is written as zeros.
+// A row-major [rows, n] matrix's hi and lo planes, in blocks of 256 columns (a single block is as wide as n,
+// rounded up to 32), zero beyond n up to a multiple of 32.  use(row) false: the row is written as zeros.
 template <class F>
 __device__ __forceinline__ void split_matrix(const float* x, u32* out, u64 rows, u64 n, float up, u64 block, u64 blocks,
                                              F use) {
-  const u64 pitch = (n + 7) / 8 * 8, plane = rows * pitch / 2;
-  const u64 segs = (n + 1023) / 1024;
+  const u64 padded = (n + 31) / 32 * 32, pitch = padded < 256 ? padded : 256;
+  const u64 segs = (padded + 1023) / 1024;
   const bool wide = n % 4 == 0 && (reinterpret_cast<u64>(x) & 15) == 0;
   for (u64 u = block; u < rows * segs; u += blocks) {
     const u64 row = u / segs, c = (u % segs) * 1024 + 4 * threadIdx.x;
-    if (c >= n) continue;
+    if (c >= padded) continue;
     float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     if (use(row)) load4(v, x + row * n, c, n, wide);
     uint2 hi, lo;
     split2(__fmul_rn(v[0], up), __fmul_rn(v[1], up), hi.x, lo.x);
     split2(__fmul_rn(v[2], up), __fmul_rn(v[3], up), hi.y, lo.y);
-    u32* o = out + (row * pitch + c) / 2;
+    u32* o = out + (((c >> 8) * 2 * rows + row) * pitch + (c & 255)) / 2;
     *reinterpret_cast<uint2*>(o) = hi;
-    *reinterpret_cast<uint2*>(o + plane) = lo;
+    *reinterpret_cast<uint2*>(o + rows * pitch / 2) = lo;
   }
 }
 
 }  // namespace tcb
 
-// Largest magnitudes of h (rows that take part), W and, in the backward, the cotangent, a partial per
-// block; the backward's row statistics {lse, g, target} too.
+// The backward has no pass before its first product: a one-off run clears its control block with this (a
+// resident program's is its own, and zero between runs).
+extern "C" __global__ void __launch_bounds__(128) tcb_gemm_prep(const tcb::Args a) {
+  tcb::grid_dependency_sync();
+  tcb::f16_clear(a, tcb::F16_CTRL);
+}
+
+// Largest magnitudes of h (rows that take part) and W, a partial pair per block.
 extern "C" __global__ void __launch_bounds__(256) tcb_nll_amax(const tcb::Args a) {
   using namespace tcb;
   grid_dependency_sync();
-  if (blockIdx.x == 0 && threadIdx.x == 0 && a.p[15]) *reinterpret_cast<u32*>(a.p[15]) = 0u;
+  f16_clear(a, F16_CTRL);
   __shared__ float sh[8];
-  const Nll n(a);
+  const Nll<false> n(a);
   const u64 R = n.R(), d = n.d(), V = n.V();
-  const bool backward = ((u32)a.p[13] & NLL_BACKWARD) != 0;
   const int lane = threadIdx.x & 31;
   const u64 warps = (u64)gridDim.x * 8, gw = (u64)blockIdx.x * 8 + (threadIdx.x >> 5);
-  float mh = 0.0f, mw = 0.0f, mg = 0.0f;
+  float mh = 0.0f, mw = 0.0f;
   const bool wide = d % 4 == 0 && (a.in[0] & 15) == 0;
   for (u64 row = gw; row < R; row += warps) {
-    const int t = n.target(row);
-    if (t >= 0)
-      for (u64 c = 4 * lane; c < d; c += 128) {
-        float x[4];
-        load4(x, n.h() + row * d, c, d, wide);
-        mh = max4(mh, make_float4(x[0], x[1], x[2], x[3]));
-      }
-    if (backward) {
-      float lse = 0.0f, g = 0.0f;
-      if (t >= 0) {
-        g = ld1(reinterpret_cast<const float*>(a.in[NLL_T + 2]) + row);
-        mg = fmaxf(mg, finite_abs(g));
-        double z = 0.0;
-        for (u64 k = lane; k < d; k += 32) z += (double)ld1(n.h() + row * d + k) * (double)ld1(n.w() + k * V + (u64)t);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
-        lse = (float)(z + (double)n.bias((u64)t) + (double)ld1(reinterpret_cast<const float*>(a.in[NLL_T + 1]) + row));
-      }
-      if (lane == 0) n.at<float4>((u64)a.p[9])[row] = make_float4(lse, g, __int_as_float(t), 0.0f);
+    if (n.target(row) < 0) continue;
+    for (u64 c = 4 * lane; c < d; c += 128) {
+      float x[4];
+      load4(x, n.h() + row * d, c, d, wide);
+      mh = max4(mh, make_float4(x[0], x[1], x[2], x[3]));
     }
   }
   const u64 total = d * V, T = (u64)gridDim.x * 256, id = (u64)blockIdx.x * 256 + threadIdx.x;
   const u64 quads = (a.in[1] & 15) == 0 ? total / 4 : 0;
   const float4* w4 = reinterpret_cast<const float4*>(n.w());
-#pragma unroll 4
-  for (u64 i = id; i < quads; i += T) mw = max4(mw, __ldg(w4 + i));
-  for (u64 i = 4 * quads + id; i < total; i += T) mw = fmaxf(mw, finite_abs(ld1(n.w() + i)));
+  u64 i = id;
+  for (; i + 7 * T < quads; i += 8 * T) {   // eight loads in flight
+    float4 q[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) q[k] = __ldg(w4 + i + k * T);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) mw = max4(mw, q[k]);
+  }
+  for (; i < quads; i += T) mw = max4(mw, __ldg(w4 + i));
+  for (i = 4 * quads + id; i < total; i += T) mw = fmaxf(mw, finite_abs(ld1(n.w() + i)));
   mh = block_max(mh, sh);
   mw = block_max(mw, sh);
-  mg = block_max(mg, sh);
   if (threadIdx.x == 0) {
-    float* m = n.amax() + 3 * blockIdx.x;
-    m[0] = mh; m[1] = mw; m[2] = mg;
+    n.amax()[2 * blockIdx.x] = mh;
+    n.amax()[2 * blockIdx.x + 1] = mw;
   }
 }
 
-// The scales from the partial maxima (every block for itself; block 0 writes them down), then h and W split.
+// The scales from the partial maxima (every block for itself; block 0 writes them down), then b log2(e), h
+// and W split.
 extern "C" __global__ void __launch_bounds__(256) tcb_nll_split(const tcb::Args a) {
   using namespace tcb;
   grid_dependency_sync();
   __shared__ float sh[8];
-  const Nll n(a);
-  float mh = 0.0f, mw = 0.0f, mg = 0.0f;
+  const Nll<false> n(a);
+  float mh = 0.0f, mw = 0.0f;
   for (u32 i = threadIdx.x; i < (u32)a.p[0]; i += 256) {
-    const float* m = n.amax() + 3 * i;
-    mh = fmaxf(mh, m[0]); mw = fmaxf(mw, m[1]); mg = fmaxf(mg, m[2]);
+    const float2 m = reinterpret_cast<const float2*>(n.amax())[i];
+    mh = fmaxf(mh, m.x);
+    mw = fmaxf(mw, m.y);
   }
   const int kh = scale_exponent(block_max(mh, sh)), kw = scale_exponent(block_max(mw, sh));
-  const int kg = scale_exponent(block_max(mg, sh));
-  if (blockIdx.x == 0 && threadIdx.x == 0)
-    *n.scales() = NllScales{pow2(kh), pow2(kw), pow2(kg), pow2(-kh), pow2(-kw), pow2(-kg)};
+  if (blockIdx.x == 0 && threadIdx.x == 0)   // the clamp: an accumulator of 0 times inf would be NaN
+    *n.scales() = NllScales{pow2(-kh), pow2(-kw), fminf(pow2(-kh) * pow2(-kw) * NLL_LOG2E, NLL_MAX)};
+  const u64 V = n.V(), padded = (V + 255) / 256 * 256;
+  for (u64 v = (u64)blockIdx.x * 256 + threadIdx.x; v < padded; v += (u64)gridDim.x * 256) {
+    float b = TCB_BIAS && v < V ? ld1(reinterpret_cast<const float*>(a.in[2]) + v) : 0.0f;
+    // a mask of the lowest float stays finite
+    if (fabsf(b) <= NLL_MAX) b = fmaxf(fminf(b * NLL_LOG2E, NLL_MAX), -NLL_MAX);
+    n.bias2()[v] = v < V ? b : TCB_MINUS_INF;
+  }
   // the last blocks take h, about its share of the values
-  const u64 hv = n.R() * n.d(), wv = n.d() * n.V();
+  const u64 hv = n.R() * n.d(), wv = n.d() * V;
   u64 hb = gridDim.x * hv / (hv + wv);
   hb = hb < 1 ? 1 : hb > gridDim.x - 1 ? gridDim.x - 1 : hb;
   const u64 wb = gridDim.x - hb;
   if (blockIdx.x < wb)
-    split_matrix(n.w(), n.w_split(), n.d(), n.V(), pow2(kw), blockIdx.x, wb, [](u64) { return true; });
+    split_matrix(n.w(), n.saved<u32>((u64)a.p[10]), n.d(), V, pow2(kw), blockIdx.x, wb, [](u64) { return true; });
   else
-    split_matrix(n.h(), n.h_split(), n.R(), n.d(), pow2(kh), blockIdx.x - wb, hb,
+    split_matrix(n.h(), n.saved<u32>((u64)a.p[9]), n.R(), n.d(), pow2(kh), blockIdx.x - wb, hb,
                  [&](u64 row) { return n.target(row) >= 0; });
 }
 
 namespace tcb {
 
-// Forward epilogue: a row's maximum and sum of exponentials over the tile's columns, the target's logit.
-// A block of -inf logits (a masked part of the vocabulary) leaves the sum alone.
+// The 32 scaled logits of a block from their sums: 8 loads of the padded bias, the same for every lane.
+__device__ __forceinline__ void nll_logits(float (&v)[32], float z2, const float* bias2) {
+#pragma unroll
+  for (int c = 0; c < 8; ++c) {
+    const float4 b = *reinterpret_cast<const float4*>(bias2 + 4 * c);
+    v[4 * c] = fmaf(v[4 * c], z2, b.x);
+    v[4 * c + 1] = fmaf(v[4 * c + 1], z2, b.y);
+    v[4 * c + 2] = fmaf(v[4 * c + 2], z2, b.z);
+    v[4 * c + 3] = fmaf(v[4 * c + 3], z2, b.w);
+  }
+}
+// The target's place among 32 columns as a bit: comparing an index with each would be turned into an
+// indexed read and keep the sums in local memory.
+__device__ __forceinline__ u32 nll_bit(int t, u32 col) {
+  return t >= (int)col && t < (int)col + 32 ? 1u << (t - (int)col) : 0u;
+}
+
+// Forward epilogue: a row's maximum and sum of exponentials over the half tile's columns, the target's
+// logit.  Columns of -inf (a masked part of the vocabulary, the padding) leave the sum alone.
 template <int BN>
 struct NllForward {
   const Args& a;
-  float dh, dw, m, s;
+  const float* bias2;
+  float z2, m, s;
   int t;
-  __device__ explicit NllForward(const Args& args) : a(args) {}
+  __device__ __forceinline__ explicit NllForward(const Args& args) : a(args) {}
+  __device__ __forceinline__ void start(unsigned char*) {
+    const Nll<false> n(a);
+    z2 = n.scales()->z2;
+    bias2 = n.bias2();
+  }
   __device__ __forceinline__ void begin(const F16Epi& e) {
-    const Nll n(a);
-    dh = n.scales()->down_h;
-    dw = n.scales()->down_w;
-    m = bits(0xff800000u);
+    const Nll<false> n(a);
+    m = TCB_MINUS_INF;
     s = 0.0f;
     t = e.row < n.R() ? n.target(e.row) : -1;
   }
   __device__ __forceinline__ void block(const F16Epi& e, int c0, float (&v)[32]) {
-    const Nll n(a);
     const u32 col = (u32)(e.T.n0 + c0);
-    const int left = (int)((u32)n.V() - col);   // > 0
+    nll_logits(v, z2, bias2 + col);
     float mx = m;
 #pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      v[j] = j < left ? v[j] * dh * dw + n.bias(col + (j < left ? j : 0)) : bits(0xff800000u);
-      mx = fmaxf(mx, v[j]);
-    }
-    // a bit per column, not an index compared: the compiler would turn that into an indexed read of v and
-    // keep the sums in local memory
-    const u32 mine = t >= (int)col && t < (int)col + 32 ? 1u << (t - (int)col) : 0u;
+    for (int j = 0; j < 32; ++j) mx = fmaxf(mx, v[j]);
+    const u32 mine = nll_bit(t, col);
     if (mine) {
       float z = 0.0f;
 #pragma unroll
       for (int j = 0; j < 32; ++j) z = (mine >> j) & 1 ? v[j] : z;
-      n.at<float>((u64)a.p[9])[e.row] = z;
+      Nll<false>(a).template scratch<float>((u64)a.p[11])[e.row] = z;
     }
-    const float safe = mx == bits(0xff800000u) ? 0.0f : mx;
-    float q[4] = {s * expf(m - safe), 0.0f, 0.0f, 0.0f};
+    const float safe = mx == TCB_MINUS_INF ? 0.0f : mx;
+    float q[4] = {s * ex2(m - safe), 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int j = 0; j < 32; ++j) q[j & 3] += expf(v[j] - safe);
+    for (int j = 0; j < 32; ++j) q[j & 3] += ex2(v[j] - safe);
     s = (q[0] + q[1]) + (q[2] + q[3]);
     m = mx;
   }
   __device__ __forceinline__ void end(const F16Epi& e) {
-    const Nll n(a);
-    if (e.row < n.R()) n.at<float2>((u64)a.p[10])[(u64)(e.T.n0 + e.c0) / (BN / 2) * n.R() + e.row] = make_float2(m, s);
+    const Nll<false> n(a);
+    if (e.row < n.R())
+      n.template scratch<float2>((u64)a.p[12])[(u64)(e.T.n0 + e.c0) / (BN / 2) * n.R() + e.row] = make_float2(m, s);
   }
   __device__ __forceinline__ void done(const F16Epi&) {}
 };
@@ -246,40 +282,64 @@ struct NllForward {
 struct NllDz {
   const Args& a;
   const TmaDesc* map;
-  float dh, dw, ug, lse, g;
+  const float* bias2;
+  float z2, up, down, lse, g;
   int t;
-  __device__ NllDz(const GemmParams& P) : a(P.a), map(&P.maps[4]) {}
+  __device__ __forceinline__ explicit NllDz(const GemmParams& P) : a(P.a), map(&P.maps[2]) {}
+  // The cotangent's scale: each CTA's epilogue warps look through all of it behind the first product.
+  __device__ __forceinline__ void start(unsigned char* smem) {
+    const Nll<true> n(a);
+    z2 = n.scales()->z2;
+    bias2 = n.bias2() + (u64)a.p[12];
+    float m = 0.0f;
+    for (u64 i = threadIdx.x - 128; i < n.R(); i += 8 * 256) {   // sixteen loads in flight
+      float x[8];
+      int c[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const u64 r = i + 256 * k;
+        x[k] = r < n.R() ? n.cotangent(r) : 0.0f;
+        c[k] = r < n.R() ? n.target(r) : -1;
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) m = fmaxf(m, c[k] >= 0 ? finite_abs(x[k]) : 0.0f);
+    }
+    m = warp_max(m);
+    float* sh = reinterpret_cast<float*>(smem);
+    if ((threadIdx.x & 31) == 0) sh[threadIdx.x / 32 - 4] = m;
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+#pragma unroll
+    for (int k = 0; k < 8; ++k) m = fmaxf(m, sh[k]);
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    const int k = scale_exponent(m);
+    up = pow2(k);
+    down = pow2(-k);
+    if (blockIdx.x == 0 && threadIdx.x == 128) *n.g_scale() = make_float2(up, down);
+  }
   __device__ __forceinline__ void begin(const F16Epi& e) {
-    const Nll n(a);
-    dh = n.scales()->down_h;
-    dw = n.scales()->down_w;
-    ug = n.scales()->up_g;
-    const float4 s = e.row < n.R() ? n.at<float4>((u64)a.p[9])[e.row]
-                                   : make_float4(0.0f, 0.0f, __int_as_float(-1), 0.0f);
-    lse = s.x;
-    g = s.y;
-    t = __float_as_int(s.z);
+    const Nll<true> n(a);
+    t = e.row < n.R() ? n.target(e.row) : -1;
+    lse = t >= 0 ? n.lse2()[e.row] : 0.0f;
+    g = t >= 0 ? n.cotangent(e.row) * up : 0.0f;
   }
   __device__ __forceinline__ void block(const F16Epi& e, int c0, float (&v)[32]) {
-    const Nll n(a);
+    const Nll<true> n(a);
     const u32 pc = (u32)(e.T.n0 + c0), col = (u32)a.p[12] + pc;
-    const int left = (int)((u32)a.p[1] - pc);
+    nll_logits(v, z2, bias2 + pc);
+    const u32 mine = nll_bit(t, col);
 #pragma unroll
     for (int j = 0; j < 32; ++j) {
-      const float z = v[j] * dh * dw + n.bias(col + (j < left ? j : 0));
-      float p = expf(z - lse);
-      if (t - (int)col == j) p -= 1.0f;
-      v[j] = t >= 0 && j < left ? g * p : 0.0f;
+      const float p = ex2(v[j] - lse);
+      v[j] = g * ((mine >> j) & 1 ? p - 1.0f : p);
     }
-    float c[32];
+    if (t < 0) {   // not by g = 0: an excluded row's logits may be anything
 #pragma unroll
-    for (int j = 0; j < 32; ++j) c[j] = v[j];
-    const float sum = column_sums32(c, e.lane);
-    if (e.lane < left)
-      n.at<float>((u64)a.p[11])[((u64)e.T.m0 / 32 + e.q) * n.V() + col + e.lane] = sum;
-#pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] *= ug;
-    store_split32(e, map, v, (int)pc, e.T.m0 + 32 * e.q, 0, 1);
+      for (int j = 0; j < 32; ++j) v[j] = 0.0f;
+    }
+    store_split32(e, map, v, (int)(pc & 255), e.T.m0 + 32 * e.q, (int)(pc >> 8));
+    const float sum = column_sums32(v, e.lane);
+    if (col + e.lane < (u32)n.V())
+      n.template scratch<float>((u64)a.p[11])[((u64)e.T.m0 / 32 + e.q) * n.V() + col + e.lane] = sum * down;
   }
   __device__ __forceinline__ void end(const F16Epi&) {}
   __device__ __forceinline__ void done(const F16Epi& e) {
@@ -292,23 +352,24 @@ template <bool DW>
 struct NllOut {
   const Args& a;
   float x, y;
-  __device__ explicit NllOut(const Args& args) : a(args) {}
-  __device__ __forceinline__ void begin(const F16Epi&) {
-    const NllScales* s = Nll(a).scales();
-    x = DW ? s->down_h : s->down_w;
-    y = s->down_g;
+  __device__ __forceinline__ explicit NllOut(const Args& args) : a(args) {}
+  __device__ __forceinline__ void start(unsigned char*) {
+    const Nll<true> n(a);
+    x = DW ? n.scales()->down_h : n.scales()->down_w;
+    y = n.g_scale()->y;
   }
+  __device__ __forceinline__ void begin(const F16Epi&) {}
   __device__ __forceinline__ void block(const F16Epi& e, int c0, float (&v)[32]) {
     turn32(e, v);
-    const u32 col = (u32)(e.T.n0 + c0) + e.lane;
-    if (col >= (u32)a.p[1]) return;
+    const u32 M = (u32)a.p[0], N = (u32)((u64)a.p[0] >> 32), col = (u32)(e.T.n0 + c0) + e.lane;
+    if (col >= N) return;
     const u64 ld = DW ? (u64)a.p[6] : (u64)a.p[5];
-    const u64 row0 = (u64)e.T.m0 + 32 * e.q;
+    const u32 row0 = (u32)e.T.m0 + 32 * e.q;
     float* o = reinterpret_cast<float*>(a.out) + row0 * ld + (DW ? (u64)a.p[12] : 0) + col;
-    const int rows = (int)((u64)a.p[0] - row0 < 32 ? (u64)a.p[0] - row0 : 32);
+    const int rows = (int)(M - row0 < 32 ? M - row0 : 32);
 #pragma unroll
     for (int r = 0; r < 32; ++r) v[r] = v[r] * x * y;
-    if (!DW && ((u32)a.p[13] & NLL_ADD)) {
+    if (!DW && a.p[13]) {
 #pragma unroll
       for (int r = 0; r < 32; ++r)
         if (r < rows) v[r] += o[(u64)r * ld];
@@ -323,48 +384,56 @@ struct NllOut {
 
 }  // namespace tcb
 
-#define TCB_NLL_GEMM(NAME, BN, AMN, BMN, EPI, ARG)                                                                    \
+#define TCB_NLL_GEMM(NAME, BN, AMN, BMN, EPI, ARG)                                                                          \
   extern "C" __global__ void __launch_bounds__(tcb::HG_THREADS, 1) NAME##_##BN(const __grid_constant__ tcb::GemmParams P) { \
-    tcb::EPI epi(ARG);                                                                                                \
-    tcb::gemm_f16x3<BN, AMN, BMN, false, 256>(P, epi);                                                                \
+    tcb::EPI epi(ARG);                                                                                                      \
+    tcb::gemm_f16x3<BN, AMN, BMN, false, true, 256>(P, epi);                                                                      \
   }
 // logits and dz: h K-major, W MN-major (its rows run along the vocabulary); dh: dz and W K-major (along the
 // vocabulary); dW: h^T and dz, both MN-major (along d and along the vocabulary)
-#define TCB_NLL_GEMMS(BN)                                          \
+#define TCB_NLL_GEMMS(BN)                                            \
   TCB_NLL_GEMM(tcb_nll_logits, BN, false, true, NllForward<BN>, P.a) \
-  TCB_NLL_GEMM(tcb_nll_dz, BN, false, true, NllDz, P)              \
-  TCB_NLL_GEMM(tcb_nll_dh, BN, false, false, NllOut<false>, P.a)   \
+  TCB_NLL_GEMM(tcb_nll_dz, BN, false, true, NllDz, P)                \
+  TCB_NLL_GEMM(tcb_nll_dh, BN, false, false, NllOut<false>, P.a)     \
   TCB_NLL_GEMM(tcb_nll_dw, BN, true, true, NllOut<true>, P.a)
 TCB_NLL_GEMMS(256)
 TCB_NLL_GEMMS(128)
 TCB_NLL_GEMMS(64)
 
-// Joins a row's tiles: a block of 8 warps takes 32 rows, warp k the tiles k, k + 8, ...
+// Joins a row's tiles: a block of 8 warps takes 32 rows, warp k the half tiles k, k + 8, ...
 extern "C" __global__ void __launch_bounds__(256) tcb_nll_finish(const tcb::Args a) {
   using namespace tcb;
   grid_dependency_sync();
   __shared__ float2 sh[8][32];
-  const Nll n(a);
+  const Nll<false> n(a);
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const u64 R = n.R(), row = (u64)blockIdx.x * 32 + lane;
   const u32 tiles = (u32)a.p[0];
-  const float2* part = n.at<float2>((u64)a.p[10]);
-  float m = bits(0xff800000u), s = 0.0f;
+  const float2* part = n.scratch<float2>((u64)a.p[12]);
+  float m = TCB_MINUS_INF, s = 0.0f;
   auto join = [&](const float2& x) {
-    const float mx = fmaxf(m, x.x), safe = mx == bits(0xff800000u) ? 0.0f : mx;
-    s = s * expf(m - safe) + x.y * expf(x.x - safe);
+    const float mx = fmaxf(m, x.x), safe = mx == TCB_MINUS_INF ? 0.0f : mx;
+    s = s * ex2(m - safe) + x.y * ex2(x.x - safe);
     m = mx;
   };
   if (row < R) {
-#pragma unroll 4
-    for (u32 k = w; k < tiles; k += 8) join(part[(u64)k * R + row]);
+    u32 k = w;
+    for (; k + 56 < tiles; k += 64) {   // eight loads in flight
+      float2 x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = part[(u64)(k + 8 * i) * R + row];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) join(x[i]);
+    }
+    for (; k < tiles; k += 8) join(part[(u64)k * R + row]);
   }
   sh[w][lane] = make_float2(m, s);
   __syncthreads();
   if (w == 0 && row < R) {
     for (int k = 1; k < 8; ++k) join(sh[k][lane]);
-    reinterpret_cast<float*>(a.out)[row] =
-        n.target(row) >= 0 ? (m - n.at<float>((u64)a.p[9])[row]) + logf(s) : 0.0f;
+    const bool in = n.target(row) >= 0;
+    reinterpret_cast<float*>(a.out)[row] = in ? (m - n.scratch<float>((u64)a.p[11])[row]) * NLL_LN2 + logf(s) : 0.0f;
+    n.lse2()[row] = m + log2f(s);
   }
 }
 
@@ -373,10 +442,10 @@ extern "C" __global__ void __launch_bounds__(256) tcb_nll_db(const tcb::Args a) 
   using namespace tcb;
   grid_dependency_sync();
   __shared__ float sh[8][32];
-  const Nll n(a);
+  const Nll<true> n(a);
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const u64 V = n.V(), parts = (n.R() + 31) / 32, col = (u64)blockIdx.x * 32 + lane;
-  const float* p = n.at<float>((u64)a.p[11]);
+  const float* p = n.scratch<float>((u64)a.p[11]);
   float s = 0.0f;
   if (col < V) {
 #pragma unroll 4

@@ -14,34 +14,38 @@
 // Chains of 128: a step passes the drift of its products on several times over (against 64 bits, a stack
 // of 256 x 1024: 4.7e-6 with 256, 2.9e-6 with 128, 1.8e-6 with 64; 4096 x 4096: 3.63, 3.84, 4.16 ms).
 //
-// p[]: [0..3] M, N, K, batch of the product; [4] m, [5] n; [6] X to read, [7] X to write, [8] S, [9] P:
-// byte offsets in scratch; [10] 1 when the step writes the float32 result.
+// p[]: [0..3] the product's (split: [0] partial sums of a matrix); [4] m, [5] n; [6] X to read, [7] X to write,
+// [8] S, [9] P: byte offsets in scratch; [10] 1 when the step writes the float32 result.
 #pragma once
 #include "tcb/gemm_f16x3.cuh"
 
 namespace tcb {
 
-constexpr u32 NS_PARTS = 64;   // partial sums of squares a matrix
+constexpr u32 NS_PARTS = 512;   // most partial sums of squares a matrix
 
 struct Ns {
   const Args& a;
   __device__ explicit Ns(const Args& args) : a(args) {}
   __device__ u64 m() const { return (u64)a.p[4]; }
   __device__ u64 n() const { return (u64)a.p[5]; }
-  __device__ double* parts() const { return reinterpret_cast<double*>(a.scratch + 512); }
+  __device__ double* parts() const { return reinterpret_cast<double*>(a.scratch); }
 };
 
-// 32 values of an fp16 pair array at (row, col), scaled by `down`; columns at or beyond the pitch are 0.
+// 32 values of an fp16 pair array at (row, col), scaled by `down`.  Beyond the pitch the last 8 columns are
+// read again (nothing uses those values): a branch around each load would have them wait one for another.
 __device__ __forceinline__ void load_split32(float (&x)[32], const unsigned char* plane, u64 plane_bytes, u64 pitch,
                                              u64 row, u32 col, float down) {
-  const unsigned char* p = plane + (row * pitch + col) * 2;
+  const unsigned char* p = plane + row * pitch * 2;
+  uint4 hq[4], lq[4];
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
-    uint4 h = make_uint4(0, 0, 0, 0), l = h;
-    if (col + 8 * c < pitch) {
-      h = *reinterpret_cast<const uint4*>(p + 16 * c);
-      l = *reinterpret_cast<const uint4*>(p + plane_bytes + 16 * c);
-    }
+    const u32 at = 2 * (col + 8 * c < (u32)pitch ? col + 8 * c : (u32)pitch - 8);
+    hq[c] = *reinterpret_cast<const uint4*>(p + at);
+    lq[c] = *reinterpret_cast<const uint4*>(p + plane_bytes + at);
+  }
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const uint4 h = hq[c], l = lq[c];
     const u32 hs[4] = {h.x, h.y, h.z, h.w}, ls[4] = {l.x, l.y, l.z, l.w};
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -56,11 +60,11 @@ __device__ __forceinline__ void load_split32(float (&x)[32], const unsigned char
 
 }  // namespace tcb
 
-// Sums of squares in double (no float32 square can overflow it), NS_PARTS partials a matrix.
+// Sums of squares in double (no float32 square can overflow it), a partial per block of a matrix.
 extern "C" __global__ void __launch_bounds__(256) tcb_orth_norm(const tcb::Args a) {
   using namespace tcb;
   grid_dependency_sync();
-  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0 && a.p[15]) *reinterpret_cast<u32*>(a.p[15]) = 0u;
+  f16_clear(a, F16_CTRL);
   __shared__ double sh[8];
   const Ns s(a);
   const u64 count = s.m() * s.n();
@@ -80,7 +84,7 @@ extern "C" __global__ void __launch_bounds__(256) tcb_orth_norm(const tcb::Args 
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int k = 1; k < 8; ++k) acc += sh[k];
-    s.parts()[blockIdx.y * NS_PARTS + blockIdx.x] = acc;
+    s.parts()[(u64)blockIdx.y * gridDim.x + blockIdx.x] = acc;
   }
 }
 
@@ -90,18 +94,22 @@ extern "C" __global__ void __launch_bounds__(256) tcb_orth_split(const tcb::Args
   grid_dependency_sync();
   const Ns s(a);
   const u64 m = s.m(), n = s.n(), pitch = (n + 7) / 8 * 8, b = blockIdx.y;
-  static_assert(NS_PARTS == 64, "two warps load a partial each lane");
-  __shared__ double sh[2];
-  double sum = threadIdx.x < (u32)a.p[0] ? s.parts()[b * NS_PARTS + threadIdx.x] : 0.0;
+  __shared__ double sh[8];
+  static_assert(NS_PARTS == 512, "a thread loads two partials");
+  const u32 parts = (u32)a.p[0];
+  const double* part = s.parts() + b * parts;
+  double sum = (threadIdx.x < parts ? part[threadIdx.x] : 0.0) + (threadIdx.x + 256 < parts ? part[threadIdx.x + 256] : 0.0);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (threadIdx.x == 0 || threadIdx.x == 32) sh[threadIdx.x >> 5] = sum;
+  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = sum;
   __syncthreads();
-  sum = sh[0] + sh[1];
+  sum = 0.0;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) sum += sh[k];
   const double inv = 1.0 / (sqrt(sum) + (double)(TCB_NS_EPS)) * (double)(1u << TCB_EX);
   const float* x = reinterpret_cast<const float*>(a.in[0]) + b * m * n;
-  u32* out = reinterpret_cast<u32*>(a.scratch + (u64)a.p[6]) + b * m * pitch / 2;
-  const u64 plane = (u64)gridDim.y * m * pitch / 2, segs = (n + 1023) / 1024;
+  u32* out = reinterpret_cast<u32*>(a.scratch + (u64)a.p[6]) + b * m * pitch;
+  const u64 plane = m * pitch / 2, segs = (n + 1023) / 1024;
   const bool wide = n % 4 == 0 && (reinterpret_cast<u64>(x) & 15) == 0;
   for (u64 u = blockIdx.x; u < m * segs; u += gridDim.x) {
     const u64 row = u / segs, c = (u % segs) * 1024 + 4 * threadIdx.x;
@@ -128,21 +136,21 @@ extern "C" __global__ void __launch_bounds__(256) tcb_orth_split(const tcb::Args
 namespace tcb {
 
 // S, or P = b S + c S S: written where computed and, when the tile across the diagonal is not computed,
-// mirrored there (lanes hold consecutive rows, which are consecutive columns of the mirror).
+// mirrored there.
 template <int BN, bool POLY>
 struct NsSymmetric {
   const Args& a;
   const TmaDesc* map;
-  __device__ explicit NsSymmetric(const GemmParams& P) : a(P.a), map(&P.maps[4]) {}
+  __device__ explicit NsSymmetric(const GemmParams& P) : a(P.a), map(&P.maps[2]) {}
+  __device__ __forceinline__ void start(unsigned char*) {}
   __device__ __forceinline__ void begin(const F16Epi&) {}
   __device__ __forceinline__ void block(const F16Epi& e, int c0, float (&v)[32]) {
-    const u64 M = (u64)a.p[0], pitch = (M + 7) / 8 * 8, batch = (u64)a.p[3];
-    const u64 plane = batch * M * pitch * 2;
+    const u64 M = (u32)a.p[0], pitch = (M + 7) / 8 * 8, plane = M * pitch * 2;   // bytes of a plane
     const u32 col = (u32)(e.T.n0 + c0);
     if (POLY) {
       float s[32];
       const u64 row = e.row < M ? e.row : M - 1;
-      load_split32(s, reinterpret_cast<const unsigned char*>(a.scratch + (u64)a.p[8]) + (u64)e.T.bz * M * pitch * 2, plane,
+      load_split32(s, reinterpret_cast<const unsigned char*>(a.scratch + (u64)a.p[8]) + (u64)e.T.bz * 2 * plane, plane,
                    pitch, row, col, pow2(TCB_EP - TCB_ES));
       const float up = pow2(TCB_EP - 2 * TCB_ES);
 #pragma unroll
@@ -152,22 +160,12 @@ struct NsSymmetric {
 #pragma unroll
       for (int j = 0; j < 32; ++j) v[j] *= up;
     }
-    store_split32(e, map, v, (int)col, e.T.m0 + 32 * e.q, e.T.bz, (int)batch + e.T.bz);
-    const u32 rb = col / HG_M;   // the mirror's tile row
-    if (((u32)e.T.m0 + 32 * e.q) / BN < rb * HG_M / BN && e.row < M) {
-      unsigned short* o = reinterpret_cast<unsigned short*>(a.scratch + (u64)a.p[POLY ? 9 : 8]) + (u64)e.T.bz * M * pitch + e.row;
-#pragma unroll
-      for (int j = 0; j < 32; j += 2) {
-        u32 hi, lo;
-        split2(v[j], v[j + 1], hi, lo);
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-          if (col + j + k < M) {
-            unsigned short* p = o + (u64)(col + j + k) * pitch;
-            p[0] = (unsigned short)(k ? hi >> 16 : hi);
-            p[plane / 2] = (unsigned short)(k ? lo >> 16 : lo);
-          }
-      }
+    store_split32(e, map, v, (int)col, e.T.m0 + 32 * e.q, e.T.bz);
+    const u32 row0 = (u32)e.T.m0 + 32 * e.q;
+    if (row0 / BN < col / HG_M * HG_M / BN) {   // the mirror's tile is not computed
+      if (e.lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+      turn32(e, v);   // lane l: row l of the mirrored block
+      store_split32(e, map, v, (int)row0, (int)col, e.T.bz);
     }
   }
   __device__ __forceinline__ void end(const F16Epi&) {}
@@ -180,20 +178,21 @@ struct NsSymmetric {
 struct NsApply {
   const Args& a;
   const TmaDesc* map;
-  __device__ explicit NsApply(const GemmParams& P) : a(P.a), map(&P.maps[4]) {}
+  __device__ explicit NsApply(const GemmParams& P) : a(P.a), map(&P.maps[2]) {}
+  __device__ __forceinline__ void start(unsigned char*) {}
   __device__ __forceinline__ void begin(const F16Epi&) {}
   __device__ __forceinline__ void block(const F16Epi& e, int c0, float (&v)[32]) {
-    const u64 m = (u64)a.p[4], n = (u64)a.p[5], pitch = (n + 7) / 8 * 8, batch = (u64)a.p[3];
+    const u64 m = (u64)a.p[4], n = (u64)a.p[5], pitch = (n + 7) / 8 * 8, plane = m * pitch * 2;
     const u32 col = (u32)(e.T.n0 + c0);
     const bool last = a.p[10] != 0;
     float x[32];
-    load_split32(x, reinterpret_cast<const unsigned char*>(a.scratch + (u64)a.p[6]) + (u64)e.T.bz * m * pitch * 2,
-                 batch * m * pitch * 2, pitch, e.row < m ? e.row : m - 1, col, last ? pow2(-TCB_EX) : 1.0f);
+    load_split32(x, reinterpret_cast<const unsigned char*>(a.scratch + (u64)a.p[6]) + (u64)e.T.bz * 2 * plane, plane, pitch,
+                 e.row < m ? e.row : m - 1, col, last ? pow2(-TCB_EX) : 1.0f);
     const float up = last ? pow2(-TCB_EP - TCB_EX) : pow2(-TCB_EP);
 #pragma unroll
     for (int j = 0; j < 32; ++j) v[j] = fmaf(TCB_NS_A, x[j], v[j] * up);
     if (!last) {
-      store_split32(e, map, v, (int)col, e.T.m0 + 32 * e.q, e.T.bz, (int)batch + e.T.bz);
+      store_split32(e, map, v, (int)col, e.T.m0 + 32 * e.q, e.T.bz);
       return;
     }
     turn32(e, v);
@@ -216,7 +215,7 @@ struct NsApply {
 #define TCB_NS_GEMM(NAME, BN, AMN, BMN, SYM, EPI)                                                                         \
   extern "C" __global__ void __launch_bounds__(tcb::HG_THREADS, 1) NAME##_##BN(const __grid_constant__ tcb::GemmParams P) { \
     tcb::EPI epi(P);                                                                                                      \
-    tcb::gemm_f16x3<BN, AMN, BMN, SYM, 128>(P, epi);                                                                      \
+    tcb::gemm_f16x3<BN, AMN, BMN, SYM, false, 128>(P, epi);                                                                      \
   }
 #define TCB_NS_S(BN) NsSymmetric<BN, false>
 #define TCB_NS_P(BN) NsSymmetric<BN, true>

@@ -152,14 +152,39 @@ def _number(v):
     return isinstance(v, (int, float)) and not isinstance(v, bool) and math.isfinite(v)
 
 
+def linear_nll_saved(R, d, V):
+    """The value linearNll saves for its backward: byte offsets of its parts (the scales at 0, the scaled bias
+    at 256) and its size in floats.  h and W are held as fp16 pairs in blocks of 256 columns."""
+    def up(n, k):
+        return -(-n // k) * k
+
+    def blocked(n):
+        return up(n, 32) if n <= 256 else up(n, 256)
+    lse = up(256 + 4 * up(V, 256), 256)
+    h = up(lse + 4 * R, 256)
+    w = up(h + 4 * R * blocked(d), 256)
+    return {"lse": lse, "h": h, "w": w}, up(w + 4 * d * blocked(V), 256) // 4
+
+
 def _infer_nll(op, shapes, attrs):
     bias = attrs.get("bias")
     if not isinstance(bias, bool):
         raise ShapeError(f"{op}: bias must be true or false")
-    back = op == "linearNllGrad"
-    want = 3 + bias + 2 * back
-    if len(shapes) != want:
-        raise ShapeError(f"{op}: takes {want} inputs, got {len(shapes)}")
+    if op == "linearNllGrad":   # of the targets, the saved value, the loss's cotangent
+        if len(shapes) != 3:
+            raise ShapeError(f"{op}: takes 3 inputs, got {len(shapes)}")
+        d, V, wrt = attrs.get("d"), attrs.get("V"), attrs.get("wrt")
+        if not _is_int(d) or not _is_int(V) or d < 1 or not 1 <= V <= MAX_CLASSES:
+            raise ShapeError(f"{op}: d and V must be the weight's sizes, got {d!r} and {V!r}")
+        t, saved, gy = shapes
+        if len(t) != 1 or list(gy) != list(t) or list(saved) != [linear_nll_saved(t[0], d, V)[1]]:
+            raise ShapeError(f"{op}: targets {fmt(t)}, saved value {fmt(saved)} and cotangent {fmt(gy)} do not belong "
+                             f"to a weight [{d},{V}]")
+        if wrt not in ("h", "w", "b") or (wrt == "b" and not bias):
+            raise ShapeError(f"{op}: no gradient with respect to {wrt!r}")
+        return [t[0], d] if wrt == "h" else [d, V] if wrt == "w" else [V]
+    if len(shapes) != 3 + bias:
+        raise ShapeError(f"{op}: takes {3 + bias} inputs, got {len(shapes)}")
     h, w = shapes[0], shapes[1]
     if len(h) != 2 or len(w) != 2 or h[1] != w[0]:
         raise ShapeError(f"{op}: rows {fmt(h)} and weight {fmt(w)} must be [R,d] and [d,V]")
@@ -167,15 +192,12 @@ def _infer_nll(op, shapes, attrs):
         raise ShapeError(f"{op}: {w[1]} classes, at most {MAX_CLASSES} (a class index is a float32)")
     if bias and list(shapes[2]) != [w[1]]:
         raise ShapeError(f"{op}: bias {fmt(shapes[2])} for {w[1]} classes")
-    for what, s in zip(("targets", "loss", "cotangent"), shapes[2 + bias:]):
-        if list(s) != [h[0]]:
-            raise ShapeError(f"{op}: {what} {fmt(s)} for {h[0]} rows")
-    if not back:
-        return [h[0]]
-    wrt = attrs.get("wrt")
-    if wrt not in ("h", "w", "b") or (wrt == "b" and not bias):
-        raise ShapeError(f"{op}: no gradient with respect to {wrt!r}")
-    return list(h) if wrt == "h" else list(w) if wrt == "w" else [w[1]]
+    if list(shapes[-1]) != [h[0]]:
+        raise ShapeError(f"{op}: targets {fmt(shapes[-1])} for {h[0]} rows")
+    out = attrs.get("out")
+    if out not in ("loss", "saved"):
+        raise ShapeError(f"{op}: out must be 'loss' or 'saved', got {out!r}")
+    return [h[0]] if out == "loss" else [linear_nll_saved(h[0], w[0], w[1])[1]]
 
 
 def _infer_head(op, shapes, attrs):
@@ -418,7 +440,7 @@ class Graph:
         A row whose target is not in 0 .. V-1 (-1, say, for padding) has loss 0 and no gradient, and
         nothing of its row of h is used.  Gradients: h, w and bias."""
         ins = [h, w] + ([] if bias is None else [bias]) + [targets]
-        return self.emit("linearNll", ins, {"bias": bias is not None})
+        return self.emit("linearNll", ins, {"bias": bias is not None, "out": "loss"})
 
     def head_norm_rope(self, x, gain, pos, base=10000.0, eps=1e-6, rotary=None, interleaved=False,
                        heads_first=True):

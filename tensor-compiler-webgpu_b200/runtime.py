@@ -234,7 +234,8 @@ class Module:
 
 def _map_desc(call, scratch, ins=(), out=0):
     """The 8-value tensor-map descriptors of a call (include/tcb200.h, tc_launch_tma): each map is over
-    scratch (at an offset), one of the launch's operands ('in', operand index) or its output ('out')."""
+    scratch (at an offset), one of the launch's operands ('in', operand index; 'in_at', byte offset << 3 |
+    operand index) or its output ('out')."""
     vals = []
     for region, off, cols, rows, batches, rs, bs, bc, br in call.tma:
         if region == "scratch":
@@ -243,6 +244,8 @@ def _map_desc(call, scratch, ins=(), out=0):
             addr = ins[off]
         elif region == "out":
             addr = out + off
+        elif region == "in_at":
+            addr = ins[off & 7] + (off >> 3)
         elif region == "abs":
             addr = off
         else:

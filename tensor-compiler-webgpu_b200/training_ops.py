@@ -4,24 +4,27 @@
 * ``headNormRope`` / ``headNormRopeGrad`` -- tcb/head_norm_rope.cuh
 * ``orthogonalize``                       -- tcb/orthogonalize.cuh
 
-Each node is one launch of a few kernel calls; the gradients of one node (its ``...Grad`` siblings, which
-differ in ``wrt`` only) are one launch with several outputs.  Sizes are run-time parameters, so one module
+Each node is one launch of a few kernel calls.  Siblings -- the gradients of one node, which differ in
+``wrt`` only; a loss and what it saves for its backward, which differ in ``out`` -- are one launch with several
+outputs.  Sizes are run-time parameters, so one module
 serves every shape of an operator and only tile widths, a head's layout and Newton-Schulz coefficients are
 compiled in.  The library's own lowering (csrc/lower.cpp) makes the same records.
 """
 from __future__ import annotations
 
 import math
+import os
 import struct
 
-from .ir import TRAINING_OPS, newton_schulz_scales, size
+from .ir import TRAINING_OPS, linear_nll_saved, newton_schulz_scales, size
 
 SM_COUNT = 148
-F16 = 1 << 33          # box_cols flag of a tensor map: 16-bit elements
+F16 = 1 << 33          # box_cols flags of a tensor map: 16-bit elements,
+PAIR = 1 << 34         # two planes (hi and lo) a box
 F16_BM, F16_BK = 128, 32
-SCALES_AT, AMAX_AT = 0, 512      # byte offsets in scratch
-AMAX_BLOCKS = 2 * SM_COUNT
-DZ_BYTES = 256 << 20             # bound of one vocabulary piece's dz
+AMAX_BLOCKS = 4 * SM_COUNT
+DZ_BYTES = int(os.environ.get('DZ','256')) << 20             # bound of one vocabulary piece's dz
+CTRL_BYTES = 4 * (4 + 8 * 2 * SM_COUNT)   # error word, and a counter per epilogue warp of a divided tile
 
 
 def _up(n, k):
@@ -39,46 +42,107 @@ def f16_smem(bn):
     return stages * stage + 1024 + 32768 + 1024
 
 
-def f16_bn(M, N, batch=1):
-    """Tile width of a split-fp16 product: the widest whose tiles cover the SMs, down to 64."""
+def f16_bn(M, N, K, batch=1):
+    """Tile width of a split-fp16 product: the widest that leaves every SM about two chains of 256 K indices
+    (tiles can be divided along K), down to 64."""
+    if os.environ.get('BNF'):
+        return int(os.environ['BNF'])
     for bn in (256, 128):
-        if N > bn // 2 and batch * math.ceil(M / F16_BM) * math.ceil(N / bn) >= SM_COUNT // 2:
+        if N > bn // 2 and batch * math.ceil(M / F16_BM) * math.ceil(N / bn) * math.ceil(K / 256) >= 2 * SM_COUNT:
             return bn
     return 64
 
 
-def _symmetric_tiles(n, bn):
-    tn = math.ceil(n / bn)
-    return sum(tn - i * F16_BM // bn for i in range(math.ceil(n / F16_BM)))
+def f16_tiles(M, N, bn, symmetric):
+    tm, tn = math.ceil(M / F16_BM), math.ceil(N / bn)
+    return sum(tn - i * F16_BM // bn for i in range(tm)) if symmetric else tm * tn
 
 
-def _operand(off, plane, cols, rows, batch, pitch, mn, bn):
-    """The maps of an operand's hi and lo planes: boxes of 64 x F16_BK when its M or N index runs along
-    the rows, else of F16_BK x (128 or the tile width)."""
-    box = (64 | F16, F16_BK) if mn else (F16_BK | F16, bn)
-    return [("scratch", off + p * plane, cols, rows, batch, pitch * 2, rows_stride, *box)
-            for p, rows_stride in ((0, rows * pitch * 2), (1, rows * pitch * 2))]
+QUANTUM = int(os.environ.get('Q', '1'))
 
 
-def _gemm(name, M, N, K, batch, bn, maps, params, tiles=None):
+def f16_plan(tiles, K, chunk, bn):
+    """(grid, whole tiles, quantum) of a product of `tiles` output tiles (tcb/gemm_f16x3.cuh).
+
+    The tiles beyond the whole waves are divided along K where that saves more than their partial sums
+    cost: about three chains of 256 a CTA.  A CTA's run is then more than a tile and cut anywhere; with
+    fewer tiles than SMs a piece is at least `quantum` chains, longer for narrow tiles, whose chains are
+    short beside the exchange."""
+    chunks = math.ceil(K / chunk)
+    if os.environ.get('WH'):
+        return min(SM_COUNT, tiles), tiles, 1
+    if tiles >= SM_COUNT:
+        idle = -tiles % SM_COUNT
+        if idle * chunks * chunk <= 3 * 256 * SM_COUNT:
+            return SM_COUNT, tiles, 1
+        return SM_COUNT, tiles - tiles % SM_COUNT - SM_COUNT, 1
+    quantum = QUANTUM * (256 // chunk)
+    per = math.ceil(chunks / quantum)
+    if per == 1:
+        return tiles, tiles, 1
+    return min(SM_COUNT, tiles * per), 0, quantum
+
+
+def f16_partial_bytes(grid, whole, tiles, bn):
+    return 0 if whole == tiles else 2 * grid * F16_BM * bn * 4
+
+
+def _operand(off, plane, cols, rows, batch, pitch, mn, bn, region="scratch"):
+    """The map of an operand's hi and lo planes, one behind the other for each matrix: boxes of 64 x F16_BK when
+    its M or N index runs along the rows, else of F16_BK x (128 or the tile width)."""
+    box = (64 | F16 | PAIR, F16_BK) if mn else (F16_BK | F16 | PAIR, bn)
+    assert plane == batch * rows * pitch * 2
+    return [(region, off, cols, rows, 2 * batch, pitch * 2, rows * pitch * 2, *box)]
+
+
+def _blocked(region, off, rows, cols, pitch, box_cols, box_rows):
+    """The map of a matrix stored in blocks of 256 columns (rows of `pitch`), hi and lo planes of a block side
+    by side."""
+    return [(region, off, pitch, rows, 2 * math.ceil(cols / 256), pitch * 2, rows * pitch * 2, box_cols | F16 | PAIR, box_rows)]
+
+
+def _pitch(cols):
+    return min(256, _up(cols, 32))
+
+
+def _blocked_operand(region, off, rows, cols, pitch, mn, bn):
+    return _blocked(region, off, rows, cols, pitch, *((64, F16_BK) if mn else (F16_BK, bn)))
+
+
+def _at(index, off):
+    """A tensor map's place in a launch operand, `off` bytes in (region 'in_at')."""
+    return off << 3 | index
+
+
+def _gemm(name, M, N, K, batch, bn, chunk, part_at, maps, params, symmetric=False):
     from .codegen import KernelCall
-    tiles = batch * math.ceil(M / F16_BM) * math.ceil(N / bn) if tiles is None else tiles
+    tiles = batch * f16_tiles(M, N, bn, symmetric)
     if tiles >= 1 << 31:
         raise ValueError(f"{name}: {tiles} tiles")
-    c = KernelCall(f"{name}_{bn}", (min(SM_COUNT, tiles), 1, 1), (384, 1, 1), f16_smem(bn), [M, N, K, batch, *params])
+    grid, whole, quantum = f16_plan(tiles, K, chunk, bn)
+    c = KernelCall(f"{name}_{bn}", (grid, 1, 1), (384, 1, 1), f16_smem(bn),
+                   [M | N << 32, K | batch << 32, whole | quantum << 32, part_at, *params])
     c.tma = maps
-    return c
+    return c, f16_partial_bytes(grid, whole, tiles, bn)
 
 
 def siblings(graph):
-    """{node id: [node ids]} of every ...Grad node: the gradients of one node, by operands and attributes."""
+    """{node id: [node ids]}: the outputs of one launch, nodes that differ in which output they are only."""
     groups, out = {}, {}
     for n in graph.nodes:
-        if n.op.endswith("Grad") and n.op in TRAINING_OPS:
-            key = (n.op, tuple(n.inputs), repr(sorted((k, v) for k, v in n.attrs.items() if k != "wrt")))
-            groups.setdefault(key, []).append(n.id)
-            out[n.id] = groups[key]
-    return out
+        which = n.attrs.get("wrt", n.attrs.get("out")) if n.op in TRAINING_OPS else None
+        if which is None:
+            continue
+        key = (n.op, tuple(n.inputs), repr(sorted((k, v) for k, v in n.attrs.items() if k not in ("wrt", "out"))))
+        for g in groups.setdefault(key, []):
+            if which not in g:
+                break
+        else:
+            g = {}
+            groups[key].append(g)
+        g[which] = n.id
+        out[n.id] = g
+    return {i: list(g.values()) for i, g in out.items()}
 
 
 # ------------------------------------------------------------------ linearNll
@@ -87,25 +151,8 @@ def nll_pieces(R, V):
     the pieces of about one size."""
     most = max(256, DZ_BYTES // (4 * R) // 256 * 256)
     n = math.ceil(V / most)
-    wide = min(_up(math.ceil(V / n), 256), _up(V, 8))
+    wide = min(_up(math.ceil(V / n), 256), _up(V, 32))
     return wide, math.ceil(V / wide)
-
-
-def nll_layout(R, d, V, backward):
-    dp, vp = _up(d, 8), _up(V, 8)
-    bz = f16_bn(R, nll_pieces(R, V)[0] if backward else V)
-    at, off = {}, _up(AMAX_AT + 12 * AMAX_BLOCKS, 256) + 256
-    at["err"] = off - 256
-    piece, _ = nll_pieces(R, V)
-    parts = [("h", 4 * R * dp), ("w", 4 * d * vp)]
-    if backward:
-        parts += [("stat", 16 * R), ("dz", 4 * R * piece), ("db", 4 * math.ceil(R / 32) * V)]
-    else:
-        parts += [("stat", 4 * R), ("part", 8 * R * math.ceil(V / (bz // 2)))]
-    for name, nbytes in parts:
-        at[name] = off
-        off += _up(nbytes, 256)
-    return at, off, bz
 
 
 def nll_source(bias):
@@ -116,75 +163,105 @@ def nll_source(bias):
 """
 
 
-def _nll_prep(R, d, V, at, flags):
-    """The scale and split passes both directions begin with."""
-    from .codegen import KernelCall
-    tail = [R, d, V, at["h"], at["w"], at["stat"], at.get("part", at.get("dz")), at.get("db", 0), 0, flags]
-    amax = KernelCall("tcb_nll_amax", (AMAX_BLOCKS, 1, 1), (256, 1, 1), 0, [AMAX_BLOCKS, 0, 0, 0, *tail])
-    amax.err_offset = at["err"]
-    units = d * math.ceil(V / 1024) + R * math.ceil(d / 1024)
-    split = KernelCall("tcb_nll_split", (max(2, min(units, SM_COUNT * 8)), 1, 1), (256, 1, 1), 0,
-                       [AMAX_BLOCKS, 0, 0, 0, *tail])
-    return [amax, split], tail
+def _regions(*parts):
+    """{name: byte offset} of scratch regions one behind the other, and their end."""
+    at, off = {}, 0
+    for name, nbytes in parts:
+        at[name] = off
+        off += _up(nbytes, 256)
+    return at, off
 
 
-def _nll_launch(graph, node):
+def _nll_launch(graph, ids):
     from .codegen import KernelCall, Launch
+    by = {graph.nodes[i].attrs["out"]: i for i in ids}
+    node = graph.nodes[ids[0]]
     (R, d), V = graph.nodes[node.inputs[0]].shape, graph.nodes[node.inputs[1]].shape[1]
-    dp, vp = _up(d, 8), _up(V, 8)
-    at, scratch, bz = nll_layout(R, d, V, False)
-    calls, tail = _nll_prep(R, d, V, at, 0)
-    maps = (_operand(at["h"], 2 * R * dp, d, R, 1, dp, False, F16_BM) +
-            _operand(at["w"], 2 * d * vp, V, d, 1, vp, True, bz))
-    gemm = _gemm("tcb_nll_logits", R, V, d, 1, bz, maps, tail)
-    gemm.err_offset = at["err"]
-    calls.append(gemm)
-    calls.append(KernelCall("tcb_nll_finish", (math.ceil(R / 32), 1, 1), (256, 1, 1), 0,
-                            [math.ceil(V / (bz // 2)), 0, 0, 0, *tail]))
+    inner, floats = linear_nll_saved(R, d, V)
+    bn = f16_bn(R, V, d)
+    halves = math.ceil(V / (bn // 2))
+    at, end = _regions(("amax", 8 * AMAX_BLOCKS), ("err", CTRL_BYTES), ("zt", 4 * R), ("part", 8 * R * halves),
+                       ("loss", 0 if "loss" in by else 4 * R), ("saved", 0 if "saved" in by else 4 * floats))
+    tail = [R, d, V, at["saved"], inner["lse"], inner["h"], inner["w"], at["zt"], at["part"], 0]
+    if "saved" in by:
+        def saved(off):
+            return "out", off
+    else:
+        def saved(off):
+            return "scratch", at["saved"] + off
+    maps = (_blocked_operand(*saved(inner["h"]), R, d, _pitch(d), False, F16_BM) +
+            _blocked_operand(*saved(inner["w"]), d, V, _pitch(V), True, bn))
+    blocks = max(1, min(AMAX_BLOCKS, math.ceil((R * d + d * V) / 2048)))
+    units = d * math.ceil(V / 1024) + R * math.ceil(d / 1024)
+    gemm, partial = _gemm("tcb_nll_logits", R, V, d, 1, bn, 256, end, maps, tail)
+    calls = [KernelCall("tcb_nll_amax", (blocks, 1, 1), (256, 1, 1), 0, [blocks, 0, 0, 0, *tail]),
+             KernelCall("tcb_nll_split", (max(2, min(units, SM_COUNT * 8)), 1, 1), (256, 1, 1), 0, [blocks, 0, 0, 0, *tail]),
+             gemm, KernelCall("tcb_nll_finish", (math.ceil(R / 32), 1, 1), (256, 1, 1), 0, [halves, 0, 0, 0, *tail])]
+    calls[0].err_offset = gemm.err_offset = at["err"]
+    if "saved" in by:
+        for c in calls:
+            c.ptr_params = ((14, by["saved"]),)
+        if by["saved"] != node.id:
+            gemm.out_node = by["saved"]
+        if node.id == by["saved"]:   # the loss comes second, or nobody asked for it
+            calls[3].out_node = by.get("loss")
     return Launch(node.id, node.op, "linear-nll", None, node.inputs, nll_source(node.attrs["bias"]), calls,
-                  scratch_bytes=scratch, info={"rnv": (R, d, V), "bn": bz, "path": "tcgen05-f16x3"})
+                  scratch_bytes=end + _up(partial, 256),
+                  info={"rnv": (R, d, V), "bn": bn, "ctrl_bytes": _up(CTRL_BYTES, 64), "path": "tcgen05-f16x3"})
 
 
 def _nll_grad_launch(graph, ids):
     from .codegen import KernelCall, Launch
     node = graph.nodes[ids[0]]
-    (R, d), V = graph.nodes[node.inputs[0]].shape, graph.nodes[node.inputs[1]].shape[1]
-    dp, vp = _up(d, 8), _up(V, 8)
-    at, scratch, bz = nll_layout(R, d, V, True)
+    R, (d, V) = graph.nodes[node.inputs[0]].shape[0], (node.attrs["d"], node.attrs["V"])
+    inner, _ = linear_nll_saved(R, d, V)
     piece, pieces = nll_pieces(R, V)
-    bh, bw = f16_bn(R, d), f16_bn(d, piece)
     want = {graph.nodes[i].attrs["wrt"]: i for i in ids}
+    at, end = _regions(("scale", 256), ("err", CTRL_BYTES), ("dz", 4 * R * _up(piece, 256 if piece > 256 else 32)), ("db", 4 * math.ceil(R / 32) * V))
+    tail = [R, d, V, 0, inner["lse"], inner["h"], inner["w"], at["db"]]
+    calls, partial, widths = [], 0, set()
 
-    def to(call, wrt):
-        if want[wrt] != node.id:
-            call.out_node = want[wrt]
-        return call
-    calls, tail = _nll_prep(R, d, V, at, 1)
+    def add(name, wrt, M, N, K, maps, params):
+        nonlocal partial
+        bn = f16_bn(M, N, K)
+        c, nbytes = _gemm(name, M, N, K, 1, bn, 256, end, maps(bn), params)
+        c.err_offset = at["err"]
+        if wrt is not None and want[wrt] != node.id:
+            c.out_node = want[wrt]
+        partial = max(partial, nbytes)
+        widths.add(bn)
+        calls.append(c)
     for k in range(pieces):
         v0 = k * piece
         n = min(piece, V - v0)
-        zp = _up(n, 8)
-        params = tail[:-2] + [v0, 1 | (2 if k else 0)]
-        hk = _operand(at["h"], 2 * R * dp, d, R, 1, dp, False, F16_BM)
-        hm = _operand(at["h"], 2 * R * dp, d, R, 1, dp, True, F16_BM)
-        wk = _operand(at["w"] + 2 * v0, 2 * d * vp, n, d, 1, vp, False, bh)
-        wm = _operand(at["w"] + 2 * v0, 2 * d * vp, n, d, 1, vp, True, bz)
-        zk = _operand(at["dz"], 2 * R * zp, n, R, 1, zp, False, F16_BM)
-        zm = _operand(at["dz"], 2 * R * zp, n, R, 1, zp, True, bw)
-        out = [("scratch", at["dz"], n, R, 2, zp * 2, R * zp * 2, 32 | F16, 32)]
-        calls.append(_gemm("tcb_nll_dz", R, n, d, 1, bz, hk + wm + out, params))
+        params = [*tail, v0, int(k > 0)]
+        w_at = inner["w"] + (4 * d * v0 if v0 else 0)   # pieces begin with a block
+
+        def h(mn):
+            return _blocked_operand("in_at", _at(1, inner["h"]), R, d, _pitch(d), mn, F16_BM)
+
+        def w(mn, bn):
+            return _blocked_operand("in_at", _at(1, w_at), d, n, _pitch(V), mn, bn)
+
+        def z(mn, bn):
+            return _blocked_operand("scratch", at["dz"], R, n, _pitch(n), mn, bn)
+        out = _blocked("scratch", at["dz"], R, n, _pitch(n), 32, 32)
+        add("tcb_nll_dz", None, R, n, d, lambda bn: h(False) + w(True, bn) + out, params)
         if "h" in want:
-            calls.append(to(_gemm("tcb_nll_dh", R, d, n, 1, bh, zk + wk, params), "h"))
+            add("tcb_nll_dh", "h", R, d, n, lambda bn: z(False, F16_BM) + w(False, bn), params)
         if "w" in want:
-            calls.append(to(_gemm("tcb_nll_dw", d, n, R, 1, bw, hm + zm, params), "w"))
-    for c in calls:
-        if c.tma:
-            c.err_offset = at["err"]
+            add("tcb_nll_dw", "w", d, n, R, lambda bn: h(True) + z(True, bn), params)
     if "b" in want:
-        calls.append(to(KernelCall("tcb_nll_db", (math.ceil(V / 32), 1, 1), (256, 1, 1), 0, [0, 0, 0, 0, *tail]), "b"))
-    return Launch(node.id, node.op, "linear-nll-grad", None, node.inputs, nll_source(node.attrs["bias"]), calls,
-                  scratch_bytes=scratch,
-                  info={"rnv": (R, d, V), "pieces": pieces, "bn": (bz, bh, bw), "path": "tcgen05-f16x3"})
+        db = KernelCall("tcb_nll_db", (math.ceil(V / 32), 1, 1), (256, 1, 1), 0, [0, 0, 0, 0, *tail, 0, 0])
+        if want["b"] != node.id:
+            db.out_node = want["b"]
+        calls.append(db)
+    # no pass of its own comes first to clear the control block of a one-off run
+    clear = KernelCall("tcb_gemm_prep", (1, 1, 1), (128, 1, 1))
+    clear.err_offset = at["err"]
+    return Launch(node.id, node.op, "linear-nll-grad", None, node.inputs, nll_source(node.attrs["bias"]), [clear] + calls,
+                  scratch_bytes=end + _up(partial, 256),
+                  info={"rnv": (R, d, V), "pieces": pieces, "ctrl_bytes": _up(CTRL_BYTES, 64), "path": "tcgen05-f16x3"})
 
 
 # ------------------------------------------------------------------ headNormRope
@@ -241,7 +318,7 @@ def _head_launch(graph, ids):
         main.out_node = want["x"]
     if "gain" in want:
         scratch = grid * D * 4
-        fin = KernelCall("tcb_head_gain_finish", (math.ceil(D / 32), 1, 1), (1024, 1, 1), 0, [grid])
+        fin = KernelCall("tcb_head_gain_finish", (math.ceil(D / 8), 1, 1), (1024, 1, 1), 0, [grid])
         if want["gain"] != node.id:
             fin.out_node = want["gain"]
         calls.append(fin)
@@ -250,7 +327,8 @@ def _head_launch(graph, ids):
 
 
 # ------------------------------------------------------------------ orthogonalize
-NS_PARTS = 64
+NS_PARTS = 512
+NS_CHUNK = 128
 
 
 def orth_source(steps, coeffs, eps):
@@ -278,20 +356,15 @@ def _orth_launch(graph, node):
     s = min(m, n)
     xp, sp = _up(n, 8), _up(s, 8)
     xplane, splane = 2 * batch * m * xp, 2 * batch * s * sp
-    off = _up(512 + 8 * NS_PARTS * batch, 256) + 256
-    err = off - 256
-    xs = (off, off + _up(2 * xplane, 256))
-    s_at = xs[1] + _up(2 * xplane, 256)
-    p_at = s_at + _up(2 * splane, 256)
-    scratch = p_at + _up(2 * splane, 256)
-    bs, bx = f16_bn(s, s, batch), f16_bn(m, n, batch)
     parts = max(1, min(NS_PARTS, math.ceil(m * n / 4096)))
+    at, end = _regions(("parts", 8 * parts * batch), ("err", CTRL_BYTES), ("x0", 2 * xplane), ("x1", 2 * xplane),
+                       ("s", 2 * splane), ("p", 2 * splane))
+    bs, bx = f16_bn(s, s, max(m, n), batch), f16_bn(m, n, s, batch)
     norm = KernelCall("tcb_orth_norm", (parts, batch, 1), (256, 1, 1), 0, [parts, 0, 0, 0, m, n])
-    norm.err_offset = err
+    norm.err_offset = at["err"]
     split = KernelCall("tcb_orth_split", (max(1, min(m * math.ceil(n / 1024), SM_COUNT * 8)), batch, 1), (256, 1, 1), 0,
-                       [parts, 0, 0, 0, m, n, xs[0]])
-    calls = [norm, split]
-    sym = batch * _symmetric_tiles(s, bs)
+                       [parts, 0, 0, 0, m, n, at["x0"]])
+    calls, partial = [norm, split], 0
 
     def x_map(off, mn, bn):
         return _operand(off, xplane, n, m, batch, xp, mn, bn)
@@ -300,32 +373,33 @@ def _orth_launch(graph, node):
         return _operand(off, splane, s, s, batch, sp, False, bn)
 
     def out(off, rows, cols, pitch):
-        return [("scratch", off, cols, rows, 2 * batch, pitch * 2, rows * pitch * 2, 32 | F16, 32)]
+        return [("scratch", off, cols, rows, 2 * batch, pitch * 2, rows * pitch * 2, 32 | F16 | PAIR, 32)]
     for k in range(a["steps"]):
-        cur, nxt = xs[k % 2], xs[1 - k % 2]
-        last = k == a["steps"] - 1
-        params = [m, n, cur, nxt, s_at, p_at, int(last)]
-        calls.append(_gemm("tcb_orth_gram_tall" if tall else "tcb_orth_gram_wide", s, s, max(m, n), batch, bs,
-                           x_map(cur, tall, F16_BM) + x_map(cur, tall, bs) + out(s_at, s, s, sp), params, sym))
-        calls.append(_gemm("tcb_orth_poly", s, s, s, batch, bs,
-                           s_map(s_at, F16_BM) + s_map(s_at, bs) + out(p_at, s, s, sp), params, sym))
-        ab = x_map(cur, False, F16_BM) + s_map(p_at, bx) if tall else s_map(p_at, F16_BM) + x_map(cur, True, bx)
-        calls.append(_gemm("tcb_orth_apply_tall" if tall else "tcb_orth_apply_wide", m, n, s, batch, bx, ab + out(nxt, m, n, xp), params))
-    for c in calls:
-        if c.tma:
-            c.err_offset = err
+        cur, nxt = (at["x0"], at["x1"]) if k % 2 == 0 else (at["x1"], at["x0"])
+        params = [m, n, cur, nxt, at["s"], at["p"], int(k == a["steps"] - 1)]
+        ab = x_map(cur, False, F16_BM) + s_map(at["p"], bx) if tall else s_map(at["p"], F16_BM) + x_map(cur, True, bx)
+        for c, nbytes in (
+                _gemm("tcb_orth_gram_tall" if tall else "tcb_orth_gram_wide", s, s, max(m, n), batch, bs, NS_CHUNK, end,
+                      x_map(cur, tall, F16_BM) + x_map(cur, tall, bs) + out(at["s"], s, s, sp), params, True),
+                _gemm("tcb_orth_poly", s, s, s, batch, bs, NS_CHUNK, end,
+                      s_map(at["s"], F16_BM) + s_map(at["s"], bs) + out(at["p"], s, s, sp), params, True),
+                _gemm("tcb_orth_apply_tall" if tall else "tcb_orth_apply_wide", m, n, s, batch, bx, NS_CHUNK, end,
+                      ab + out(nxt, m, n, xp), params)):
+            c.err_offset = at["err"]
+            calls.append(c)
+            partial = max(partial, nbytes)
     return Launch(node.id, node.op, "orthogonalize", None, node.inputs,
-                  orth_source(a["steps"], a["coeffs"], a["eps"]), calls, scratch_bytes=scratch,
-                  info={"mn": (batch, m, n), "bn": (bs, bx), "path": "tcgen05-f16x3"})
+                  orth_source(a["steps"], a["coeffs"], a["eps"]), calls, scratch_bytes=end + _up(partial, 256),
+                  info={"mn": (batch, m, n), "bn": (bs, bx), "ctrl_bytes": _up(CTRL_BYTES, 64), "path": "tcgen05-f16x3"})
 
 
 def training_launch(graph, node, groups):
-    """The launch of a TRAINING_OPS node, or None for a gradient that an earlier sibling's launch computes."""
+    """The launch of a TRAINING_OPS node, or None for one that an earlier sibling's launch computes."""
     ids = groups.get(node.id, [node.id])
     if ids[0] != node.id:
         return None
     if node.op == "linearNll":
-        lau = _nll_launch(graph, node)
+        lau = _nll_launch(graph, ids)
     elif node.op == "linearNllGrad":
         lau = _nll_grad_launch(graph, ids)
     elif node.op in ("headNormRope", "headNormRopeGrad"):

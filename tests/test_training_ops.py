@@ -80,15 +80,21 @@ def test_raw_emit_is_checked(pkg):
     g, h, w, b, y = nll_graph(pkg, 5, 3, 7)
     js = g.to_json()
     assert pkg.ir.Graph.from_json(js).nodes[y].shape == [5]
-    js["nodes"][y]["attrs"] = {"bias": False}
-    with pytest.raises(pkg.ir.ShapeError):
-        pkg.ir.Graph.from_json(js)
-    t, gy = g.input_id("t"), g.input("gy", [5])
-    for wrt in ("t", None, "bias"):
+    for attrs in ({"bias": False, "out": "loss"}, {"bias": True}, {"bias": True, "out": "logits"}, {"out": "loss"}):
+        js["nodes"][y]["attrs"] = attrs
         with pytest.raises(pkg.ir.ShapeError):
-            g.emit("linearNllGrad", [h, w, b, t, y, gy], {"bias": True, "wrt": wrt})
+            pkg.ir.Graph.from_json(js)
+    t, gy = g.input_id("t"), g.input("gy", [5])
+    saved = g.emit("linearNll", [h, w, b, t], {"bias": True, "out": "saved"})
+    ok = {"bias": True, "d": 3, "V": 7, "wrt": "h"}
+    assert g.shape(g.emit("linearNllGrad", [t, saved, gy], ok)) == [5, 3]
+    for bad in ({"wrt": "t"}, {"wrt": None}, {"d": 40}, {"V": 800}, {"V": 0}, {"d": 3.0}, {"bias": False, "wrt": "b"}):
+        with pytest.raises(pkg.ir.ShapeError):
+            g.emit("linearNllGrad", [t, saved, gy], {**ok, **bad})
     with pytest.raises(pkg.ir.ShapeError):
-        g.emit("linearNllGrad", [h, w, t, y, gy], {"bias": False, "wrt": "b"})
+        g.emit("linearNllGrad", [t, gy, saved], ok)
+    with pytest.raises(pkg.autodiff.GradientError):
+        pkg.autodiff.grad(g, [saved], [h])
 
 
 def test_orthogonalize_has_no_gradient(pkg):
@@ -195,6 +201,22 @@ def test_gradients_of_a_node_are_one_launch(mods):
     lau = [l for l in cg.lower(G)["launches"] if l.kind == "linear-nll-grad"]
     assert len(lau) == 1 and [c.name.rsplit("_", 1)[0] for c in lau[0].calls if c.tma] == ["tcb_nll_dz", "tcb_nll_dh"]
     assert not hasattr(lau[0], "nodes")
+    # the loss and what it saves are one launch too; without a backward nothing is saved
+    (fwd,) = [l for l in cg.lower(G)["launches"] if l.kind == "linear-nll"]
+    assert fwd.nodes[0] == y and len(fwd.nodes) == 2
+    (fwd,) = cg.lower(g)["launches"]
+    assert not hasattr(fwd, "nodes")
+
+
+def test_equal_nodes_are_launches_of_their_own(mods):
+    """The same loss emitted twice: either is computed, neither is taken for the other's sibling."""
+    pkg, cg, to, rt = mods
+    g, h, w, b, y = nll_graph(pkg, 30, 8, 10)
+    y2 = g.linear_nll(h, w, b, g.input_id("t"))
+    assert [l.node for l in cg.lower(g)["launches"]] == [y, y2]
+    G, grads = _grads(pkg, g, g.add(y, y2), [h])
+    made = [i for l in cg.lower_fused(G)["launches"] for i in (getattr(l, "nodes", None) or [l.node])]
+    assert len(made) == len(set(made)) and {n.id for n in G.nodes if n.op in pkg.ir.TRAINING_OPS} <= set(made)
 
 
 def test_two_nodes_keep_their_gradients_apart(mods):
@@ -207,32 +229,69 @@ def test_two_nodes_keep_their_gradients_apart(mods):
 
 @pytest.mark.parametrize("R,d,V", [(1, 1, 1), (64, 64, 65), (4095, 256, 8192), (8192, 1024, 50001), (16384, 17, 131072),
                                    (3, 2048, 1 << 24), (1 << 20, 64, 65)])
-def test_nll_scratch_holds_every_part(mods, R, d, V):
-    """Every region the kernels address lies inside scratch and overlaps no other, maps start on 16 bytes."""
+def test_nll_maps_stay_inside(mods, R, d, V):
+    """Every tensor map starts on 16 bytes and ends inside its region; a piece of dz is bounded."""
     pkg, cg, to, rt = mods
     g, h, w, b, y = nll_graph(pkg, R, d, V)
+    inner, floats = pkg.ir.linear_nll_saved(R, d, V)
+    def blocked(n):
+        return -(-n // 256) * min(256, to._up(n, 32))
+    parts = sorted([(0, 12), (256, 4 * to._up(V, 256)), (inner["lse"], 4 * R), (inner["h"], 4 * R * blocked(d)),
+                    (inner["w"], 4 * d * blocked(V))])
+    assert all(o + n <= o2 for (o, n), (o2, _) in itertools.pairwise(parts)) and sum(parts[-1]) <= 4 * floats
+    piece, pieces = to.nll_pieces(R, V)
+    assert piece * pieces >= V > piece * (pieces - 1) and (pieces == 1 or piece % 256 == 0)
+    assert 4 * R * piece <= max(to.DZ_BYTES, 4 * R * 256)
     G, _ = _grads(pkg, g, y, [h, w, b])
-    for lau in cg.lower_fused(G)["launches"]:
-        back = lau.kind == "linear-nll-grad"
-        at, total, bz = to.nll_layout(R, d, V, back)
-        assert lau.scratch_bytes == total
-        piece, pieces = to.nll_pieces(R, V)
-        assert piece * pieces >= V > piece * (pieces - 1) and (pieces == 1 or piece % 256 == 0)
-        size = {"err": 16, "h": 4 * R * to._up(d, 8), "w": 4 * d * to._up(V, 8)}
-        size.update({"stat": 16 * R, "dz": 4 * R * piece, "db": 4 * -(-R // 32) * V} if back
-                    else {"stat": 4 * R, "part": 8 * R * -(-V // (bz // 2))})
-        assert set(size) == set(at)
-        ranges = sorted((at[k], at[k] + n) for k, n in size.items())
-        assert ranges[0][0] >= to.AMAX_AT + 12 * to.AMAX_BLOCKS and ranges[-1][1] <= total
-        assert all(a[1] <= b_[0] for a, b_ in itertools.pairwise(ranges))
-        if back:
-            assert 4 * R * piece <= max(to.DZ_BYTES, 4 * R * 256)
-        for c in lau.calls:
-            for region, off, cols, rows, batch, rs, bs, bc, br in c.tma or []:
-                # the last element of the map lies in scratch
-                end = off + (batch - 1) * bs + (rows - 1) * rs + 2 * cols
-                assert region == "scratch" and off % 16 == 0 and rs % 16 == 0 and bs % 16 == 0 and end <= total
-                assert 2 * cols <= rs
+    for graph in (g, G):
+        for lau in cg.lower_fused(graph)["launches"]:
+            sizes = {"scratch": lau.scratch_bytes, "out": 4 * floats, "in_at": 4 * floats}
+            for c in lau.calls:
+                for region, off, cols, rows, batch, rs, bs, bc, br in c.tma or []:
+                    if region == "in_at":
+                        assert off & 7 == 1
+                        off >>= 3
+                    end = off + (batch - 1) * bs + (rows - 1) * rs + 2 * cols
+                    assert off % 16 == 0 and rs % 16 == 0 and bs % 16 == 0 and end <= sizes[region] and 2 * cols <= rs
+
+
+@pytest.mark.parametrize("tiles,K,chunk,bn", [(1, 16384, 256, 64), (1, 256, 256, 256), (7, 5000, 256, 128), (147, 1024, 256, 256),
+                                              (148, 1024, 256, 256), (149, 4096, 256, 256), (256, 8192, 256, 256),
+                                              (300, 700, 128, 256), (1000, 33, 256, 64), (443, 12345, 128, 256)])
+def test_division_of_a_product(mods, tiles, K, chunk, bn):
+    """The device's division of tiles among CTAs, restated: every chunk of every tile once, the pieces of a
+    divided tile found by the warp that adds them, no two in one slot."""
+    pkg, cg, to, rt = mods
+    grid, whole, q = to.f16_plan(tiles, K, chunk, bn)
+    chunks = -(-K // chunk)
+    per = -(-chunks // q)
+    total = (tiles - whole) * per
+    assert 1 <= grid <= 148 and (total == 0 or grid <= total) and tiles - whole <= 2 * 148
+    seen, slots = {}, {}
+    for c in range(grid):
+        for t in range(c, whole, grid):
+            seen.setdefault(t, []).append((0, chunks, c))
+        at, end = c * total // grid, (c + 1) * total // grid
+        while at < end:
+            t, k = divmod(at, per)
+            n = min(end - at, per - k)
+            piece = (k * q, min((k + n) * q, chunks), c)
+            seen.setdefault(whole + t, []).append(piece)
+            if piece[:2] != (0, chunks):
+                slot = 2 * c + (k == 0)
+                assert slot not in slots
+                slots[slot] = (whole + t, piece)
+            at += n
+    assert sorted(seen) == list(range(tiles))
+    for t, pieces in seen.items():
+        pieces.sort()
+        assert pieces[0][0] == 0 and pieces[-1][1] == chunks and all(a[1] == b[0] for a, b in itertools.pairwise(pieces))
+        if len(pieces) > 1:
+            first = (t - whole) * per
+            ca, cb = (((x + 1) * grid - 1) // total for x in (first, first + per - 1))
+            assert [p[2] for p in pieces] == list(range(ca, cb + 1))
+            assert [slots[2 * c + (c == ca)][1] for c in range(ca, cb + 1)] == pieces
+    assert to.f16_partial_bytes(grid, whole, tiles, bn) >= (max(slots) + 1 if slots else 0) * 128 * bn * 4
 
 
 @pytest.mark.parametrize("shape", [[1, 1], [64, 64], [100, 70], [3, 70, 300], [4095, 1000], [2, 2, 256, 1024]])
