@@ -13,7 +13,6 @@ compiled in.  The library's own lowering (csrc/lower.cpp) makes the same records
 from __future__ import annotations
 
 import math
-import os
 import struct
 
 from .ir import TRAINING_OPS, linear_nll_saved, newton_schulz_scales, size
@@ -23,7 +22,7 @@ F16 = 1 << 33          # box_cols flags of a tensor map: 16-bit elements,
 PAIR = 1 << 34         # two planes (hi and lo) a box
 F16_BM, F16_BK = 128, 32
 AMAX_BLOCKS = 4 * SM_COUNT
-DZ_BYTES = int(os.environ.get('DZ','256')) << 20             # bound of one vocabulary piece's dz
+DZ_BYTES = 128 << 20             # bound of one vocabulary piece's dz
 CTRL_BYTES = 4 * (4 + 8 * 2 * SM_COUNT)   # error word, and a counter per epilogue warp of a divided tile
 
 
@@ -42,45 +41,42 @@ def f16_smem(bn):
     return stages * stage + 1024 + 32768 + 1024
 
 
-def f16_bn(M, N, K, batch=1):
-    """Tile width of a split-fp16 product: the widest that leaves every SM about two chains of 256 K indices
-    (tiles can be divided along K), down to 64."""
-    if os.environ.get('BNF'):
-        return int(os.environ['BNF'])
-    for bn in (256, 128):
-        if N > bn // 2 and batch * math.ceil(M / F16_BM) * math.ceil(N / bn) * math.ceil(K / 256) >= 2 * SM_COUNT:
-            return bn
-    return 64
-
-
 def f16_tiles(M, N, bn, symmetric):
     tm, tn = math.ceil(M / F16_BM), math.ceil(N / bn)
     return sum(tn - i * F16_BM // bn for i in range(tm)) if symmetric else tm * tn
 
 
-QUANTUM = int(os.environ.get('Q', '1'))
+# Nanoseconds of a split-fp16 product by tile width, as measured with every SM busy: a K step of 16 of one tile;
+# an epilogue; the exchange of a divided tile's partial sums, at all and for each part.
+F16_COST = {256: (290, 6000, 3000, 2500), 128: (180, 3000, 1500, 1200), 64: (140, 1500, 1000, 700)}
 
 
-def f16_plan(tiles, K, chunk, bn):
-    """(grid, whole tiles, quantum) of a product of `tiles` output tiles (tcb/gemm_f16x3.cuh).
+def f16_plan(M, N, K, batch, chunk, symmetric=False):
+    """(tile width, grid, whole tiles, quantum) of a product (tcb/gemm_f16x3.cuh), the cheapest by F16_COST.
 
-    The tiles beyond the whole waves are divided along K where that saves more than their partial sums
-    cost: about three chains of 256 a CTA.  A CTA's run is then more than a tile and cut anywhere; with
-    fewer tiles than SMs a piece is at least `quantum` chains, longer for narrow tiles, whose chains are
-    short beside the exchange."""
-    chunks = math.ceil(K / chunk)
-    if os.environ.get('WH'):
-        return min(SM_COUNT, tiles), tiles, 1
-    if tiles >= SM_COUNT:
-        idle = -tiles % SM_COUNT
-        if idle * chunks * chunk <= 3 * 256 * SM_COUNT:
-            return SM_COUNT, tiles, 1
-        return SM_COUNT, tiles - tiles % SM_COUNT - SM_COUNT, 1
-    quantum = QUANTUM * (256 // chunk)
-    per = math.ceil(chunks / quantum)
-    if per == 1:
-        return tiles, tiles, 1
-    return min(SM_COUNT, tiles * per), 0, quantum
+    Tiles go whole to the SMs in waves, or, where they are fewer than the SMs, in pieces of `quantum` chains
+    of `chunk` K indices.  Dividing the last wave of more tiles than that does not pay: the CTAs then no
+    longer read the same operands at the same time (4096 x 1024 products of K 8192, 128 of 148 SMs, 146 us
+    whole, 216 divided)."""
+    best = None
+    steps = math.ceil(K / 16)
+    for bn, (step, epi, once, part) in F16_COST.items():
+        if bn > 64 and N <= bn // 2:
+            continue
+        tiles = batch * f16_tiles(M, N, bn, symmetric)
+        plans = [(math.ceil(tiles / SM_COUNT) * (steps * step + epi), bn, min(SM_COUNT, tiles), tiles, 1)]
+        for q in (1, 2, 4, 8, 16, 32, 64):
+            per = math.ceil(K / (256 * q))
+            if tiles >= SM_COUNT or per == 1:
+                break
+            grid = min(SM_COUNT, tiles * per)
+            run = math.ceil(tiles * per / grid)
+            pieces = per if run == 1 else per // run + 2
+            plans.append((run * q * 16 * step + once + pieces * part + epi, bn, grid, 0, q * (256 // chunk)))
+        for p in plans:
+            if best is None or p[0] < best[0]:
+                best = p
+    return best[1:]
 
 
 def f16_partial_bytes(grid, whole, tiles, bn):
@@ -114,12 +110,12 @@ def _at(index, off):
     return off << 3 | index
 
 
-def _gemm(name, M, N, K, batch, bn, chunk, part_at, maps, params, symmetric=False):
+def _gemm(name, M, N, K, batch, plan, part_at, maps, params, symmetric=False):
     from .codegen import KernelCall
+    bn, grid, whole, quantum = plan
     tiles = batch * f16_tiles(M, N, bn, symmetric)
     if tiles >= 1 << 31:
         raise ValueError(f"{name}: {tiles} tiles")
-    grid, whole, quantum = f16_plan(tiles, K, chunk, bn)
     c = KernelCall(f"{name}_{bn}", (grid, 1, 1), (384, 1, 1), f16_smem(bn),
                    [M | N << 32, K | batch << 32, whole | quantum << 32, part_at, *params])
     c.tma = maps
@@ -146,6 +142,9 @@ def siblings(graph):
 
 
 # ------------------------------------------------------------------ linearNll
+NLL_CHUNK = 256
+
+
 def nll_pieces(R, V):
     """(columns of a piece, pieces): dz of a piece, 4 bytes a value, within DZ_BYTES; whole 256-wide tiles,
     the pieces of about one size."""
@@ -178,7 +177,8 @@ def _nll_launch(graph, ids):
     node = graph.nodes[ids[0]]
     (R, d), V = graph.nodes[node.inputs[0]].shape, graph.nodes[node.inputs[1]].shape[1]
     inner, floats = linear_nll_saved(R, d, V)
-    bn = f16_bn(R, V, d)
+    plan = f16_plan(R, V, d, 1, NLL_CHUNK)
+    bn = plan[0]
     halves = math.ceil(V / (bn // 2))
     at, end = _regions(("amax", 8 * AMAX_BLOCKS), ("err", CTRL_BYTES), ("zt", 4 * R), ("part", 8 * R * halves),
                        ("loss", 0 if "loss" in by else 4 * R), ("saved", 0 if "saved" in by else 4 * floats))
@@ -193,7 +193,7 @@ def _nll_launch(graph, ids):
             _blocked_operand(*saved(inner["w"]), d, V, _pitch(V), True, bn))
     blocks = max(1, min(AMAX_BLOCKS, math.ceil((R * d + d * V) / 2048)))
     units = d * math.ceil(V / 1024) + R * math.ceil(d / 1024)
-    gemm, partial = _gemm("tcb_nll_logits", R, V, d, 1, bn, 256, end, maps, tail)
+    gemm, partial = _gemm("tcb_nll_logits", R, V, d, 1, plan, end, maps, tail)
     calls = [KernelCall("tcb_nll_amax", (blocks, 1, 1), (256, 1, 1), 0, [blocks, 0, 0, 0, *tail]),
              KernelCall("tcb_nll_split", (max(2, min(units, SM_COUNT * 8)), 1, 1), (256, 1, 1), 0, [blocks, 0, 0, 0, *tail]),
              gemm, KernelCall("tcb_nll_finish", (math.ceil(R / 32), 1, 1), (256, 1, 1), 0, [halves, 0, 0, 0, *tail])]
@@ -219,17 +219,16 @@ def _nll_grad_launch(graph, ids):
     want = {graph.nodes[i].attrs["wrt"]: i for i in ids}
     at, end = _regions(("scale", 256), ("err", CTRL_BYTES), ("dz", 4 * R * _up(piece, 256 if piece > 256 else 32)), ("db", 4 * math.ceil(R / 32) * V))
     tail = [R, d, V, 0, inner["lse"], inner["h"], inner["w"], at["db"]]
-    calls, partial, widths = [], 0, set()
+    calls, partial = [], 0
 
     def add(name, wrt, M, N, K, maps, params):
         nonlocal partial
-        bn = f16_bn(M, N, K)
-        c, nbytes = _gemm(name, M, N, K, 1, bn, 256, end, maps(bn), params)
+        plan = f16_plan(M, N, K, 1, NLL_CHUNK)
+        c, nbytes = _gemm(name, M, N, K, 1, plan, end, maps(plan[0]), params)
         c.err_offset = at["err"]
         if wrt is not None and want[wrt] != node.id:
             c.out_node = want[wrt]
         partial = max(partial, nbytes)
-        widths.add(bn)
         calls.append(c)
     for k in range(pieces):
         v0 = k * piece
@@ -359,7 +358,8 @@ def _orth_launch(graph, node):
     parts = max(1, min(NS_PARTS, math.ceil(m * n / 4096)))
     at, end = _regions(("parts", 8 * parts * batch), ("err", CTRL_BYTES), ("x0", 2 * xplane), ("x1", 2 * xplane),
                        ("s", 2 * splane), ("p", 2 * splane))
-    bs, bx = f16_bn(s, s, max(m, n), batch), f16_bn(m, n, s, batch)
+    gram, poly = f16_plan(s, s, max(m, n), batch, NS_CHUNK, True), f16_plan(s, s, s, batch, NS_CHUNK, True)
+    app = f16_plan(m, n, s, batch, NS_CHUNK)
     norm = KernelCall("tcb_orth_norm", (parts, batch, 1), (256, 1, 1), 0, [parts, 0, 0, 0, m, n])
     norm.err_offset = at["err"]
     split = KernelCall("tcb_orth_split", (max(1, min(m * math.ceil(n / 1024), SM_COUNT * 8)), batch, 1), (256, 1, 1), 0,
@@ -377,20 +377,20 @@ def _orth_launch(graph, node):
     for k in range(a["steps"]):
         cur, nxt = (at["x0"], at["x1"]) if k % 2 == 0 else (at["x1"], at["x0"])
         params = [m, n, cur, nxt, at["s"], at["p"], int(k == a["steps"] - 1)]
-        ab = x_map(cur, False, F16_BM) + s_map(at["p"], bx) if tall else s_map(at["p"], F16_BM) + x_map(cur, True, bx)
+        ab = x_map(cur, False, F16_BM) + s_map(at["p"], app[0]) if tall else s_map(at["p"], F16_BM) + x_map(cur, True, app[0])
         for c, nbytes in (
-                _gemm("tcb_orth_gram_tall" if tall else "tcb_orth_gram_wide", s, s, max(m, n), batch, bs, NS_CHUNK, end,
-                      x_map(cur, tall, F16_BM) + x_map(cur, tall, bs) + out(at["s"], s, s, sp), params, True),
-                _gemm("tcb_orth_poly", s, s, s, batch, bs, NS_CHUNK, end,
-                      s_map(at["s"], F16_BM) + s_map(at["s"], bs) + out(at["p"], s, s, sp), params, True),
-                _gemm("tcb_orth_apply_tall" if tall else "tcb_orth_apply_wide", m, n, s, batch, bx, NS_CHUNK, end,
+                _gemm("tcb_orth_gram_tall" if tall else "tcb_orth_gram_wide", s, s, max(m, n), batch, gram, end,
+                      x_map(cur, tall, F16_BM) + x_map(cur, tall, gram[0]) + out(at["s"], s, s, sp), params, True),
+                _gemm("tcb_orth_poly", s, s, s, batch, poly, end,
+                      s_map(at["s"], F16_BM) + s_map(at["s"], poly[0]) + out(at["p"], s, s, sp), params, True),
+                _gemm("tcb_orth_apply_tall" if tall else "tcb_orth_apply_wide", m, n, s, batch, app, end,
                       ab + out(nxt, m, n, xp), params)):
             c.err_offset = at["err"]
             calls.append(c)
             partial = max(partial, nbytes)
     return Launch(node.id, node.op, "orthogonalize", None, node.inputs,
                   orth_source(a["steps"], a["coeffs"], a["eps"]), calls, scratch_bytes=end + _up(partial, 256),
-                  info={"mn": (batch, m, n), "bn": (bs, bx), "ctrl_bytes": _up(CTRL_BYTES, 64), "path": "tcgen05-f16x3"})
+                  info={"mn": (batch, m, n), "bn": (gram[0], poly[0], app[0]), "ctrl_bytes": _up(CTRL_BYTES, 64), "path": "tcgen05-f16x3"})
 
 
 def training_launch(graph, node, groups):

@@ -255,18 +255,21 @@ def test_nll_maps_stay_inside(mods, R, d, V):
                     assert off % 16 == 0 and rs % 16 == 0 and bs % 16 == 0 and end <= sizes[region] and 2 * cols <= rs
 
 
-@pytest.mark.parametrize("tiles,K,chunk,bn", [(1, 16384, 256, 64), (1, 256, 256, 256), (7, 5000, 256, 128), (147, 1024, 256, 256),
-                                              (148, 1024, 256, 256), (149, 4096, 256, 256), (256, 8192, 256, 256),
-                                              (300, 700, 128, 256), (1000, 33, 256, 64), (443, 12345, 128, 256)])
-def test_division_of_a_product(mods, tiles, K, chunk, bn):
+@pytest.mark.parametrize("M,N,K,batch,chunk,sym", [(64, 50, 16384, 1, 256, False), (1, 1, 1, 1, 256, False), (57, 1365, 55301, 1, 256, False),
+                                                   (256, 256, 1024, 4, 128, True), (1000, 1000, 4095, 1, 128, True),
+                                                   (4095, 256, 8192, 1, 256, False), (8192, 1024, 4096, 1, 256, False),
+                                                   (18, 18, 3593, 14, 128, True), (300, 4099, 700, 1, 128, False),
+                                                   (128, 2048, 12345, 1, 128, False)])
+def test_division_of_a_product(mods, M, N, K, batch, chunk, sym):
     """The device's division of tiles among CTAs, restated: every chunk of every tile once, the pieces of a
     divided tile found by the warp that adds them, no two in one slot."""
     pkg, cg, to, rt = mods
-    grid, whole, q = to.f16_plan(tiles, K, chunk, bn)
+    bn, grid, whole, q = to.f16_plan(M, N, K, batch, chunk, sym)
+    tiles = batch * to.f16_tiles(M, N, bn, sym)
     chunks = -(-K // chunk)
     per = -(-chunks // q)
     total = (tiles - whole) * per
-    assert 1 <= grid <= 148 and (total == 0 or grid <= total) and tiles - whole <= 2 * 148
+    assert 1 <= grid <= 148 and (total == 0 or grid <= total) and tiles - whole < 148 and (bn == 64 or N > bn // 2)
     seen, slots = {}, {}
     for c in range(grid):
         for t in range(c, whole, grid):
