@@ -7,6 +7,11 @@ the tanh MLP of the C1 workload can be built), ``src/m3b/model.js:29-145``
 ``src/m3b/step.js:13-31`` (forward + grad + Adam).  The reference hard-codes
 the transformer's sizes (src/m3b/model.js:12); here they are a ``cfg`` dict
 whose default is that same CONFIG.
+
+Beyond the reference, ``cfg`` may ask for ``"rope": base`` (queries and keys
+normalised per head and turned by position, in place of the learned positions)
+and ``"targets": "index"`` (``y`` holds each token's class, -1 for none, and the
+loss never makes the logits), and ``opt`` may be of kind ``"muon"``.
 """
 from __future__ import annotations
 
@@ -132,11 +137,15 @@ def param_spec(V, cfg=CONFIG):
 
     def linear(fan_in):
         return ("uniform", 1 / math.sqrt(fan_in))
-    spec = [("tok", [V, d], ("uniform", 1)), ("pos", [T, d], ("uniform", 1))]
+    spec = [("tok", [V, d], ("uniform", 1))]
+    if not cfg.get("rope"):
+        spec.append(("pos", [T, d], ("uniform", 1)))
     for l in range(L):
         p = f"b{l}."
-        spec += [(f"{p}ln1.g", [d], ("ones",)), (f"{p}ln1.b", [d], ("zeros",)),
-                 (f"{p}wq", [d, d], linear(d)), (f"{p}wk", [d, d], linear(d)), (f"{p}wv", [d, d], linear(d)),
+        spec += [(f"{p}ln1.g", [d], ("ones",)), (f"{p}ln1.b", [d], ("zeros",))]
+        if cfg.get("rope"):
+            spec += [(f"{p}qn", [cfg["dh"]], ("ones",)), (f"{p}kn", [cfg["dh"]], ("ones",))]
+        spec += [(f"{p}wq", [d, d], linear(d)), (f"{p}wk", [d, d], linear(d)), (f"{p}wv", [d, d], linear(d)),
                  (f"{p}wo", [d, d], linear(d)), (f"{p}bo", [d], linear(d)),
                  (f"{p}ln2.g", [d], ("ones",)), (f"{p}ln2.b", [d], ("zeros",)),
                  (f"{p}w1", [d, ff], linear(d)), (f"{p}b1", [ff], linear(d)),
@@ -209,7 +218,13 @@ def _attention(g, a, p, B, cfg, bug=None, trace=None):
 
     def heads(w):
         return g.transpose(g.reshape(g.matmul(a, p[w]), [B, T, H, dh]), [0, 2, 1, 3])
-    q, k, v = heads("wq"), heads("wk"), heads("wv")
+    def turned(w, gain):
+        x = g.reshape(g.matmul(a, p[w]), [B, T, H, dh])
+        return g.head_norm_rope(x, p[gain], g.const(list(range(T)), [T]), base=cfg["rope"], eps=cfg["eps"])
+    if cfg.get("rope"):
+        q, k, v = turned("wq", "qn"), turned("wk", "kn"), heads("wv")
+    else:
+        q, k, v = heads("wq"), heads("wk"), heads("wv")
     s = g.matmul(q, g.transpose(k, [0, 1, 3, 2]))
     if bug != "scale-missing":
         s = g.mul(s, g.const(1 / math.sqrt(dh)))
@@ -235,19 +250,28 @@ def _shift_matrix(T):
 BLOCK_KEYS = ("ln1.g", "ln1.b", "wq", "wk", "wv", "wo", "bo", "ln2.g", "ln2.b", "w1", "b1", "w2", "b2")
 
 
-def logits_of(g, ids, V, B, cfg=CONFIG, bug=None, trace=None):
-    """src/m3b/model.js:112-124."""
+def hidden_of(g, ids, V, B, cfg=CONFIG, bug=None, trace=None):
+    """The last layer norm's rows [B*T, d] (src/m3b/model.js:112-123)."""
     T, d, L = cfg["T"], cfg["d"], cfg["L"]
-    pos = ids["pos"]
-    if bug == "position-off-by-one":
-        pos = g.matmul(g.const(_shift_matrix(T), [T, T]), pos)
-    h = g.reshape(g.add(g.reshape(g.matmul(ids["x"], ids["tok"]), [B, T, d]), pos), [B * T, d])
+    if cfg.get("rope"):
+        h = g.matmul(ids["x"], ids["tok"])
+    else:
+        pos = ids["pos"]
+        if bug == "position-off-by-one":
+            pos = g.matmul(g.const(_shift_matrix(T), [T, T]), pos)
+        h = g.reshape(g.add(g.reshape(g.matmul(ids["x"], ids["tok"]), [B, T, d]), pos), [B * T, d])
+    keys = BLOCK_KEYS + (("qn", "kn") if cfg.get("rope") else ())
     for l in range(L):
-        p = {k: ids[f"b{l}.{k}"] for k in BLOCK_KEYS}
+        p = {k: ids[f"b{l}.{k}"] for k in keys}
         h = g.add(h, _attention(g, layer_norm(g, h, p["ln1.g"], p["ln1.b"], cfg, bug), p, B, cfg, bug, trace))
         m = layer_norm(g, h, p["ln2.g"], p["ln2.b"], cfg, bug)
         h = g.add(h, g.add(g.matmul(gelu(g, g.add(g.matmul(m, p["w1"]), p["b1"])), p["w2"]), p["b2"]))
-    return g.add(g.matmul(layer_norm(g, h, ids["lnf.g"], ids["lnf.b"], cfg, bug), ids["head"]), ids["headb"])
+    return layer_norm(g, h, ids["lnf.g"], ids["lnf.b"], cfg, bug)
+
+
+def logits_of(g, ids, V, B, cfg=CONFIG, bug=None, trace=None):
+    """src/m3b/model.js:112-124."""
+    return g.add(g.matmul(hidden_of(g, ids, V, B, cfg, bug, trace), ids["head"]), ids["headb"])
 
 
 def loss_of(g, logits, y, rows):
@@ -261,8 +285,13 @@ def build_forward(V, B, cfg=CONFIG, bug=None):
     g = Graph()
     ids = {name: g.input(name, shape) for name, shape, _ in param_spec(V, cfg)}
     ids["x"] = g.input("x", [B * T, V])
-    ids["y"] = g.input("y", [B * T, V])
     scores = []
+    if cfg.get("targets") == "index":   # no logits: the per-token losses stand in their place
+        ids["y"] = g.input("y", [B * T])
+        each = g.linear_nll(hidden_of(g, ids, V, B, cfg, bug, scores), ids["head"], ids["headb"], ids["y"])
+        loss = g.div(g.sum(each, 0), g.const(B * T))
+        return {"graph": g, "ids": ids, "logits": each, "loss": loss, "scores": scores}
+    ids["y"] = g.input("y", [B * T, V])
     logits = logits_of(g, ids, V, B, cfg, bug, scores)
     loss = loss_of(g, logits, ids["y"], B * T)
     return {"graph": g, "ids": ids, "logits": logits, "loss": loss, "scores": scores}
@@ -314,6 +343,46 @@ def adam_update(B, names, ids, grads, state, opt, sabotage=None):
     return outputs
 
 
+# ---------------------------------------------------------------- Muon
+MUON_3B = {"kind": "muon", "lr": 2e-2, "momentum": 0.95, "steps": 5, "weightDecay": 0, "adam": ADAM_3B}
+MUON_KEYS = ("wq", "wk", "wv", "wo", "w1", "w2")
+
+
+def muon_names(names):
+    """The blocks' weight matrices, which Muon updates; Adam updates every other parameter."""
+    return [n for n in names if n.rsplit(".", 1)[-1] in MUON_KEYS]
+
+
+def state_spec(names, shapes, opt=ADAM_3B):
+    """The optimizer's state, (name, shape) in order: Adam's moments, or for Muon's matrices a momentum buffer."""
+    if opt["kind"] != "muon":
+        return adam_state_spec(names, shapes)
+    mu = muon_names(names)
+    return [(f"{p}.buf", shapes[p]) for p in mu] + adam_state_spec([n for n in names if n not in mu], shapes)
+
+
+def initial_state(names, shapes, opt=ADAM_3B):
+    return {name: [1.0 if name.endswith("Pow") else 0.0] * _count(shape) for name, shape in state_spec(names, shapes, opt)}
+
+
+def muon_update(B, names, ids, grads, state, opt):
+    """Momentum with Nesterov's look ahead, orthogonalised: W [m, n] -= lr sqrt(max(1, m / n)) orth(g + mu buf),
+    after decoupled weight decay.  Parameters that are not a block's weight matrix get Adam."""
+    c = B.const
+    mu = muon_names(names)
+    outputs = adam_update(B, [n for n in names if n not in mu], ids, grads, state, opt["adam"])
+    for p in mu:
+        buf = B.add(B.mul(c(opt["momentum"]), state[f"{p}.buf"]), grads[p])
+        o = B.orthogonalize(B.add(grads[p], B.mul(c(opt["momentum"]), buf)), steps=opt["steps"])
+        m, n = B.shape(ids[p])
+        w = ids[p]
+        if opt["weightDecay"]:
+            w = B.mul(w, c(1 - opt["lr"] * opt["weightDecay"]))
+        outputs[p] = B.sub(w, B.mul(c(opt["lr"] * math.sqrt(max(1.0, m / n))), o))
+        outputs[f"{p}.buf"] = buf
+    return outputs
+
+
 def param_names(V, cfg=CONFIG):
     return [n for n, _, _ in param_spec(V, cfg)]
 
@@ -323,14 +392,15 @@ def param_shapes(V, cfg=CONFIG):
 
 
 def build_step3b(V, B, cfg=CONFIG, opt=ADAM_3B, bug=None, rules=None):
-    """Forward + grad + Adam as one graph (src/m3b/step.js:18-31)."""
+    """Forward + grad + optimizer as one graph (src/m3b/step.js:18-31; `opt` of kind "muon": muon_update)."""
     f = build_forward(V, B, cfg, bug)
     names = param_names(V, cfg)
     G = grad(f["graph"], [f["loss"]], [f["ids"][n] for n in names], rules=rules)
     g = G.graph
     grads = {n: G.grads[k] for k, n in enumerate(names)}
-    state = {name: g.input(name, shape) for name, shape in adam_state_spec(names, param_shapes(V, cfg))}
-    outputs = adam_update(g, names, f["ids"], grads, state, opt)
+    state = {name: g.input(name, shape) for name, shape in state_spec(names, param_shapes(V, cfg), opt)}
+    update = muon_update if opt["kind"] == "muon" else adam_update
+    outputs = update(g, names, f["ids"], grads, state, opt)
     inputs = {**{n: f["ids"][n] for n in names}, "x": f["ids"]["x"], "y": f["ids"]["y"], **state}
     return {"graph": g, "names": names, "stateNames": list(state), "loss": f["loss"], "logits": f["logits"],
             "grads": grads, "inputs": inputs, "outputs": outputs, "cotangent": G.cotangents[0]}
@@ -360,10 +430,14 @@ def build_adam_graph(V, cfg=CONFIG, opt=ADAM_3B):
     return {"graph": g, "names": names, "inputs": inputs, "outputs": outputs}
 
 
-def encode_batch(seqs, V, T):
-    """One-hot x, y [B*T, V] from T+1-token sequences (src/m3b/data.js:62-72), as numpy float32."""
+def encode_batch(seqs, V, T, targets="one-hot"):
+    """One-hot x, y [B*T, V] from T+1-token sequences (src/m3b/data.js:62-72), as numpy float32; with `targets`
+    "index" y holds the classes themselves, [B*T]."""
     import numpy as np
     B = len(seqs)
+    if targets == "index":
+        x, _ = encode_batch(seqs, V, T)
+        return x, np.asarray([s[1:T + 1] for s in seqs], np.float32).reshape(-1)
     x = np.zeros((B * T, V), dtype=np.float32)
     y = np.zeros((B * T, V), dtype=np.float32)
     for b, s in enumerate(seqs):
