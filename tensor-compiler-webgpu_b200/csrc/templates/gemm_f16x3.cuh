@@ -36,8 +36,9 @@
 //
 // p[0] = M | N << 32, p[1] = K | batch << 32, p[2] = full | quantum << 32, p[3] = byte offset in scratch of
 // the partial sums (two 128 x BN slots a CTA), p[15] = control block: the error word, 16 bytes on a
-// counter per warp and tile, zero between launches.  Maps: A, B ({cols, rows, 2 batch}: each matrix's hi
-// plane, then its lo plane, a box taking both) and the epilogue's.  BLOCKED operands (no batch) are stored in
+// counter per warp and divided tile (fewer than 148 tiles), zero between launches.  Maps: A, B ({cols, rows,
+// 2 batch}: each matrix's hi plane, then its lo plane, a box taking both) and the epilogue's.  A kernel may run
+// two products side by side, each on CTAs of its own (F16Job).  BLOCKED operands (no batch) are stored in
 // blocks of 256 columns, a block's planes of 512-byte rows in the place of a batch: with rows as long as a
 // vocabulary every row of a K-major box lies in a page of its own (dh at 8192 x 1024 x 50001: 1.34 us a stage
 // of 32 K indices, the same product of short rows 0.70).
@@ -163,22 +164,22 @@ __device__ __forceinline__ u32 f16_tiles(u32 tm, u32 tn) {
 // The work of one CTA, in order: whole tiles, then its run of the divided ones.
 struct F16Work {
   u32 tiles, full, chunks, quantum, per;   // per: units of a divided tile
-  u32 u;                                   // next whole tile
+  u32 grid, u;                             // CTAs; next whole tile
   u64 at, end, total;                      // the run, in units over the divided tiles
   u32 tile, c0, c1;                        // the current piece: chunks c0 .. c1 of a tile
-  __device__ __forceinline__ F16Work(u32 tiles_, u32 full_, u32 chunks_, u32 quantum_)
+  __device__ __forceinline__ F16Work(u32 tiles_, u32 full_, u32 chunks_, u32 quantum_, u32 block, u32 grid_)
       : tiles(tiles_), full(full_), chunks(chunks_), quantum(quantum_), per((chunks_ + quantum_ - 1) / quantum_),
-        u(blockIdx.x) {
+        grid(grid_), u(block) {
     total = (u64)(tiles - full) * per;
-    at = blockIdx.x * total / gridDim.x;
-    end = (blockIdx.x + 1) * total / gridDim.x;
+    at = block * total / grid;
+    end = (block + 1) * total / grid;
   }
   __device__ __forceinline__ bool next() {
     if (u < full) {
       tile = u;
       c0 = 0;
       c1 = chunks;
-      u += gridDim.x;
+      u += grid;
       return true;
     }
     if (at >= end) return false;
@@ -192,7 +193,7 @@ struct F16Work {
   }
   __device__ __forceinline__ bool whole() const { return c0 == 0 && c1 == chunks; }
   // the CTA whose run holds unit x
-  __device__ __forceinline__ u32 owner(u64 x) const { return (u32)(((x + 1) * gridDim.x - 1) / total); }
+  __device__ __forceinline__ u32 owner(u64 x) const { return (u32)(((x + 1) * grid - 1) / total); }
 };
 
 // An epilogue warp's view of one tile: rows 32 q .. of it, columns from c0, this lane's row.
@@ -200,6 +201,7 @@ struct F16Epi {
   F16Tile T;
   int q, c0, lane;
   u64 row;             // of the output, may lie beyond M
+  u32 M, N;
   u32 stage;           // shared-memory address of the warp's 4 KB block
   unsigned char* gstage;
 };
@@ -265,12 +267,23 @@ __device__ __forceinline__ void f16_blocks(EPI& epi, const F16Epi& e, float (&v)
 
 // EPI: struct with start(staging) once, by all 256 epilogue threads, begin(e), block(e, c0, v) for each 32 columns (from column c0 of the tile) that reach into
 // the output, end(e), and done(e) once after the last tile.
+struct F16Job {
+  const TmaDesc *ma, *mb;
+  u32 M, N, K, batch, full, quantum, block, grid;
+  float* part;
+  u32* counters;
+};
+__device__ __forceinline__ F16Job f16_job(const GemmParams& P) {
+  return {&P.maps[0], &P.maps[1], (u32)P.a.p[0], (u32)((u64)P.a.p[0] >> 32), (u32)P.a.p[1], (u32)((u64)P.a.p[1] >> 32),
+          (u32)P.a.p[2], (u32)((u64)P.a.p[2] >> 32), blockIdx.x, gridDim.x,
+          reinterpret_cast<float*>(P.a.scratch + (u64)P.a.p[3]), reinterpret_cast<u32*>(P.a.p[15]) + 4};
+}
+
 template <int BN, bool A_MN, bool B_MN, bool SYM, bool BLOCKED, int CHUNK, class EPI>
-__device__ __forceinline__ void gemm_f16x3(const GemmParams& P, EPI& epi) {
+__device__ __forceinline__ void gemm_f16x3(const F16Job& J, u32* err, EPI& epi) {
   using S = F16x3<BN>;
   constexpr u32 STAGES = S::STAGES;
   extern __shared__ unsigned char smem_raw[];
-  u32* err = reinterpret_cast<u32*>(P.a.p[15]);
   const u32 raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
   unsigned char* gbase = smem_raw + (base - raw);
   const u32 bars = base + STAGES * S::STAGE, staging = bars + 1024;
@@ -280,16 +293,15 @@ __device__ __forceinline__ void gemm_f16x3(const GemmParams& P, EPI& epi) {
   auto empty = [&](u32 s) { return bars + 8u * (STAGES + s); };
   auto accf = [&](u32 b) { return bars + 8u * (2 * STAGES + b); };
   auto acce = [&](u32 b) { return bars + 8u * (2 * STAGES + 2 + b); };
-  const u32 M = (u32)P.a.p[0], N = (u32)((u64)P.a.p[0] >> 32), K = (u32)P.a.p[1], batch = (u32)((u64)P.a.p[1] >> 32);
-  const u32 tm = (M + HG_M - 1) / HG_M, tn = (N + BN - 1) / BN, kbs = (K + HG_K - 1) / HG_K;
+  const u32 M = J.M, N = J.N;
+  const u32 tm = (M + HG_M - 1) / HG_M, tn = (N + BN - 1) / BN, kbs = (J.K + HG_K - 1) / HG_K;
   constexpr u32 CK = CHUNK / HG_K;   // stages of a chunk
   const u32 per = f16_tiles<BN, SYM>(tm, tn);
-  F16Work work(per * batch, (u32)P.a.p[2], (kbs + CK - 1) / CK, (u32)((u64)P.a.p[2] >> 32));
+  F16Work work(per * J.batch, J.full, (kbs + CK - 1) / CK, J.quantum, J.block, J.grid);
 
   if (threadIdx.x == 32 * 3) {
-#pragma unroll
-    for (int m = 0; m < 2; ++m)
-      asm volatile("prefetch.tensormap [%0];" :: "l"(reinterpret_cast<u64>(&P.maps[m])) : "memory");
+    asm volatile("prefetch.tensormap [%0];" :: "l"(reinterpret_cast<u64>(J.ma)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" :: "l"(reinterpret_cast<u64>(J.mb)) : "memory");
   }
   if (threadIdx.x == 0) {
     for (u32 s = 0; s < STAGES; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
@@ -333,15 +345,15 @@ __device__ __forceinline__ void gemm_f16x3(const GemmParams& P, EPI& epi) {
             // a box holds a tile's hi plane and, behind it, its lo plane
             if (A_MN) {
 #pragma unroll
-              for (int c = 0; c < HG_M / 64; ++c) load(st + c * HG_K * 256, &P.maps[0], T.m0 + 64 * c, kc);
+              for (int c = 0; c < HG_M / 64; ++c) load(st + c * HG_K * 256, J.ma, T.m0 + 64 * c, kc);
             } else {
-              load(st, &P.maps[0], kc, T.m0);
+              load(st, J.ma, kc, T.m0);
             }
             if (B_MN) {
 #pragma unroll
-              for (int c = 0; c < BN / 64; ++c) load(sb + c * HG_K * 256, &P.maps[1], T.n0 + 64 * c, kc);
+              for (int c = 0; c < BN / 64; ++c) load(sb + c * HG_K * 256, J.mb, T.n0 + 64 * c, kc);
             } else {
-              load(sb, &P.maps[1], kc, T.n0);
+              load(sb, J.mb, kc, T.n0);
             }
           }
           __syncwarp();
@@ -402,6 +414,8 @@ __device__ __forceinline__ void gemm_f16x3(const GemmParams& P, EPI& epi) {
     e.q = warp & 3;
     e.c0 = w / 4 * (BN / 2);
     e.lane = lane;
+    e.M = M;
+    e.N = N;
     e.stage = staging + (u32)w * 4096;
     e.gstage = gbase + (e.stage - base);
     epi.start(e.gstage - w * 4096);
@@ -429,13 +443,13 @@ __device__ __forceinline__ void gemm_f16x3(const GemmParams& P, EPI& epi) {
       if (mine && !work.whole()) {
         // CTA c's slots: 2 c + 1 for the beginning of a tile, 2 c for a later part of one
         constexpr u64 SLOT = (u64)8 * NB * 1024;
-        float* part = reinterpret_cast<float*>(P.a.scratch + (u64)P.a.p[3]) + (u64)w * NB * 1024 + lane;
-        f16_partial_store<0>(v, part + (2 * blockIdx.x + (work.c0 == 0)) * SLOT);
+        float* part = J.part + (u64)w * NB * 1024 + lane;
+        f16_partial_store<0>(v, part + (2 * J.block + (work.c0 == 0)) * SLOT);
         __threadfence();
         __syncwarp();
         const u64 first = (u64)(work.tile - work.full) * work.per;
         const u32 ca = work.owner(first), cb = work.owner(first + work.per - 1);
-        u32* count = reinterpret_cast<u32*>(P.a.p[15]) + 4 + (work.tile - work.full) * 8 + w;
+        u32* count = J.counters + (work.tile - work.full) * 8 + w;
         u32 old = 0;
         if (lane == 0) old = atomicAdd(count, 1u);
         old = __shfl_sync(0xffffffffu, old, 0);
@@ -471,7 +485,7 @@ __device__ __forceinline__ void f16_clear(const Args& a, u32 n) {
   if (blockIdx.x == 0 && blockIdx.y == 0 && a.p[15])
     for (u32 i = threadIdx.x; i < n; i += blockDim.x) reinterpret_cast<u32*>(a.p[15])[i] = 0u;
 }
-constexpr u32 F16_CTRL = 4 + 8 * 2 * 148;   // words: the error word, 8 counters for each of up to 2 tiles an SM
+constexpr u32 F16_CTRL = 4 + 8 * 2 * 148;   // words: the error word, 8 counters for each divided tile of two products
 
 // 32 columns of hi / lo pairs through the warp's staging block to two planes of an fp16 array by TMA
 // store (map: {cols, rows, planes}, boxes of 32 x 32 x 2, 64-byte swizzle).

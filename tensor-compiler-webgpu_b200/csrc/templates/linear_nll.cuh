@@ -9,25 +9,25 @@
 // takes and gives no gradient, and what its row of h holds is never used.
 //
 // Forward: one matrix product (tcb/gemm_f16x3.cuh) whose epilogue keeps, per row and half tile of columns,
-// the running maximum and the sum of exponentials; tcb_nll_finish joins a row's tiles.  The logits exist in
-// tensor memory and registers only, in units of log 2: z2 = log2(e) z is one fma from the sums, its
+// the running maximum and the sum of exponentials; the last to arrive at 32 rows joins their tiles (a launch of
+// its own, tcb_nll_finish, when they are many).  The logits exist in tensor memory and registers only, in units of log 2: z2 = log2(e) z is one fma from the sums, its
 // exponential one ex2 (2^-22 relative, as far off as the operands' split).
 // What the backward needs of it is saved in one opaque value (NllSaved): the scales, b log2(e), each
 // row's log2 of the sum, and h and W as split for the tensor core, 4 bytes a value.
 // Backward: the vocabulary is walked in pieces (a bounded workspace).  A piece's logits are computed
 // again, turned into dz in the epilogue -- as fp16 hi / lo, what the two products after it read;
 // |dz| <= |g_i|, so its scale is known before -- and dh += dz W_piece^T and dW_piece = h^T dz follow.
-// db's column sums are taken in the dz epilogue.
+// db's column sums are taken in the dz epilogue, and added up there (or by tcb_nll_db) in the same way.
 //
 // dz below 2^-40 of the largest |g_i| rounds to zero, and keeps fewer than 22 bits below 2^-18 of it: the
 // gradient of a class whose probability is that small in every row has that absolute accuracy, which is
 // beneath the float32 rounding of the sums it enters.
 //
 // p[] of every kernel: [0..3] the product's (split: [0] blocks of the amax launch; finish: [0] half tiles of a
-// row), [4] R, [5] d, [6] V, [7] byte offset of the saved value in scratch (a forward whose backward nobody
-// asks for), [8..10] byte offsets in it of the row sums, h and W, [11] byte offset in scratch of the targets'
+// row), [4] R, [5] d, [6] V, [7] byte offset of the saved value in scratch (when nobody asks for a backward;
+// else the address of the loss), [8..10] byte offsets in it of the row sums, h and W, [11] byte offset in scratch of the targets'
 // logits (backward: of the column-sum partials), [12] of the row partials (backward: the piece's first
-// column), [13] 1 to add to dh, [14] address of the saved value or 0.
+// column), [13] flags, [14] address of the saved value or 0 (dz: of db or 0).
 // in[]: h, W, (b), t forward; t, saved, the loss's cotangent backward.
 #pragma once
 #include "tcb/gemm_f16x3.cuh"
@@ -38,6 +38,8 @@
 
 namespace tcb {
 
+constexpr u32 NLL_ADD = 1, NLL_JOIN = 2, NLL_NO_LOSS = 4;   // flags: add to dh; join in the product's kernel; no loss
+constexpr u32 NLL_CTRL = F16_CTRL + 512;   // words of the control block: a counter more for each 32 rows or columns joined
 constexpr float NLL_LOG2E = 1.44269504f, NLL_LN2 = 0.693147181f, NLL_MAX = 3.402823466e38f;
 #define TCB_MINUS_INF bits(0xff800000u)
 
@@ -132,14 +134,14 @@ __device__ __forceinline__ void split_matrix(const float* x, u32* out, u64 rows,
 // resident program's is its own, and zero between runs).
 extern "C" __global__ void __launch_bounds__(128) tcb_gemm_prep(const tcb::Args a) {
   tcb::grid_dependency_sync();
-  tcb::f16_clear(a, tcb::F16_CTRL);
+  tcb::f16_clear(a, tcb::NLL_CTRL);
 }
 
 // Largest magnitudes of h (rows that take part) and W, a partial pair per block.
 extern "C" __global__ void __launch_bounds__(256) tcb_nll_amax(const tcb::Args a) {
   using namespace tcb;
   grid_dependency_sync();
-  f16_clear(a, F16_CTRL);
+  f16_clear(a, NLL_CTRL);
   __shared__ float sh[8];
   const Nll<false> n(a);
   const u64 R = n.R(), d = n.d(), V = n.V();
@@ -230,6 +232,47 @@ __device__ __forceinline__ u32 nll_bit(int t, u32 col) {
   return t >= (int)col && t < (int)col + 32 ? 1u << (t - (int)col) : 0u;
 }
 
+// A warp's arrival at one of n: true, in all lanes, for the last, which leaves the counter at zero.
+__device__ __forceinline__ bool nll_last(const Args& a, u32 counter, u32 n, int lane) {
+  __threadfence();
+  __syncwarp();
+  u32* c = reinterpret_cast<u32*>(a.p[15]) + 4 + 8 * 2 * 148 + counter;   // behind the divided tiles' counters
+  u32 old = 0;
+  if (lane == 0) old = atomicAdd(c, 1u);
+  const bool last = __shfl_sync(0xffffffffu, old, 0) == n - 1;
+  if (last) {
+    if (lane == 0) *c = 0u;
+    __threadfence();
+  }
+  return last;
+}
+__device__ __forceinline__ void nll_join(float& m, float& s, const float2& x) {
+  const float mx = fmaxf(m, x.x), safe = mx == TCB_MINUS_INF ? 0.0f : mx;
+  s = s * ex2(m - safe) + x.y * ex2(x.x - safe);
+  m = mx;
+}
+// Half tiles k, k + step, ... of a row joined, eight loads in flight.
+__device__ __forceinline__ void nll_join_tiles(const float2* part, u64 R, u64 row, u32 k, u32 step, u32 tiles, float& m,
+                                               float& s) {
+  m = TCB_MINUS_INF;
+  s = 0.0f;
+  for (; k + 7 * step < tiles; k += 8 * step) {
+    float2 x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = __ldcg(part + (u64)(k + i * step) * R + row);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) nll_join(m, s, x[i]);
+  }
+  for (; k < tiles; k += step) nll_join(m, s, __ldcg(part + (u64)k * R + row));
+}
+__device__ __forceinline__ void nll_write(const Nll<false>& n, u64 row, float m, float s) {
+  const Args& a = n.a;
+  if (!((u32)a.p[13] & NLL_NO_LOSS))
+    reinterpret_cast<float*>(a.p[14] ? (u64)a.p[7] : a.out)[row] =
+        n.target(row) >= 0 ? (m - __ldcg(n.scratch<float>((u64)a.p[11]) + row)) * NLL_LN2 + logf(s) : 0.0f;
+  n.lse2()[row] = m + log2f(s);
+}
+
 // Forward epilogue: a row's maximum and sum of exponentials over the half tile's columns, the target's
 // logit.  Columns of -inf (a masked part of the vocabulary, the padding) leave the sum alone.
 template <int BN>
@@ -272,8 +315,13 @@ struct NllForward {
   }
   __device__ __forceinline__ void end(const F16Epi& e) {
     const Nll<false> n(a);
-    if (e.row < n.R())
-      n.template scratch<float2>((u64)a.p[12])[(u64)(e.T.n0 + e.c0) / (BN / 2) * n.R() + e.row] = make_float2(m, s);
+    float2* part = n.template scratch<float2>((u64)a.p[12]);
+    if (e.row < n.R()) part[(u64)(e.T.n0 + e.c0) / (BN / 2) * n.R() + e.row] = make_float2(m, s);
+    if (!((u32)a.p[13] & NLL_JOIN)) return;
+    const u32 halves = ((u32)n.V() + BN / 2 - 1) / (BN / 2);
+    if (!nll_last(a, (u32)e.T.m0 / 32 + e.q, halves, e.lane) || e.row >= n.R()) return;
+    nll_join_tiles(part, n.R(), e.row, 0, 1, halves, m, s);
+    nll_write(n, e.row, m, s);
   }
   __device__ __forceinline__ void done(const F16Epi&) {}
 };
@@ -338,8 +386,16 @@ struct NllDz {
     }
     store_split32(e, map, v, (int)(pc & 255), e.T.m0 + 32 * e.q, (int)(pc >> 8));
     const float sum = column_sums32(v, e.lane);
-    if (col + e.lane < (u32)n.V())
-      n.template scratch<float>((u64)a.p[11])[((u64)e.T.m0 / 32 + e.q) * n.V() + col + e.lane] = sum * down;
+    float* part = n.template scratch<float>((u64)a.p[11]) + col + e.lane;
+    const bool in = col + e.lane < (u32)n.V();
+    if (in) part[((u64)e.T.m0 / 32 + e.q) * n.V()] = sum * down;
+    if (!((u32)a.p[13] & NLL_JOIN)) return;
+    const u32 rows = ((u32)n.R() + 31) / 32;
+    if (!nll_last(a, col / 32, rows, e.lane) || !in) return;
+    float x = 0.0f;
+#pragma unroll 8
+    for (u32 k = 0; k < rows; ++k) x += __ldcg(part + (u64)k * n.V());
+    reinterpret_cast<float*>(a.p[14])[col + e.lane] = x;
   }
   __device__ __forceinline__ void end(const F16Epi&) {}
   __device__ __forceinline__ void done(const F16Epi& e) {
@@ -351,8 +407,9 @@ struct NllDz {
 template <bool DW>
 struct NllOut {
   const Args& a;
+  float* out;
   float x, y;
-  __device__ __forceinline__ explicit NllOut(const Args& args) : a(args) {}
+  __device__ __forceinline__ NllOut(const Args& args, u64 o) : a(args), out(reinterpret_cast<float*>(o)) {}
   __device__ __forceinline__ void start(unsigned char*) {
     const Nll<true> n(a);
     x = DW ? n.scales()->down_h : n.scales()->down_w;
@@ -361,15 +418,15 @@ struct NllOut {
   __device__ __forceinline__ void begin(const F16Epi&) {}
   __device__ __forceinline__ void block(const F16Epi& e, int c0, float (&v)[32]) {
     turn32(e, v);
-    const u32 M = (u32)a.p[0], N = (u32)((u64)a.p[0] >> 32), col = (u32)(e.T.n0 + c0) + e.lane;
-    if (col >= N) return;
+    const u32 col = (u32)(e.T.n0 + c0) + e.lane;
+    if (col >= e.N) return;
     const u64 ld = DW ? (u64)a.p[6] : (u64)a.p[5];
     const u32 row0 = (u32)e.T.m0 + 32 * e.q;
-    float* o = reinterpret_cast<float*>(a.out) + row0 * ld + (DW ? (u64)a.p[12] : 0) + col;
-    const int rows = (int)(M - row0 < 32 ? M - row0 : 32);
+    float* o = out + row0 * ld + (DW ? (u64)a.p[12] : 0) + col;
+    const int rows = (int)(e.M - row0 < 32 ? e.M - row0 : 32);
 #pragma unroll
     for (int r = 0; r < 32; ++r) v[r] = v[r] * x * y;
-    if (!DW && a.p[13]) {
+    if (!DW && ((u32)a.p[13] & NLL_ADD)) {
 #pragma unroll
       for (int r = 0; r < 32; ++r)
         if (r < rows) v[r] += o[(u64)r * ld];
@@ -384,21 +441,49 @@ struct NllOut {
 
 }  // namespace tcb
 
-#define TCB_NLL_GEMM(NAME, BN, AMN, BMN, EPI, ARG)                                                                          \
+#define TCB_NLL_GEMM(NAME, BN, AMN, BMN, EPI, ...)                                                                          \
   extern "C" __global__ void __launch_bounds__(tcb::HG_THREADS, 1) NAME##_##BN(const __grid_constant__ tcb::GemmParams P) { \
-    tcb::EPI epi(ARG);                                                                                                      \
-    tcb::gemm_f16x3<BN, AMN, BMN, false, true, 256>(P, epi);                                                                      \
+    tcb::EPI epi(__VA_ARGS__);                                                                                              \
+    tcb::gemm_f16x3<BN, AMN, BMN, false, true, 256>(tcb::f16_job(P), reinterpret_cast<u32*>(P.a.p[15]), epi);               \
   }
 // logits and dz: h K-major, W MN-major (its rows run along the vocabulary); dh: dz and W K-major (along the
 // vocabulary); dW: h^T and dz, both MN-major (along d and along the vocabulary)
-#define TCB_NLL_GEMMS(BN)                                            \
-  TCB_NLL_GEMM(tcb_nll_logits, BN, false, true, NllForward<BN>, P.a) \
-  TCB_NLL_GEMM(tcb_nll_dz, BN, false, true, NllDz, P)                \
-  TCB_NLL_GEMM(tcb_nll_dh, BN, false, false, NllOut<false>, P.a)     \
-  TCB_NLL_GEMM(tcb_nll_dw, BN, true, true, NllOut<true>, P.a)
+#define TCB_NLL_GEMMS(BN)                                                   \
+  TCB_NLL_GEMM(tcb_nll_logits, BN, false, true, NllForward<BN>, P.a)        \
+  TCB_NLL_GEMM(tcb_nll_dz, BN, false, true, NllDz, P)                       \
+  TCB_NLL_GEMM(tcb_nll_dh, BN, false, false, NllOut<false>, P.a, P.a.out)   \
+  TCB_NLL_GEMM(tcb_nll_dw, BN, true, true, NllOut<true>, P.a, P.a.out)
 TCB_NLL_GEMMS(256)
 TCB_NLL_GEMMS(128)
 TCB_NLL_GEMMS(64)
+
+// dh and dW in one launch where their CTAs find room side by side: the first p[14] CTAs are dh's, maps 2 and 3,
+// p[7] (plan), p[8] (partial sums) and p[9] (address) dW's.
+template <int BH, int BW>
+__device__ __forceinline__ void nll_both(const tcb::GemmParams& P) {
+  using namespace tcb;
+  const Args& a = P.a;
+  u32* err = reinterpret_cast<u32*>(a.p[15]);
+  F16Job j = f16_job(P);
+  if (blockIdx.x < (u32)a.p[14]) {
+    j.grid = (u32)a.p[14];
+    NllOut<false> epi(a, a.out);
+    gemm_f16x3<BH, false, false, false, true, 256>(j, err, epi);
+  } else {
+    j = F16Job{&P.maps[2], &P.maps[3], (u32)a.p[5], j.K, j.M, 1, (u32)a.p[7], (u32)((u64)a.p[7] >> 32),
+               blockIdx.x - (u32)a.p[14], gridDim.x - (u32)a.p[14], reinterpret_cast<float*>(a.scratch + (u64)a.p[8]),
+               j.counters + 8 * 148};
+    NllOut<true> epi(a, (u64)a.p[9]);
+    gemm_f16x3<BW, true, true, false, true, 256>(j, err, epi);
+  }
+}
+#define TCB_NLL_BOTH(BH, BW)                                                                                          \
+  extern "C" __global__ void __launch_bounds__(tcb::HG_THREADS, 1)                                                    \
+      tcb_nll_both_##BH##_##BW(const __grid_constant__ tcb::GemmParams P) { nll_both<BH, BW>(P); }
+TCB_NLL_BOTH(64, 64)
+TCB_NLL_BOTH(64, 128)
+TCB_NLL_BOTH(128, 64)
+TCB_NLL_BOTH(128, 128)
 
 // Joins a row's tiles: a block of 8 warps takes 32 rows, warp k the half tiles k, k + 8, ...
 extern "C" __global__ void __launch_bounds__(256) tcb_nll_finish(const tcb::Args a) {
@@ -408,32 +493,13 @@ extern "C" __global__ void __launch_bounds__(256) tcb_nll_finish(const tcb::Args
   const Nll<false> n(a);
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const u64 R = n.R(), row = (u64)blockIdx.x * 32 + lane;
-  const u32 tiles = (u32)a.p[0];
-  const float2* part = n.scratch<float2>((u64)a.p[12]);
   float m = TCB_MINUS_INF, s = 0.0f;
-  auto join = [&](const float2& x) {
-    const float mx = fmaxf(m, x.x), safe = mx == TCB_MINUS_INF ? 0.0f : mx;
-    s = s * ex2(m - safe) + x.y * ex2(x.x - safe);
-    m = mx;
-  };
-  if (row < R) {
-    u32 k = w;
-    for (; k + 56 < tiles; k += 64) {   // eight loads in flight
-      float2 x[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = part[(u64)(k + 8 * i) * R + row];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) join(x[i]);
-    }
-    for (; k < tiles; k += 8) join(part[(u64)k * R + row]);
-  }
+  if (row < R) nll_join_tiles(n.scratch<float2>((u64)a.p[12]), R, row, w, 8, (u32)a.p[0], m, s);
   sh[w][lane] = make_float2(m, s);
   __syncthreads();
   if (w == 0 && row < R) {
-    for (int k = 1; k < 8; ++k) join(sh[k][lane]);
-    const bool in = n.target(row) >= 0;
-    reinterpret_cast<float*>(a.out)[row] = in ? (m - n.scratch<float>((u64)a.p[11])[row]) * NLL_LN2 + logf(s) : 0.0f;
-    n.lse2()[row] = m + log2f(s);
+    for (int k = 1; k < 8; ++k) nll_join(m, s, sh[k][lane]);
+    nll_write(n, row, m, s);
   }
 }
 

@@ -143,6 +143,17 @@ def siblings(graph):
 
 # ------------------------------------------------------------------ linearNll
 NLL_CHUNK = 256
+# Rows (in 32s) of a forward whose tiles, columns (in 32s) of a backward whose row sums are joined in the
+# product's own kernel, and the most parts a warp then adds up on its own
+JOIN_COUNTERS, JOIN_PARTS = 512, 4
+NLL_CTRL_BYTES = CTRL_BYTES + 4 * JOIN_COUNTERS
+NLL_ADD, NLL_JOIN, NLL_NO_LOSS = 1, 2, 4
+
+
+def _joined(groups, parts):
+    """Joining in the product's kernel saves a launch (64 x 64 x 65: 24.9 us to 22.8), but every part's warp waits for
+    its stores and an atomic (4095 x 256 x 8192 with up to 64 parts: 231 us to 269): for few parts only."""
+    return groups <= JOIN_COUNTERS and parts <= JOIN_PARTS
 
 
 def nll_pieces(R, V):
@@ -180,9 +191,11 @@ def _nll_launch(graph, ids):
     plan = f16_plan(R, V, d, 1, NLL_CHUNK)
     bn = plan[0]
     halves = math.ceil(V / (bn // 2))
-    at, end = _regions(("amax", 8 * AMAX_BLOCKS), ("err", CTRL_BYTES), ("zt", 4 * R), ("part", 8 * R * halves),
+    at, end = _regions(("amax", 8 * AMAX_BLOCKS), ("err", NLL_CTRL_BYTES), ("zt", 4 * R), ("part", 8 * R * halves),
                        ("loss", 0 if "loss" in by else 4 * R), ("saved", 0 if "saved" in by else 4 * floats))
-    tail = [R, d, V, at["saved"], inner["lse"], inner["h"], inner["w"], at["zt"], at["part"], 0]
+    joined = _joined(math.ceil(R / 32), halves)
+    flags = (NLL_JOIN if joined else 0) | (0 if "loss" in by else NLL_NO_LOSS)
+    tail = [R, d, V, at["saved"], inner["lse"], inner["h"], inner["w"], at["zt"], at["part"], flags]
     if "saved" in by:
         def saved(off):
             return "out", off
@@ -196,18 +209,18 @@ def _nll_launch(graph, ids):
     gemm, partial = _gemm("tcb_nll_logits", R, V, d, 1, plan, end, maps, tail)
     calls = [KernelCall("tcb_nll_amax", (blocks, 1, 1), (256, 1, 1), 0, [blocks, 0, 0, 0, *tail]),
              KernelCall("tcb_nll_split", (max(2, min(units, SM_COUNT * 8)), 1, 1), (256, 1, 1), 0, [blocks, 0, 0, 0, *tail]),
-             gemm, KernelCall("tcb_nll_finish", (math.ceil(R / 32), 1, 1), (256, 1, 1), 0, [halves, 0, 0, 0, *tail])]
+             gemm]
+    if not joined:
+        calls.append(KernelCall("tcb_nll_finish", (math.ceil(R / 32), 1, 1), (256, 1, 1), 0, [halves, 0, 0, 0, *tail]))
     calls[0].err_offset = gemm.err_offset = at["err"]
-    if "saved" in by:
+    if "saved" in by:   # `out` is then the saved value, which the product's maps lie in, and the loss an address
         for c in calls:
-            c.ptr_params = ((14, by["saved"]),)
-        if by["saved"] != node.id:
-            gemm.out_node = by["saved"]
-        if node.id == by["saved"]:   # the loss comes second, or nobody asked for it
-            calls[3].out_node = by.get("loss")
+            c.ptr_params = ((14, by["saved"]),) + (((7, by["loss"]),) if "loss" in by else ())
+            if by["saved"] != node.id:
+                c.out_node = by["saved"]
     return Launch(node.id, node.op, "linear-nll", None, node.inputs, nll_source(node.attrs["bias"]), calls,
                   scratch_bytes=end + _up(partial, 256),
-                  info={"rnv": (R, d, V), "bn": bn, "ctrl_bytes": _up(CTRL_BYTES, 64), "path": "tcgen05-f16x3"})
+                  info={"rnv": (R, d, V), "bn": bn, "ctrl_bytes": _up(NLL_CTRL_BYTES, 64), "path": "tcgen05-f16x3"})
 
 
 def _nll_grad_launch(graph, ids):
@@ -217,8 +230,9 @@ def _nll_grad_launch(graph, ids):
     inner, _ = linear_nll_saved(R, d, V)
     piece, pieces = nll_pieces(R, V)
     want = {graph.nodes[i].attrs["wrt"]: i for i in ids}
-    at, end = _regions(("scale", 256), ("err", CTRL_BYTES), ("dz", 4 * R * _up(piece, 256 if piece > 256 else 32)), ("db", 4 * math.ceil(R / 32) * V))
+    at, end = _regions(("scale", 256), ("err", NLL_CTRL_BYTES), ("dz", 4 * R * _up(piece, 256 if piece > 256 else 32)), ("db", 4 * math.ceil(R / 32) * V))
     tail = [R, d, V, 0, inner["lse"], inner["h"], inner["w"], at["db"]]
+    joined = "b" in want and _joined(math.ceil(V / 32), math.ceil(R / 32))
     calls, partial = [], 0
 
     def add(name, wrt, M, N, K, maps, params):
@@ -233,7 +247,7 @@ def _nll_grad_launch(graph, ids):
     for k in range(pieces):
         v0 = k * piece
         n = min(piece, V - v0)
-        params = [*tail, v0, int(k > 0)]
+        params = [*tail, v0, (NLL_ADD if k else 0) | (NLL_JOIN if joined else 0)]
         w_at = inner["w"] + (4 * d * v0 if v0 else 0)   # pieces begin with a block
 
         def h(mn):
@@ -246,11 +260,29 @@ def _nll_grad_launch(graph, ids):
             return _blocked_operand("scratch", at["dz"], R, n, _pitch(n), mn, bn)
         out = _blocked("scratch", at["dz"], R, n, _pitch(n), 32, 32)
         add("tcb_nll_dz", None, R, n, d, lambda bn: h(False) + w(True, bn) + out, params)
+        if joined:
+            calls[-1].ptr_params = ((14, want["b"]),)
+        ph, pw = f16_plan(R, d, n, 1, NLL_CHUNK), f16_plan(d, n, R, 1, NLL_CHUNK)
+        if "h" in want and "w" in want and max(ph[0], pw[0]) <= 128 and ph[1] + pw[1] <= SM_COUNT:
+            # both find room side by side
+            c, hb = _gemm("tcb_nll_both", R, d, n, 1, ph, end, z(False, F16_BM) + w(False, ph[0]) + h(True) + z(True, pw[0]), params)
+            wb = f16_partial_bytes(pw[1], pw[2], f16_tiles(d, n, pw[0], False), pw[0])
+            c.name = f"tcb_nll_both_{ph[0]}_{pw[0]}"
+            c.grid, c.smem = (ph[1] + pw[1], 1, 1), max(f16_smem(ph[0]), f16_smem(pw[0]))
+            c.params[7:9] = [pw[2] | pw[3] << 32, end + _up(hb, 256)]
+            c.params += [ph[1]]
+            c.ptr_params = ((9, want["w"]),)
+            c.err_offset = at["err"]
+            if want["h"] != node.id:
+                c.out_node = want["h"]
+            partial = max(partial, _up(hb, 256) + wb)
+            calls.append(c)
+            continue
         if "h" in want:
             add("tcb_nll_dh", "h", R, d, n, lambda bn: z(False, F16_BM) + w(False, bn), params)
         if "w" in want:
             add("tcb_nll_dw", "w", d, n, R, lambda bn: h(True) + z(True, bn), params)
-    if "b" in want:
+    if "b" in want and not joined:
         db = KernelCall("tcb_nll_db", (math.ceil(V / 32), 1, 1), (256, 1, 1), 0, [0, 0, 0, 0, *tail, 0, 0])
         if want["b"] != node.id:
             db.out_node = want["b"]
@@ -260,7 +292,7 @@ def _nll_grad_launch(graph, ids):
     clear.err_offset = at["err"]
     return Launch(node.id, node.op, "linear-nll-grad", None, node.inputs, nll_source(node.attrs["bias"]), [clear] + calls,
                   scratch_bytes=end + _up(partial, 256),
-                  info={"rnv": (R, d, V), "pieces": pieces, "ctrl_bytes": _up(CTRL_BYTES, 64), "path": "tcgen05-f16x3"})
+                  info={"rnv": (R, d, V), "pieces": pieces, "ctrl_bytes": _up(NLL_CTRL_BYTES, 64), "path": "tcgen05-f16x3"})
 
 
 # ------------------------------------------------------------------ headNormRope
