@@ -2,7 +2,7 @@
 
 * ``linearNll`` / ``linearNllGrad``       -- tcb/linear_nll.cuh
 * ``headNormRope`` / ``headNormRopeGrad`` -- tcb/head_norm_rope.cuh
-* ``orthogonalize``                       -- tcb/orthogonalize.cuh
+* ``orthogonalize``                       -- tcb/orthogonalize.cuh, tcb/orth_small.cuh
 
 Each node is one launch of a few kernel calls.  Siblings -- the gradients of one node, which differ in
 ``wrt`` only; a loss and what it saves for its backward, which differ in ``out`` -- are one launch with several
@@ -362,19 +362,31 @@ NS_PARTS = 512
 NS_CHUNK = 128
 
 
-def orth_source(steps, coeffs, eps):
+ORTH_SMALL = ((64, 512), (128, 128))   # (short, long) sides of matrices that fit one SM
+
+
+def orth_small(s, long):
+    """The (short, long) limits of the one-SM form a matrix fits, or None."""
+    for rows, cols in ORTH_SMALL:
+        if s <= rows and long <= cols:
+            return rows, cols
+    return None
+
+
+def orth_source(steps, coeffs, eps, small=None):
     from .codegen import f32_literal
     ex, es, ep = newton_schulz_scales(steps, coeffs)
-    return f"""// Newton-Schulz orthogonalisation
+    limits = f"#define TCB_ROWS {small[0]}\n#define TCB_COLS {small[1]}\n" if small else ""
+    return f"""// Newton-Schulz orthogonalisation{' on one SM' if small else ''}
 #include "tcb/common.cuh"
-#define TCB_EX {ex}
+{limits}#define TCB_EX {ex}
 #define TCB_ES {es}
 #define TCB_EP {ep}
 #define TCB_NS_A {f32_literal(coeffs[0])}
 #define TCB_NS_B {f32_literal(coeffs[1])}
 #define TCB_NS_C {f32_literal(coeffs[2])}
 #define TCB_NS_EPS {f32_literal(eps)}
-#include "tcb/orthogonalize.cuh"
+#include "tcb/{'orth_small' if small else 'orthogonalize'}.cuh"
 """
 
 
@@ -385,6 +397,15 @@ def _orth_launch(graph, node):
     a = node.attrs
     tall = m > n
     s = min(m, n)
+    small = orth_small(s, max(m, n))
+    if small:
+        rows, cols = small
+        block = 2 * rows * 128
+        c = KernelCall("tcb_orth_small", (batch, 1, 1), (256, 1, 1), (cols // 64 + 2 * (rows // 64)) * block + 16384 + 1024,
+                       [m, n, a["steps"]])
+        c.err_offset = 0
+        return Launch(node.id, node.op, "orthogonalize", None, node.inputs, orth_source(a["steps"], a["coeffs"], a["eps"], small),
+                      [c], scratch_bytes=256, info={"mn": (batch, m, n), "ctrl_bytes": 64, "path": "tcgen05-f16x3"})
     xp, sp = _up(n, 8), _up(s, 8)
     xplane, splane = 2 * batch * m * xp, 2 * batch * s * sp
     parts = max(1, min(NS_PARTS, math.ceil(m * n / 4096)))

@@ -280,6 +280,19 @@ def check_orth(mods, runner, pkg, x, **kw):
     return got
 
 
+@pytest.mark.parametrize("shape", [(1, 1), (3, 64, 50), (64, 512), (500, 63), (17, 511), (1, 300), (128, 128), (2, 127, 65), (66, 128),
+                                   (40, 130), (64, 257), (256, 64)])
+def test_orthogonalize_both_forms(pkg, mods, runner, monkeypatch, shape):
+    """What fits one SM, and the same by the launches of larger matrices."""
+    to = importlib.import_module(P + ".training_ops")
+    x = f32(np.random.default_rng(shape[-1]).standard_normal(shape))
+    assert to.orth_small(min(shape[-2:]), max(shape[-2:])) if len(shape) > 1 else True
+    a = check_orth(mods, runner, pkg, x)
+    monkeypatch.setattr(to, "orth_small", lambda s, long: None)
+    b = check_orth(mods, runner, pkg, x)
+    assert np.allclose(a, b, atol=1e-3)
+
+
 @pytest.mark.parametrize("shape", [(1, 1), (2, 3), (16, 16), (64, 64), (65, 64), (64, 65), (100, 70), (3, 70, 300),
                                    (2, 2, 129, 128), (128, 257), (257, 130), (256, 1024), (700, 512), (5, 1000), (1000, 5)])
 def test_orthogonalize(pkg, mods, runner, shape):

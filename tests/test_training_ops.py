@@ -303,6 +303,9 @@ def test_orthogonalize_scratch(mods, shape):
     g = pkg.ir.Graph()
     g.orthogonalize(g.input("x", shape))
     (lau,) = cg.lower(g)["launches"]
+    if to.orth_small(min(shape[-2:]), max(shape[-2:])):
+        assert len(lau.calls) == 1 and lau.calls[0].smem <= 227 * 1024 and lau.calls[0].err_offset is not None
+        return
     assert len(lau.calls) == 2 + 15
     for c in lau.calls:
         for region, off, cols, rows, batch, rs, bs, bc, br in c.tma or []:
@@ -331,10 +334,12 @@ def test_head_launch_geometry(mods, B, T, H, D, rot):
             assert lau.scratch_bytes == main.grid[0] * D * 4
 
 
-@pytest.mark.parametrize("which", ["nll", "nll-bias", "orth", "head-64", "head-odd", "head-none"])
+@pytest.mark.parametrize("which", ["nll", "nll-bias", "orth", "orth-64", "orth-128", "head-64", "head-odd", "head-none"])
 def test_sources_compile(mods, which):
     pkg, cg, to, rt = mods
     code = {"nll": lambda: to.nll_source(False), "nll-bias": lambda: to.nll_source(True),
-            "orth": lambda: to.orth_source(5, pkg.ir.NEWTON_SCHULZ, 1e-7), "head-64": lambda: to.head_source(64, 64, False),
+            "orth": lambda: to.orth_source(5, pkg.ir.NEWTON_SCHULZ, 1e-7),
+            "orth-64": lambda: to.orth_source(5, pkg.ir.NEWTON_SCHULZ, 1e-7, (64, 512)),
+            "orth-128": lambda: to.orth_source(5, pkg.ir.NEWTON_SCHULZ, 1e-7, (128, 128)), "head-64": lambda: to.head_source(64, 64, False),
             "head-odd": lambda: to.head_source(33, 6, True), "head-none": lambda: to.head_source(7, 0, False)}[which]()
     assert rt.compile_check(code) > 0
