@@ -1650,6 +1650,8 @@ static Launch mo_launch(const Graph& g, const Node& P, const Node& Q) {
   return l;
 }
 
+#include "lower_training.h"
+
 // ---------------------------------------------------------------- lower / lowerFused / fusedKernel
 static Launch fused_kernel(const Node& node, const std::string& matmul, const std::string& sabotage) {
   const Graph& body = *node.body;
@@ -1701,6 +1703,7 @@ static void lower_graph(Lowering& L, const Options& o) {
   }
   std::set<int> readers;
   for (auto& kv : mos) readers.insert(kv.second);
+  const std::map<int, std::vector<int>> groups = siblings(g);
   for (auto& node : g.nodes) {
     if (node.op == "input" || node.op == "const" || folds.count(node.id) || readers.count(node.id) ||
         tmats.count(node.id))
@@ -1721,6 +1724,11 @@ static void lower_graph(Lowering& L, const Options& o) {
     if (sums.count(node.id)) {
       auto [pid, write, row] = sums[node.id];
       if (!write) L.launches.push_back(row ? rowsum_launch(g, g.nodes[pid], node, false) : colsum_launch(g, g.nodes[pid], node, false));
+      continue;
+    }
+    if (is_training(node.op)) {
+      Launch t;
+      if (training_launch(g, node, groups, &t)) L.launches.push_back(std::move(t));
       continue;
     }
     std::pair<int, int> ab;

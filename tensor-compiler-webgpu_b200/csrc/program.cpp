@@ -215,6 +215,7 @@ int prepare_call(const Call& c, const std::vector<uint64_t>& ins, uint64_t out, 
     uint64_t addr;
     if (m.region == "scratch") addr = scratch + (uint64_t)m.off;
     else if (m.region == "in") addr = ins.at((size_t)m.off);
+    else if (m.region == "in_at") addr = ins.at((size_t)(m.off & 7)) + (uint64_t)(m.off >> 3);
     else if (m.region == "out") addr = out + (uint64_t)m.off;
     else return tcb_detail::fail_msg(TC_ERR_INVALID, "tensor map over '" + m.region + "'");
     if (addr % 16) return tcb_detail::fail_msg(TC_ERR_INVALID, "call " + c.name + ": tensor map base is not 16-byte aligned");

@@ -343,3 +343,99 @@ def test_sources_compile(mods, which):
             "orth-128": lambda: to.orth_source(5, pkg.ir.NEWTON_SCHULZ, 1e-7, (128, 128)), "head-64": lambda: to.head_source(64, 64, False),
             "head-odd": lambda: to.head_source(33, 6, True), "head-none": lambda: to.head_source(7, 0, False)}[which]()
     assert rt.compile_check(code) > 0
+
+
+# ---------------------------------------------------------------- the library's own lowering
+def _graphs(pkg):
+    for R, d, V, bias, wrt in ((1, 1, 1, True, "hwb"), (64, 64, 65, True, "hwb"), (300, 64, 1000, False, "hw"), (2500, 8, 2500, True, "wb"),
+                               (4095, 256, 8192, True, "hwb"), (8192, 1024, 50001, True, "hwb"), (16384, 1024, 131072, True, ""),
+                               (57, 1365, 55301, True, "h"), (16384, 39, 50, True, "hwb"), (100, 513, 3, True, "b"),
+                               (70000, 64, 600, False, "hw"), (3, 40, 1 << 24, True, "hwb")):
+        g, h, w, b, y = nll_graph(pkg, R, d, V, bias)
+        ids = [{"h": h, "w": w, "b": b}[k] for k in wrt]
+        yield pkg.autodiff.grad(g, [y], ids).graph if wrt else g
+    for B, T, H, D, kw in ((1, 1, 4, 64, {}), (3, 1001, 5, 80, {"rotary": 40, "interleaved": True, "shared": False}), (2, 8191, 32, 128, {}),
+                           (512, 256, 4, 64, {"heads_first": False}), (1, 5, 3, 7, {"rotary": 6, "base": 500000, "eps": 0}),
+                           (2, 3, 1, 512, {"rotary": 0}), (9, 1, 33, 33, {"rotary": 2, "base": 0.5})):
+        g, x, gain, y = head_graph(pkg, B, T, H, D, **kw)
+        yield g
+        for wrt in ([x, gain], [x], [gain]):
+            yield pkg.autodiff.grad(g, [y], wrt).graph
+    for shape, kw in (([1, 1], {}), ([64, 64], {}), ([3, 128, 128], {}), ([63, 513], {}), ([4, 256, 1024], {}), ([4095, 1000], {}), ([4096, 4096], {}),
+                      ([2, 2, 129, 18], {"steps": 8, "coeffs": (1.5, -0.5, 0)}), ([700, 512], {"steps": 1, "coeffs": (1.875, -1.25, 0.375), "eps": 0}),
+                      ([14, 3593, 18], {}), ([1, 16384], {})):
+        g = pkg.ir.Graph()
+        g.orthogonalize(g.input("x", shape), **kw)
+        yield g
+
+
+def test_library_lowers_identically(mods):
+    """tc_lower_json makes the Python host's records, field for field."""
+    from test_lower_abi import _compare
+    pkg, cg, to, rt = mods
+    n = 0
+    for g in _graphs(pkg):
+        n += _compare(rt.lib(), cg, g)
+        n += _compare(rt.lib(), cg, g, fused=False)
+    assert n > 100
+    g, h, w, b, y = nll_graph(pkg, 300, 64, 1000)
+    y2 = g.linear_nll(h, w, b, g.input_id("t"))
+    assert _compare(rt.lib(), cg, pkg.autodiff.grad(g, [g.add(y, y2)], [h, b]).graph) > 4
+
+
+def test_library_lowers_the_training_step_identically(mods):
+    from test_lower_abi import _compare
+    pkg, cg, to, rt = mods
+    s = pkg.steps
+    cfg = s.make_config(T=40, d=64, H=4, L=2, ff=300, targets="index", rope=10000.0)
+    step = s.build_step3b(300, 3, cfg, opt=s.MUON_3B)
+    keep = [step["loss"], *step["outputs"].values()]
+    f = pkg.fuse.fuse(step["graph"], keep=keep)
+    kept = [f.index[i] for i in keep]
+    for kw in ({}, {"fold": True, "keep": kept, "colfuse": True, "mofuse": True}):
+        assert _compare(rt.lib(), cg, f.graph, matmul="tiled", **kw) > 100
+
+
+@pytest.mark.parametrize("change", [{"bias": False}, {"out": "logits"}, {"out": None}, {"bias": 1}])
+def test_library_refuses_bad_attributes(mods, change):
+    import ctypes
+    import json
+    pkg, cg, to, rt = mods
+    g, h, w, b, y = nll_graph(pkg, 5, 3, 7)
+    js = g.to_json()
+    js["nodes"][y]["attrs"].update(change)
+    out = ctypes.c_void_p()
+    assert rt.lib().tc_lower_json(json.dumps(js).encode(), b"{}", ctypes.byref(out)) == 1
+    assert b"linearNll" in rt.lib().tc_last_error()
+
+
+@pytest.mark.parametrize("node,shape", [("w", [4, 7]), ("t", [6]), ("b", [8]), ("y", [6]), ("h", [3])])
+def test_library_refuses_bad_shapes(mods, node, shape):
+    import ctypes
+    import json
+    pkg, cg, to, rt = mods
+    g, h, w, b, y = nll_graph(pkg, 5, 3, 7)
+    js = g.to_json()
+    for n in js["nodes"]:
+        if n["attrs"].get("name") == node or (node == "y" and n["op"] == "linearNll"):
+            n["shape"] = shape
+    out = ctypes.c_void_p()
+    assert rt.lib().tc_lower_json(json.dumps(js).encode(), b"{}", ctypes.byref(out)) == 1
+
+
+@pytest.mark.parametrize("op,change", [("head", {"rotary": 10}), ("head", {"rotary": 3}), ("head", {"eps": -1}), ("head", {"base": 0}),
+                                       ("head", {"headsFirst": 0}), ("head", {"interleaved": None}), ("orth", {"steps": 0}), ("orth", {"steps": 2.5}),
+                                       ("orth", {"coeffs": [1, 2]}), ("orth", {"coeffs": [400, 0, 0]}), ("orth", {"eps": -1})])
+def test_library_refuses_bad_settings(mods, op, change):
+    import ctypes
+    import json
+    pkg, cg, to, rt = mods
+    if op == "head":
+        g, _, _, y = head_graph(pkg, 2, 5, 3, 8)
+    else:
+        g = pkg.ir.Graph()
+        y = g.orthogonalize(g.input("x", [4, 4]))
+    js = g.to_json()
+    js["nodes"][y]["attrs"].update(change)
+    out = ctypes.c_void_p()
+    assert rt.lib().tc_lower_json(json.dumps(js).encode(), b"{}", ctypes.byref(out)) == 1
