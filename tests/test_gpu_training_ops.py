@@ -348,3 +348,92 @@ def test_runner_reads_every_node_with_canaries(pkg, mods, runner):
     graph, y = orth_case(pkg, [2, 70, 33])
     out = runner.run(graph, cg.lower(graph), {"x": np.ones((2, 70, 33))}, canary=True)
     assert all(out["canaryIntact"])
+
+
+def small_graphs(pkg):
+    graph, y, grads, x = nll_case(pkg, 150, 30, 200)
+    yield graph, [y, *grads.values()], x
+    graph, y, grads, x = nll_case(pkg, 700, 260, 3000, bias=False)
+    yield graph, [y, *grads.values()], x
+    graph, y, grads, x = head_case(pkg, 2, 21, 3, 20, 20, True)
+    yield graph, [y, *grads.values()], x
+    for shape in ([2, 70, 33], [3, 200, 300]):
+        graph, y = orth_case(pkg, shape)
+        yield graph, [y], {"x": f32(np.random.default_rng(1).standard_normal(shape))}
+
+
+def test_c_abi_runs_them_bit_for_bit(pkg, mods, runner):
+    """tc_lower_json -> tc_lowered_run and tc_program_*: the Python host's values."""
+    import ctypes
+    import json
+    rt, cg = mods
+    lib = rt.lib()
+    for graph, keep, x in small_graphs(pkg):
+        want = run_graph(mods, runner, graph, x, keep)
+        low = ctypes.c_void_p()
+        rt.check(lib.tc_lower_json(json.dumps(graph.to_json()).encode(), b'{"matmul": "tiled"}', ctypes.byref(low)))
+        N = len(graph.nodes)
+        ins, outs = (ctypes.c_void_p * N)(), (ctypes.c_void_p * N)()
+        held, got, intact = [], {}, (ctypes.c_int * N)()
+        for n in graph.nodes:
+            if n.op == "input":
+                held.append(np.ascontiguousarray(np.asarray(x[n.attrs["name"]], np.float32)))
+                ins[n.id] = held[-1].ctypes.data
+        for i in keep:
+            got[i] = np.zeros(graph.shape(i), np.float32)
+            outs[i] = got[i].ctypes.data
+        rt.check(lib.tc_lowered_run(runner.ctx, low, ins, outs, 1, intact))
+        assert all(intact)
+        k = (ctypes.c_int32 * len(keep))(*keep)
+        prog = ctypes.c_void_p()
+        rt.check(lib.tc_program_create(runner.ctx, low, k, len(keep), None, 0, 1, ctypes.byref(prog)))
+        for n in graph.nodes:
+            if n.op == "input":
+                a = np.ascontiguousarray(np.asarray(x[n.attrs["name"]], np.float32).reshape(-1))
+                rt.check(lib.tc_program_write(prog, n.id, a.ctypes.data, a.size))
+        for _ in range(2):
+            rt.check(lib.tc_program_run(prog))
+        rt.check(lib.tc_program_check(prog))
+        for i, w in zip(keep, want):
+            assert np.array_equal(got[i], w), graph.nodes[i].op
+            a = np.zeros(w.size, np.float32)
+            rt.check(lib.tc_program_read(prog, i, a.ctypes.data, a.size))
+            assert np.array_equal(a.reshape(w.shape), w), graph.nodes[i].op
+        rt.check(lib.tc_program_free(prog))
+        rt.check(lib.tc_lowered_free(low))
+
+
+def test_programs_on_two_streams_at_once(pkg, mods, runner):
+    """Captured programs share no workspace: run side by side, again and again, each gives its own values."""
+    import ctypes
+    rt, cg = mods
+    lib = rt.lib()
+    cases = [c for c in small_graphs(pkg)]
+    want = [run_graph(mods, runner, g, x, keep) for g, keep, x in cases]
+    progs, streams = [], []
+    try:
+        for g, keep, x in cases:
+            p = rt.Program(runner, g, cg.lower_fused(g, matmul="tiled", keep=keep), keep=keep, capture=True)
+            for n in g.inputs():
+                p.write(n.id, x[n.attrs["name"]])
+            progs.append(p)
+            s = ctypes.c_uint64()
+            rt.check(lib.tc_stream_create(runner.ctx, ctypes.byref(s)))
+            streams.append(s.value)
+        for _ in range(20):
+            for p, s in zip(progs, streams):
+                rt.check(lib.tc_plan_run_on(p.plan, s))
+        ev = rt.Events(runner, len(progs))
+        for k, s in enumerate(streams):
+            rt.check(lib.tc_event_record_on(runner.ctx, ev.ev[k], s))
+            rt.check(lib.tc_event_sync(ev.ev[k], 20000))
+        ev.free()
+        for p, (g, keep, x), w in zip(progs, cases, want):
+            p.check_errors()
+            for i, v in zip(keep, w):
+                assert np.array_equal(p.read(i).reshape(v.shape), v)
+    finally:
+        for p in progs:
+            p.free()
+        for s in streams:
+            rt.check(lib.tc_stream_destroy(runner.ctx, s))

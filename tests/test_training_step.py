@@ -144,3 +144,27 @@ def test_trainer_on_the_gpu(pkg, runner, capture):
                 now[n] = trainer.read([n])[n].astype(np.float64).reshape(np.shape(now[n]))
     finally:
         trainer.destroy()
+
+
+@pytest.mark.gpu
+def test_data_parallel_trainer_takes_the_new_model(pkg, runner):
+    """The data-parallel trainer (one rank) on the model with rotation and index targets: the gradient program's
+    losses are the single trainer's, as for the plain model."""
+    rt = importlib.import_module("tensor-compiler-webgpu_b200.runtime")
+    dp = importlib.import_module("tensor-compiler-webgpu_b200.dp")
+    s, V, B = pkg.steps, 300, 3
+    cfg = s.make_config(T=40, d=64, H=4, L=1, ff=128, targets="index", rope=10000.0)
+    params = {n: np.asarray(v, np.float32) for n, v in s.init_params_normal(V, 0, 0.05, cfg).items()}
+    names = s.param_names(V, cfg)
+    state = s.initial_state(names, s.param_shapes(V, cfg))
+    one = rt.FusedTrainer(runner, rt.fused_step(s.build_step3b(V, B, cfg), matmul="tiled"), params, state)
+    many = dp.DPTrainer(runner, V, B, cfg, params)
+    try:
+        for t in range(3):
+            x, y = batch(pkg, V, B, cfg["T"], t, "index")
+            a, b = one.train(x.reshape(-1), y), many.train(x.reshape(-1), y)
+            # the folded program orders some sums otherwise: a few 2^-24 of the loss
+            assert abs(a - b) <= 1e-5 * abs(a), t
+    finally:
+        one.destroy()
+        many.destroy()
