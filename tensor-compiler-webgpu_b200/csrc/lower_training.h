@@ -437,8 +437,8 @@ static Launch head_launch(const Graph& g, const std::vector<int>& ids) {
   i64 heads = 1;
   while (heads * 8 <= H && heads * 2 <= rows) heads *= 2;
   while (heads < H && heads * 2 <= rows && cdiv(T, rows / heads) * B < SM_COUNT * 4) heads *= 2;
-  const i64 tiles = cdiv(T, rows / heads), parts = std::min<i64>(B, std::max<i64>(1, cdiv(SM_COUNT * 8, tiles)));
-  const i64 grid = std::min<i64>(tiles * parts, SM_COUNT * 8);
+  const i64 steps = cdiv(T, rows / heads) * B * cdiv(H, heads);
+  const i64 grid = std::min<i64>(steps, SM_COUNT * (back ? 2 : 4));
   i64 flags = (in_shape(g, node, 2).size() == 1 ? 1 : 0) | (bool_attr(node, "headsFirst") ? 2 : 0);
   flags |= (wx ? 4 : 0) | (wg ? 8 : 0);
   const float eps = (float)number_attr(node, "eps");
@@ -451,7 +451,7 @@ static Launch head_launch(const Graph& g, const std::vector<int>& ids) {
   if (wg) smem = 4 * D * std::max(head_rows(D, rot, 1), wide ? head_rows(D, rot, 4) : 0);
   std::vector<Call> calls;
   calls.push_back(make_call(back ? "tcb_head_norm_rope_grad" : "tcb_head_norm_rope", {grid, 1, 1}, {256, 1, 1}, smem,
-                            {B, T, H, flags, heads, parts, (i64)eps_bits, step_bits}));
+                            {B, T, H, flags, heads, (i64)eps_bits, step_bits}));
   if (back && wx && want["x"] != node.id) calls[0].out_node = want["x"];
   if (wg) {
     scratch = grid * D * 4;
@@ -463,7 +463,7 @@ static Launch head_launch(const Graph& g, const std::vector<int>& ids) {
                      "\n#define TCB_ROT " + std::to_string(rot) + "\n#define TCB_INTERLEAVED " + (pairs ? "1" : "0") +
                      "\n#include \"tcb/head_norm_rope.cuh\"\n";
   Launch l = training_record(node, back ? "head-norm-rope-grad" : "head-norm-rope", code, std::move(calls), scratch);
-  l.info = {{"bthd", arr({num(B), num(T), num(H), num(D)})}, {"heads", num(heads)}, {"parts", num(parts)}};
+  l.info = {{"bthd", arr({num(B), num(T), num(H), num(D)})}, {"heads", num(heads)}};
   return l;
 }
 

@@ -332,9 +332,8 @@ def _head_launch(graph, ids):
         heads *= 2
     while heads < H and heads * 2 <= rows and math.ceil(T / (rows // heads)) * B < SM_COUNT * 4:
         heads *= 2
-    tiles = math.ceil(T / (rows // heads))
-    parts = min(B, max(1, math.ceil(SM_COUNT * 8 / tiles)))
-    grid = min(tiles * parts, SM_COUNT * 8)
+    steps = math.ceil(T / (rows // heads)) * B * math.ceil(H / heads)
+    grid = min(steps, SM_COUNT * (2 if back else 4))   # one wave of as many CTAs as the kernel's registers allow
     flags = (1 if len(graph.nodes[node.inputs[2]].shape) == 1 else 0) | (2 if a["headsFirst"] else 0)
     flags |= (4 if "x" in want else 0) | (8 if "gain" in want else 0)
     eps = struct.unpack("<I", struct.pack("<f", a["eps"]))[0]
@@ -343,7 +342,7 @@ def _head_launch(graph, ids):
     if "gain" in want:
         smem = 4 * D * max(_head_rows(D, rot, v)[1] for v in ((4, 1) if wide else (1,)))
     main = KernelCall("tcb_head_norm_rope_grad" if back else "tcb_head_norm_rope", (grid, 1, 1), (256, 1, 1), smem,
-                      [B, T, H, flags, heads, parts, eps, step])
+                      [B, T, H, flags, heads, eps, step])
     calls, scratch = [main], 0
     if back and "x" in want and want["x"] != node.id:
         main.out_node = want["x"]
@@ -354,7 +353,7 @@ def _head_launch(graph, ids):
             fin.out_node = want["gain"]
         calls.append(fin)
     return Launch(node.id, node.op, "head-norm-rope-grad" if back else "head-norm-rope", None, node.inputs,
-                  head_source(D, rot, a["interleaved"]), calls, scratch_bytes=scratch, info={"bthd": (B, T, H, D), "heads": heads, "parts": parts})
+                  head_source(D, rot, a["interleaved"]), calls, scratch_bytes=scratch, info={"bthd": (B, T, H, D), "heads": heads})
 
 
 # ------------------------------------------------------------------ orthogonalize

@@ -323,8 +323,8 @@ def test_head_launch_geometry(mods, B, T, H, D, rot):
     G, _ = _grads(pkg, g, y, [x, gain])
     for lau in cg.lower_fused(G)["launches"]:
         main = lau.calls[0]
-        heads, parts = main.params[4:6]
-        assert 1 <= parts <= B and main.grid[0] >= 1
+        heads = main.params[4]
+        assert 1 <= main.grid[0] <= 148 * 4 and main.grid[0] <= B * T * H
         for v in ((4, 1) if rot % 8 == 0 and D % 4 == 0 else (1,)):
             lanes, rows = to._head_rows(D, rot, v)
             assert lanes <= 32 and 256 % lanes == 0 and main.smem <= 48 * 1024
