@@ -13,11 +13,12 @@ static bool is_training(const std::string& op) {
 
 constexpr i64 F16_FLAG = (i64)1 << 33, PAIR_FLAG = (i64)1 << 34;
 constexpr i64 F16_BM = 128, F16_BK = 32;
+constexpr i64 F16_EXTRA = 256 + 8 * 128 + 8 * 4096 + 1024;
 constexpr i64 AMAX_BLOCKS = 4 * SM_COUNT, DZ_BYTES = (i64)128 << 20;
 constexpr i64 CTRL_BYTES = 4 * (4 + 8 * 2 * SM_COUNT);
 constexpr i64 JOIN_COUNTERS = 512, JOIN_PARTS = 4, NLL_CTRL_BYTES = CTRL_BYTES + 4 * JOIN_COUNTERS;
 constexpr i64 NLL_CHUNK = 256, NS_CHUNK = 128, NS_PARTS = 512;
-constexpr i64 NLL_ADD = 1, NLL_JOIN = 2, NLL_NO_LOSS = 4;
+constexpr i64 NLL_ADD = 1, NLL_JOIN = 2, NLL_NO_LOSS = 4, NLL_DB = 8;
 constexpr double F16_ROOM = 60000.0;
 
 static i64 up_to(i64 n, i64 k) { return cdiv(n, k) * k; }
@@ -210,8 +211,8 @@ static std::map<int, std::vector<int>> siblings(const Graph& g) {
 // ---------------------------------------------------------------- split-fp16 products
 static i64 f16_smem(i64 bn) {
   i64 stage = 2 * F16_BM * F16_BK * 2 + 2 * bn * F16_BK * 2;
-  i64 stages = std::min<i64>(8, (227 * 1024 - 2048 - 32768) / stage);
-  return stages * stage + 1024 + 32768 + 1024;
+  i64 stages = std::min<i64>(8, (227 * 1024 - F16_EXTRA) / stage);
+  return stages * stage + F16_EXTRA;
 }
 static i64 f16_tiles(i64 M, i64 N, i64 bn, bool symmetric) {
   i64 tm = cdiv(M, F16_BM), tn = cdiv(N, bn), t = 0;
@@ -361,7 +362,8 @@ static Launch nll_grad_launch(const Graph& g, const std::vector<int>& ids) {
   const bool wh = want.count("h"), ww = want.count("w"), wb = want.count("b");
   Regions r;
   r.add(256);
-  const i64 err = r.add(NLL_CTRL_BYTES), dz = r.add(4 * R * up_to(piece, piece > 256 ? 256 : 32)), db = r.add(4 * cdiv(R, 32) * V);
+  const i64 err = r.add(NLL_CTRL_BYTES), dz = r.add(4 * R * up_to(piece, piece > 256 ? 256 : 32)),
+            db = r.add(wb ? 4 * cdiv(R, 32) * V : 0);
   const std::vector<i64> tail = {R, d, V, 0, in.lse, in.h, in.w, db};
   const bool joined = wb && nll_joined(cdiv(V, 32), cdiv(R, 32));
   std::vector<Call> calls;
@@ -373,7 +375,7 @@ static Launch nll_grad_launch(const Graph& g, const std::vector<int>& ids) {
   };
   for (i64 k = 0; k < pieces; ++k) {
     const i64 v0 = k * piece, n = std::min(piece, V - v0);
-    const std::vector<i64> params = cat(tail, {v0, (k ? NLL_ADD : 0) | (joined ? NLL_JOIN : 0)});
+    const std::vector<i64> params = cat(tail, {v0, (k ? NLL_ADD : 0) | (joined ? NLL_JOIN : 0) | (wb ? NLL_DB : 0)});
     const i64 w_at = in.w + (v0 ? 4 * d * v0 : 0);
     auto h = [&](bool mn) { return blocked_operand("in_at", in.h << 3 | 1, R, d, nll_pitch(d), mn, F16_BM); };
     auto w = [&](bool mn, i64 bn) { return blocked_operand("in_at", w_at << 3 | 1, d, n, nll_pitch(V), mn, bn); };

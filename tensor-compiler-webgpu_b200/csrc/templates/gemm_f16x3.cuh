@@ -56,12 +56,42 @@ __device__ __forceinline__ u32 f16x2(float a, float b) {
 __device__ __forceinline__ void f16x2_float(u32 v, float& a, float& b) {
   asm("{\n .reg .b16 l, h;\n mov.b32 {l, h}, %2;\n cvt.f32.f16 %0, l;\n cvt.f32.f16 %1, h;\n}" : "=f"(a), "=f"(b) : "r"(v));
 }
+// Two float32 operations in one instruction, each rounded to nearest: the epilogues' warps, two an SM
+// quarter, are bound by what they issue (dz at 4095 x 256 x 8192: 73 us with single ones and every target's
+// column tested, DZ_US so).
+__device__ __forceinline__ u64 pair2(float a, float b) {
+  u64 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair2(u64 r, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r)); }
+__device__ __forceinline__ void add2(float& a, float& b, float x, float y) {
+  u64 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair2(a, b)), "l"(pair2(x, y)));
+  unpair2(r, a, b);
+}
+__device__ __forceinline__ void mul2(float& a, float& b, float x, float y) {
+  u64 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair2(a, b)), "l"(pair2(x, y)));
+  unpair2(r, a, b);
+}
+// a = a x + c, b = b y + d
+__device__ __forceinline__ void fma2(float& a, float& b, float x, float y, float c, float d) {
+  u64 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(pair2(a, b)), "l"(pair2(x, y)), "l"(pair2(c, d)));
+  unpair2(r, a, b);
+}
+template <int N> __device__ __forceinline__ void add32(float (&v)[N], const float (&w)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; i += 2) add2(v[i], v[i + 1], w[i], w[i + 1]);
+}
 // hi and lo of two scaled values
 __device__ __forceinline__ void split2(float a, float b, u32& hi, u32& lo) {
   hi = f16x2(a, b);
   float x, y;
   f16x2_float(hi, x, y);
-  lo = f16x2(__fsub_rn(a, x), __fsub_rn(b, y));
+  fma2(x, y, -1.0f, -1.0f, a, b);
+  lo = f16x2(x, y);
 }
 // 2^k for k in [-126, 127]
 __device__ __forceinline__ float pow2(int k) { return __uint_as_float((u32)(k + 127) << 23); }
@@ -79,8 +109,8 @@ constexpr u32 HG_THREADS = 384;
 template <int BN> struct F16x3 {
   static constexpr u32 A_BYTES = HG_M * HG_K * 2, B_BYTES = BN * HG_K * 2;
   static constexpr u32 STAGE = 2 * A_BYTES + 2 * B_BYTES;
-  static constexpr u32 STAGING = 8 * 4096;                           // a 4 KB block per epilogue warp
-  static constexpr u32 FIT = (227 * 1024 - 2048 - STAGING) / STAGE;  // 1 KB of barriers, 1 KB to align
+  static constexpr u32 BARS = 256, VECTORS = 8 * 128, STAGING = 8 * 4096;   // 128 bytes, a 4 KB block an epilogue warp
+  static constexpr u32 FIT = (227 * 1024 - 1024 - BARS - VECTORS - STAGING) / STAGE;   // 1 KB to align the ring
   static constexpr u32 STAGES = FIT > 8 ? 8 : FIT;
   static constexpr u32 ACCS = BN == 256 ? 1 : BN == 128 ? 2 : 3;     // accumulators of a TMEM buffer
   static constexpr u32 TMEM = 512;                                   // columns allocated: 2 ACCS BN, a power of 2
@@ -204,6 +234,7 @@ struct F16Epi {
   u32 M, N;
   u32 stage;           // shared-memory address of the warp's 4 KB block
   unsigned char* gstage;
+  float* vec;          // 32 floats of the warp's own
 };
 
 // Written out block by block, so that every index into the sums is a constant and they stay in registers.
@@ -217,18 +248,15 @@ __device__ __forceinline__ void f16_collect(float (&v)[NB][32], u32 t) {
       if constexpr (ACCS > 2) {
         float x[32];
         tmem_ld32(t + 2 * BN + 32 * I, x);
-#pragma unroll
-        for (int i = 0; i < 32; ++i) w[i] = __fadd_rn(w[i], x[i]);
+        add32(w, x);
       }
       float x[32];
       tmem_ld32(t + 32 * I, x);
-#pragma unroll
-      for (int i = 0; i < 32; ++i) w[i] = __fadd_rn(w[i], x[i]);
+      add32(w, x);
     } else {
       tmem_ld32(t + 32 * I, w);
     }
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[I][i] = __fadd_rn(v[I][i], w[i]);
+    add32(v[I], w);
     f16_collect<BN, I + 1>(v, t);
   }
 }
@@ -286,8 +314,8 @@ __device__ __forceinline__ void gemm_f16x3(const F16Job& J, u32* err, EPI& epi) 
   extern __shared__ unsigned char smem_raw[];
   const u32 raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
   unsigned char* gbase = smem_raw + (base - raw);
-  const u32 bars = base + STAGES * S::STAGE, staging = bars + 1024;
-  u32* tmem_slot = reinterpret_cast<u32*>(gbase + STAGES * S::STAGE + (2 * STAGES + 4) * 8);
+  const u32 staging = base + STAGES * S::STAGE, bars = staging + S::STAGING, vectors = bars + S::BARS;
+  u32* tmem_slot = reinterpret_cast<u32*>(gbase + (bars - base) + (2 * STAGES + 4) * 8);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   auto full = [&](u32 s) { return bars + 8u * s; };
   auto empty = [&](u32 s) { return bars + 8u * (STAGES + s); };
@@ -418,12 +446,14 @@ __device__ __forceinline__ void gemm_f16x3(const F16Job& J, u32* err, EPI& epi) 
     e.N = N;
     e.stage = staging + (u32)w * 4096;
     e.gstage = gbase + (e.stage - base);
+    e.vec = reinterpret_cast<float*>(gbase + (vectors - base)) + w * 32;
     epi.start(e.gstage - w * 4096);
     u32 j = 0;
     bool ok = true;
     while (ok && work.next()) {
       e.T = f16_tile<BN, SYM>(work.tile, tm, tn, per);
       e.row = (u64)e.T.m0 + 32 * e.q + lane;
+      epi.begin(e);   // its loads are on their way while the products run
       float v[NB][32];
 #pragma unroll
       for (int b = 0; b < NB; ++b)
@@ -463,7 +493,6 @@ __device__ __forceinline__ void gemm_f16x3(const F16Job& J, u32* err, EPI& epi) 
         }
       }
       if (mine) {
-        epi.begin(e);
         f16_blocks<0>(epi, e, v, N);
         epi.end(e);
       }
@@ -489,7 +518,7 @@ constexpr u32 F16_CTRL = 4 + 8 * 2 * 148;   // words: the error word, 8 counters
 
 // 32 columns of hi / lo pairs through the warp's staging block to two planes of an fp16 array by TMA
 // store (map: {cols, rows, planes}, boxes of 32 x 32 x 2, 64-byte swizzle).
-__device__ __forceinline__ void store_split32(const F16Epi& e, const TmaDesc* map, const float (&v)[32], int col, int row, int matrix) {
+__device__ __forceinline__ void stage_split32(const F16Epi& e, const float (&v)[32]) {
   if (e.lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");   // the last store has read it
   __syncwarp();
   uint4* sp = reinterpret_cast<uint4*>(e.gstage);
@@ -504,12 +533,19 @@ __device__ __forceinline__ void store_split32(const F16Epi& e, const TmaDesc* ma
     sp[e.lane * 4 + (c ^ sw)] = h;
     sp[128 + e.lane * 4 + (c ^ sw)] = l;
   }
+}
+__device__ __forceinline__ void send_split32(const F16Epi& e, const TmaDesc* map, int col, int row, int matrix) {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   __syncwarp();
   if (e.lane == 0) {
     tma_store_3d(map, e.stage, col, row, 2 * matrix);
     bulk_commit();
   }
+}
+
+__device__ __forceinline__ void store_split32(const F16Epi& e, const TmaDesc* map, const float (&v)[32], int col, int row, int matrix) {
+  stage_split32(e, v);
+  send_split32(e, map, col, row, matrix);
 }
 
 // 32 x 32 floats, a row per lane, turned in the warp's staging block so that lane l holds column l
@@ -535,9 +571,13 @@ __device__ __forceinline__ float column_sums32(float (&v)[32], int lane) {
     const bool up = (lane & o) != 0;
 #pragma unroll
     for (int j = 0; j < o; ++j) {
-      const float send = up ? v[j] : v[j + o], keep = up ? v[j + o] : v[j];
-      v[j] = __fadd_rn(keep, __shfl_xor_sync(0xffffffffu, send, o));
+      const float send = up ? v[j] : v[j + o];
+      v[j] = up ? v[j + o] : v[j];
+      v[j + o] = __shfl_xor_sync(0xffffffffu, send, o);
     }
+#pragma unroll
+    for (int j = 0; j + 1 < o; j += 2) add2(v[j], v[j + 1], v[j + o], v[j + o + 1]);
+    if (o == 1) v[0] = __fadd_rn(v[0], v[1]);
   }
   return v[0];
 }

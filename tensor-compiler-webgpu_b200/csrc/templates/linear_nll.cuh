@@ -38,7 +38,7 @@
 
 namespace tcb {
 
-constexpr u32 NLL_ADD = 1, NLL_JOIN = 2, NLL_NO_LOSS = 4;   // flags: add to dh; join in the product's kernel; no loss
+constexpr u32 NLL_ADD = 1, NLL_JOIN = 2, NLL_NO_LOSS = 4, NLL_DB = 8;   // flags: add to dh; join in the product's kernel; no loss; db wanted
 constexpr u32 NLL_CTRL = F16_CTRL + 512;   // words of the control block: a counter more for each 32 rows or columns joined
 constexpr float NLL_LOG2E = 1.44269504f, NLL_LN2 = 0.693147181f, NLL_MAX = 3.402823466e38f;
 #define TCB_MINUS_INF bits(0xff800000u)
@@ -215,16 +215,23 @@ extern "C" __global__ void __launch_bounds__(256) tcb_nll_split(const tcb::Args 
 
 namespace tcb {
 
-// The 32 scaled logits of a block from their sums: 8 loads of the padded bias, the same for every lane.
-__device__ __forceinline__ void nll_logits(float (&v)[32], float z2, const float* bias2) {
+// The 32 scaled logits of a block from their sums and the bias, a column a lane (loaded a block ahead), which
+// the warp's shared memory hands to every lane.
+__device__ __forceinline__ void nll_logits(const F16Epi& e, float (&v)[32], float z2, float bias) {
+  __syncwarp();
+  e.vec[e.lane] = bias;
+  __syncwarp();
 #pragma unroll
   for (int c = 0; c < 8; ++c) {
-    const float4 b = *reinterpret_cast<const float4*>(bias2 + 4 * c);
-    v[4 * c] = fmaf(v[4 * c], z2, b.x);
-    v[4 * c + 1] = fmaf(v[4 * c + 1], z2, b.y);
-    v[4 * c + 2] = fmaf(v[4 * c + 2], z2, b.z);
-    v[4 * c + 3] = fmaf(v[4 * c + 3], z2, b.w);
+    const float4 b = *reinterpret_cast<const float4*>(e.vec + 4 * c);
+    fma2(v[4 * c], v[4 * c + 1], z2, z2, b.x, b.y);
+    fma2(v[4 * c + 2], v[4 * c + 3], z2, z2, b.z, b.w);
   }
+}
+// This lane's column of the block at c0 of a tile, the last one again beyond N.
+__device__ __forceinline__ u32 nll_column(const F16Epi& e, int c0) {
+  const u32 col = (u32)(e.T.n0 + c0 + e.lane), last = (e.N + 31) / 32 * 32 - 1;
+  return col < last ? col : last;
 }
 // The target's place among 32 columns as a bit: comparing an index with each would be turned into an
 // indexed read and keep the sums in local memory.
@@ -279,7 +286,7 @@ template <int BN>
 struct NllForward {
   const Args& a;
   const float* bias2;
-  float z2, m, s;
+  float z2, m, s, bias;
   int t;
   __device__ __forceinline__ explicit NllForward(const Args& args) : a(args) {}
   __device__ __forceinline__ void start(unsigned char*) {
@@ -292,10 +299,12 @@ struct NllForward {
     m = TCB_MINUS_INF;
     s = 0.0f;
     t = e.row < n.R() ? n.target(e.row) : -1;
+    bias = bias2[nll_column(e, e.c0)];
   }
   __device__ __forceinline__ void block(const F16Epi& e, int c0, float (&v)[32]) {
     const u32 col = (u32)(e.T.n0 + c0);
-    nll_logits(v, z2, bias2 + col);
+    nll_logits(e, v, z2, bias);
+    bias = bias2[nll_column(e, c0 + 32)];
     float mx = m;
 #pragma unroll
     for (int j = 0; j < 32; ++j) mx = fmaxf(mx, v[j]);
@@ -309,7 +318,10 @@ struct NllForward {
     const float safe = mx == TCB_MINUS_INF ? 0.0f : mx;
     float q[4] = {s * ex2(m - safe), 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int j = 0; j < 32; ++j) q[j & 3] += ex2(v[j] - safe);
+    for (int j = 0; j < 32; j += 2) {
+      add2(v[j], v[j + 1], -safe, -safe);
+      add2(q[j & 3], q[(j & 3) + 1], ex2(v[j]), ex2(v[j + 1]));
+    }
     s = (q[0] + q[1]) + (q[2] + q[3]);
     m = mx;
   }
@@ -331,7 +343,8 @@ struct NllDz {
   const Args& a;
   const TmaDesc* map;
   const float* bias2;
-  float z2, up, down, lse, g;
+  float* part_row;   // where this lane's column sums go
+  float z2, up, down, lse, g, bias;
   int t;
   __device__ __forceinline__ explicit NllDz(const GemmParams& P) : a(P.a), map(&P.maps[2]) {}
   // The cotangent's scale: each CTA's epilogue warps look through all of it behind the first product.
@@ -345,9 +358,9 @@ struct NllDz {
       int c[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const u64 r = i + 256 * k;
-        x[k] = r < n.R() ? n.cotangent(r) : 0.0f;
-        c[k] = r < n.R() ? n.target(r) : -1;
+        const u64 r = i + 256 * k < n.R() ? i + 256 * k : i;   // (a branch would have the loads wait one for another)
+        x[k] = n.cotangent(r);
+        c[k] = n.target(r);
       }
 #pragma unroll
       for (int k = 0; k < 8; ++k) m = fmaxf(m, c[k] >= 0 ? finite_abs(x[k]) : 0.0f);
@@ -366,30 +379,44 @@ struct NllDz {
   }
   __device__ __forceinline__ void begin(const F16Epi& e) {
     const Nll<true> n(a);
-    t = e.row < n.R() ? n.target(e.row) : -1;
-    lse = t >= 0 ? n.lse2()[e.row] : 0.0f;
-    g = t >= 0 ? n.cotangent(e.row) * up : 0.0f;
+    const u64 row = e.row < n.R() ? e.row : n.R() - 1;
+    t = n.target(row);
+    lse = n.lse2()[row];
+    g = n.cotangent(row) * up;
+    if (e.row != row) t = -1;
+    part_row = n.template scratch<float>((u64)a.p[11]) + ((u64)e.T.m0 / 32 + e.q) * n.V() + (u64)a.p[12] + e.lane;
+    bias = bias2[nll_column(e, e.c0)];
   }
   __device__ __forceinline__ void block(const F16Epi& e, int c0, float (&v)[32]) {
     const Nll<true> n(a);
     const u32 pc = (u32)(e.T.n0 + c0), col = (u32)a.p[12] + pc;
-    nll_logits(v, z2, bias2 + pc);
+    nll_logits(e, v, z2, bias);
+    bias = bias2[nll_column(e, c0 + 32)];
     const u32 mine = nll_bit(t, col);
 #pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      const float p = ex2(v[j] - lse);
-      v[j] = g * ((mine >> j) & 1 ? p - 1.0f : p);
+    for (int j = 0; j < 32; j += 2) {
+      add2(v[j], v[j + 1], -lse, -lse);
+      v[j] = ex2(v[j]);
+      v[j + 1] = ex2(v[j + 1]);
     }
+    if (__any_sync(0xffffffffu, mine != 0u)) {   // in one block of 8 at 8192 classes
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] = (mine >> j) & 1 ? v[j] - 1.0f : v[j];
+    }
+#pragma unroll
+    for (int j = 0; j < 32; j += 2) mul2(v[j], v[j + 1], g, g);
     if (t < 0) {   // not by g = 0: an excluded row's logits may be anything
 #pragma unroll
       for (int j = 0; j < 32; ++j) v[j] = 0.0f;
     }
-    store_split32(e, map, v, (int)(pc & 255), e.T.m0 + 32 * e.q, (int)(pc >> 8));
-    const float sum = column_sums32(v, e.lane);
-    float* part = n.template scratch<float>((u64)a.p[11]) + col + e.lane;
-    const bool in = col + e.lane < (u32)n.V();
-    if (in) part[((u64)e.T.m0 / 32 + e.q) * n.V()] = sum * down;
+    stage_split32(e, v);
+    const bool db = ((u32)a.p[13] & NLL_DB) != 0;
+    const float sum = db ? column_sums32(v, e.lane) : 0.0f;   // while the values are on their way to shared memory
+    send_split32(e, map, (int)(pc & 255), e.T.m0 + 32 * e.q, (int)(pc >> 8));
+    const bool in = pc + e.lane < e.N;
+    if (db && in) part_row[pc] = sum * down;
     if (!((u32)a.p[13] & NLL_JOIN)) return;
+    const float* part = n.template scratch<float>((u64)a.p[11]) + col + e.lane;
     const u32 rows = ((u32)n.R() + 31) / 32;
     if (!nll_last(a, col / 32, rows, e.lane) || !in) return;
     float x = 0.0f;
@@ -409,11 +436,14 @@ struct NllOut {
   const Args& a;
   float* out;
   float x, y;
+  __device__ static int exponent(float power) { return (int)(__float_as_uint(power) >> 23) - 127; }
   __device__ __forceinline__ NllOut(const Args& args, u64 o) : a(args), out(reinterpret_cast<float*>(o)) {}
   __device__ __forceinline__ void start(unsigned char*) {
     const Nll<true> n(a);
-    x = DW ? n.scales()->down_h : n.scales()->down_w;
-    y = n.g_scale()->y;
+    // the two powers of two as two of about one size: operands far from 1 would leave the range half way
+    const int k = exponent(DW ? n.scales()->down_h : n.scales()->down_w) + exponent(n.g_scale()->y);
+    x = pow2(k >> 1);
+    y = pow2(k - (k >> 1));
   }
   __device__ __forceinline__ void begin(const F16Epi&) {}
   __device__ __forceinline__ void block(const F16Epi& e, int c0, float (&v)[32]) {

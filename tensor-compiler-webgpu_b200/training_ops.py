@@ -21,6 +21,7 @@ SM_COUNT = 148
 F16 = 1 << 33          # box_cols flags of a tensor map: 16-bit elements,
 PAIR = 1 << 34         # two planes (hi and lo) a box
 F16_BM, F16_BK = 128, 32
+F16_EXTRA = 256 + 8 * 128 + 8 * 4096 + 1024   # beside the ring: barriers, vectors, staging, and to align it
 AMAX_BLOCKS = 4 * SM_COUNT
 DZ_BYTES = 128 << 20             # bound of one vocabulary piece's dz
 CTRL_BYTES = 4 * (4 + 8 * 2 * SM_COUNT)   # error word, and a counter per epilogue warp of a divided tile
@@ -32,13 +33,13 @@ def _up(n, k):
 
 def _f16_stages(bn):
     stage = 2 * F16_BM * F16_BK * 2 + 2 * bn * F16_BK * 2
-    return min(8, (227 * 1024 - 2048 - 32768) // stage), stage
+    return min(8, (227 * 1024 - F16_EXTRA) // stage), stage
 
 
 def f16_smem(bn):
-    """Ring, barriers, staging and 1 KB to align the ring (tcb/gemm_f16x3.cuh)."""
+    """Bytes of shared memory (tcb/gemm_f16x3.cuh)."""
     stages, stage = _f16_stages(bn)
-    return stages * stage + 1024 + 32768 + 1024
+    return stages * stage + F16_EXTRA
 
 
 def f16_tiles(M, N, bn, symmetric):
@@ -147,7 +148,7 @@ NLL_CHUNK = 256
 # product's own kernel, and the most parts a warp then adds up on its own
 JOIN_COUNTERS, JOIN_PARTS = 512, 4
 NLL_CTRL_BYTES = CTRL_BYTES + 4 * JOIN_COUNTERS
-NLL_ADD, NLL_JOIN, NLL_NO_LOSS = 1, 2, 4
+NLL_ADD, NLL_JOIN, NLL_NO_LOSS, NLL_DB = 1, 2, 4, 8
 
 
 def _joined(groups, parts):
@@ -230,7 +231,8 @@ def _nll_grad_launch(graph, ids):
     inner, _ = linear_nll_saved(R, d, V)
     piece, pieces = nll_pieces(R, V)
     want = {graph.nodes[i].attrs["wrt"]: i for i in ids}
-    at, end = _regions(("scale", 256), ("err", NLL_CTRL_BYTES), ("dz", 4 * R * _up(piece, 256 if piece > 256 else 32)), ("db", 4 * math.ceil(R / 32) * V))
+    at, end = _regions(("scale", 256), ("err", NLL_CTRL_BYTES), ("dz", 4 * R * _up(piece, 256 if piece > 256 else 32)),
+                       ("db", 4 * math.ceil(R / 32) * V if "b" in want else 0))
     tail = [R, d, V, 0, inner["lse"], inner["h"], inner["w"], at["db"]]
     joined = "b" in want and _joined(math.ceil(V / 32), math.ceil(R / 32))
     calls, partial = [], 0
@@ -247,7 +249,7 @@ def _nll_grad_launch(graph, ids):
     for k in range(pieces):
         v0 = k * piece
         n = min(piece, V - v0)
-        params = [*tail, v0, (NLL_ADD if k else 0) | (NLL_JOIN if joined else 0)]
+        params = [*tail, v0, (NLL_ADD if k else 0) | (NLL_JOIN if joined else 0) | (NLL_DB if "b" in want else 0)]
         w_at = inner["w"] + (4 * d * v0 if v0 else 0)   # pieces begin with a block
 
         def h(mn):

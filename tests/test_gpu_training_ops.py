@@ -157,6 +157,15 @@ def test_nll_magnitudes(pkg, mods, runner, sh, sw, sg):
     check_nll(mods, runner, case)
 
 
+@pytest.mark.parametrize("sh,sw,sg,wrt", [(1e36, 1e-36, 1e-30, "hwb"), (1e-36, 1e36, 1e30, "wb"), (1e36, 1e-36, 1.0, "w")])
+def test_nll_magnitudes_that_cancel(pkg, mods, runner, sh, sw, sg, wrt):
+    """The scale of h, or of its gradient's operand, alone takes the sums out of the range; both together do not."""
+    case = nll_case(pkg, 70, 33, 90, seed=9, wrt=wrt)
+    x = case[3]
+    x["h"], x["w"], x["d0"] = f32(x["h"] * sh), f32(x["w"] * sw), f32(x["d0"] * sg)
+    check_nll(mods, runner, case)
+
+
 def test_nll_pieces(pkg, mods, runner, monkeypatch):
     """The vocabulary in several pieces: dh is added up over them, dW and db land at their columns."""
     to = importlib.import_module(P + ".training_ops")
