@@ -28,11 +28,14 @@
 // ever transposed in memory.  A symmetric product (SYM) computes the tiles on or above the diagonal only
 // and its epilogue mirrors them.
 //
-// Work: the first `full` tiles go whole to the CTAs in turn, in grouped raster order.  The others, where a
-// last wave would leave SMs idle or there are fewer tiles than SMs, are one line of units of `quantum`
-// chunks, cut into equal runs, one a CTA.  A run that holds a part of a tile only leaves its sums in
-// scratch; the warp that arrives last at its part of the tile adds them all, in order, and goes on to the
-// epilogue: no CTA waits for another, and the result does not depend on which came last.
+// What bounds it: 48 KB a stage of 32 K indices against 768 clocks of products at BN = 256, as many bytes a
+// clock as an SM takes from L2 at best (64, measured with boxes of 16 KB); narrower tiles ask for more.
+//
+// Work: where there are as many tiles as SMs or more, they go whole to the CTAs in turn, in grouped raster
+// order (full = tiles).  Fewer ones may be divided (full = 0): they are one line of units of `quantum` chunks,
+// cut into equal runs, one a CTA.  A run that holds a part of a tile only leaves its sums in scratch; the warp
+// that arrives last at its part of the tile adds them all, in order, and goes on to the epilogue: no CTA waits
+// for another, and the result does not depend on which came last.
 //
 // p[0] = M | N << 32, p[1] = K | batch << 32, p[2] = full | quantum << 32, p[3] = byte offset in scratch of
 // the partial sums (two 128 x BN slots a CTA), p[15] = control block: the error word, 16 bytes on a
@@ -57,8 +60,8 @@ __device__ __forceinline__ void f16x2_float(u32 v, float& a, float& b) {
   asm("{\n .reg .b16 l, h;\n mov.b32 {l, h}, %2;\n cvt.f32.f16 %0, l;\n cvt.f32.f16 %1, h;\n}" : "=f"(a), "=f"(b) : "r"(v));
 }
 // Two float32 operations in one instruction, each rounded to nearest: the epilogues' warps, two an SM
-// quarter, are bound by what they issue (dz at 4095 x 256 x 8192: 73 us with single ones and every target's
-// column tested, DZ_US so).
+// quarter, wait on what they issue (dz at 4095 x 256 x 8192: 73.2 us with single operations and every column
+// compared with the target, 70.0 so).
 __device__ __forceinline__ u64 pair2(float a, float b) {
   u64 r;
   asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
@@ -293,8 +296,9 @@ __device__ __forceinline__ void f16_blocks(EPI& epi, const F16Epi& e, float (&v)
   }
 }
 
-// EPI: struct with start(staging) once, by all 256 epilogue threads, begin(e), block(e, c0, v) for each 32 columns (from column c0 of the tile) that reach into
-// the output, end(e), and done(e) once after the last tile.
+// EPI: struct with start(staging) once, by all 256 epilogue threads, begin(e) before a tile's or part's products
+// have come, block(e, c0, v) for each 32 columns (from column c0 of the tile) that reach into the output, end(e),
+// and done(e) once after the last tile.
 struct F16Job {
   const TmaDesc *ma, *mb;
   u32 M, N, K, batch, full, quantum, block, grid;

@@ -10,8 +10,9 @@
 //
 // Forward: one matrix product (tcb/gemm_f16x3.cuh) whose epilogue keeps, per row and half tile of columns,
 // the running maximum and the sum of exponentials; the last to arrive at 32 rows joins their tiles (a launch of
-// its own, tcb_nll_finish, when they are many).  The logits exist in tensor memory and registers only, in units of log 2: z2 = log2(e) z is one fma from the sums, its
-// exponential one ex2 (2^-22 relative, as far off as the operands' split).
+// its own, tcb_nll_finish, when they are many).  The logits exist in tensor memory and registers only, in units
+// of log 2: z2 = log2(e) z is one fma from the sums, its exponential one ex2 (2^-22 relative, as far off as the
+// operands' split).
 // What the backward needs of it is saved in one opaque value (NllSaved): the scales, b log2(e), each
 // row's log2 of the sum, and h and W as split for the tensor core, 4 bytes a value.
 // Backward: the vocabulary is walked in pieces (a bounded workspace).  A piece's logits are computed
@@ -25,9 +26,9 @@
 //
 // p[] of every kernel: [0..3] the product's (split: [0] blocks of the amax launch; finish: [0] half tiles of a
 // row), [4] R, [5] d, [6] V, [7] byte offset of the saved value in scratch (when nobody asks for a backward;
-// else the address of the loss), [8..10] byte offsets in it of the row sums, h and W, [11] byte offset in scratch of the targets'
-// logits (backward: of the column-sum partials), [12] of the row partials (backward: the piece's first
-// column), [13] flags, [14] address of the saved value or 0 (dz: of db or 0).
+// else the address of the loss), [8..10] byte offsets in it of the row sums, h and W, [11] byte offset in scratch
+// of the targets' logits (backward: of the column-sum partials), [12] of the row partials (backward: the piece's
+// first column), [13] flags, [14] address of the saved value or 0 (dz: of db or 0).
 // in[]: h, W, (b), t forward; t, saved, the loss's cotangent backward.
 #pragma once
 #include "tcb/gemm_f16x3.cuh"
@@ -38,7 +39,8 @@
 
 namespace tcb {
 
-constexpr u32 NLL_ADD = 1, NLL_JOIN = 2, NLL_NO_LOSS = 4, NLL_DB = 8;   // flags: add to dh; join in the product's kernel; no loss; db wanted
+// flags: add to dh; join in the product's kernel; no loss; db wanted
+constexpr u32 NLL_ADD = 1, NLL_JOIN = 2, NLL_NO_LOSS = 4, NLL_DB = 8;
 constexpr u32 NLL_CTRL = F16_CTRL + 512;   // words of the control block: a counter more for each 32 rows or columns joined
 constexpr float NLL_LOG2E = 1.44269504f, NLL_LN2 = 0.693147181f, NLL_MAX = 3.402823466e38f;
 #define TCB_MINUS_INF bits(0xff800000u)

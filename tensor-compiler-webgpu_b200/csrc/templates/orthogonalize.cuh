@@ -215,7 +215,7 @@ struct NsApply {
 #define TCB_NS_GEMM(NAME, BN, AMN, BMN, SYM, EPI)                                                                         \
   extern "C" __global__ void __launch_bounds__(tcb::HG_THREADS, 1) NAME##_##BN(const __grid_constant__ tcb::GemmParams P) { \
     tcb::EPI epi(P);                                                                                                      \
-    tcb::gemm_f16x3<BN, AMN, BMN, SYM, false, 128>(tcb::f16_job(P), reinterpret_cast<u32*>(P.a.p[15]), epi);                                                                      \
+    tcb::gemm_f16x3<BN, AMN, BMN, SYM, false, 128>(tcb::f16_job(P), reinterpret_cast<u32*>(P.a.p[15]), epi);              \
   }
 #define TCB_NS_S(BN) NsSymmetric<BN, false>
 #define TCB_NS_P(BN) NsSymmetric<BN, true>
