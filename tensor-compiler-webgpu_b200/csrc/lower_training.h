@@ -209,15 +209,17 @@ static std::map<int, std::vector<int>> siblings(const Graph& g) {
 }
 
 // ---------------------------------------------------------------- split-fp16 products
+static i64 f16_ctas(i64 bn) { return bn == 256 ? 2 : 1; }
 static i64 f16_smem(i64 bn) {
-  i64 stage = 2 * F16_BM * F16_BK * 2 + 2 * bn * F16_BK * 2;
+  i64 stage = 2 * F16_BM * F16_BK * 2 + 2 * (bn / f16_ctas(bn)) * F16_BK * 2;
   i64 stages = std::min<i64>(8, (227 * 1024 - F16_EXTRA) / stage);
   return stages * stage + F16_EXTRA;
 }
 static i64 f16_tiles(i64 M, i64 N, i64 bn, bool symmetric) {
-  i64 tm = cdiv(M, F16_BM), tn = cdiv(N, bn), t = 0;
+  const i64 rows = F16_BM * f16_ctas(bn);
+  i64 tm = cdiv(M, rows), tn = cdiv(N, bn), t = 0;
   if (!symmetric) return tm * tn;
-  for (i64 i = 0; i < tm; ++i) t += tn - i * F16_BM / bn;
+  for (i64 i = 0; i < tm; ++i) t += tn - i * rows / bn;
   return t;
 }
 
@@ -234,15 +236,16 @@ static F16Plan f16_plan(i64 M, i64 N, i64 K, i64 batch, i64 chunk, bool symmetri
   const i64 steps = cdiv(K, 16);
   for (auto& row : COST) {
     const i64 bn = row[0], step = row[1], epi = row[2], once = row[3], part = row[4];
-    if (bn > 64 && N <= bn / 2) continue;
+    const i64 ctas = f16_ctas(bn), units = SM_COUNT / ctas;
+    if ((bn > 64 && N <= bn / 2) || M <= F16_BM * (ctas - 1)) continue;
     const i64 tiles = batch * f16_tiles(M, N, bn, symmetric);
-    take(cdiv(tiles, SM_COUNT) * (steps * step + epi), bn, std::min<i64>(SM_COUNT, tiles), tiles, 1);
+    take(cdiv(tiles, units) * (steps * step + epi), bn, std::min<i64>(units, tiles) * ctas, tiles, 1);
     for (i64 q = 1; q <= 64; q *= 2) {
       const i64 per = cdiv(K, 256 * q);
-      if (tiles >= SM_COUNT || per == 1) break;
-      const i64 grid = std::min<i64>(SM_COUNT, tiles * per), run = cdiv(tiles * per, grid);
+      if (tiles >= units || per == 1) break;
+      const i64 grid = std::min<i64>(units, tiles * per), run = cdiv(tiles * per, grid);
       const i64 pieces = run == 1 ? per : per / run + 2;
-      take(run * q * 16 * step + once + pieces * part + epi, bn, grid, 0, q * (256 / chunk));
+      take(run * q * 16 * step + once + pieces * part + epi, bn, grid * ctas, 0, q * (256 / chunk));
     }
   }
   return best;
@@ -251,13 +254,14 @@ static i64 f16_partial_bytes(const F16Plan& p, i64 tiles) { return p.whole == ti
 
 static Map f16_operand(i64 off, i64 cols, i64 rows, i64 batch, i64 pitch, bool mn, i64 bn) {
   return {"scratch", off, cols, rows, 2 * batch, pitch * 2, rows * pitch * 2, (mn ? 64 : F16_BK) | F16_FLAG | PAIR_FLAG,
-          mn ? F16_BK : bn};
+          mn ? F16_BK : bn / f16_ctas(bn)};
 }
 static Map blocked(const std::string& region, i64 off, i64 rows, i64 cols, i64 pitch, i64 box_cols, i64 box_rows) {
   return {region, off, pitch, rows, 2 * cdiv(cols, 256), pitch * 2, rows * pitch * 2, box_cols | F16_FLAG | PAIR_FLAG, box_rows};
 }
 static Map blocked_operand(const std::string& region, i64 off, i64 rows, i64 cols, i64 pitch, bool mn, i64 bn) {
-  return mn ? blocked(region, off, rows, cols, pitch, 64, F16_BK) : blocked(region, off, rows, cols, pitch, F16_BK, bn);
+  return mn ? blocked(region, off, rows, cols, pitch, 64, F16_BK)
+            : blocked(region, off, rows, cols, pitch, F16_BK, bn / f16_ctas(bn));
 }
 
 static Call f16_gemm(const std::string& name, i64 M, i64 N, i64 K, i64 batch, const F16Plan& p, i64 part_at,

@@ -110,7 +110,8 @@ __device__ __forceinline__ int scale_exponent(float m) {
 constexpr int HG_M = 128, HG_K = 32;
 constexpr u32 HG_THREADS = 384;
 template <int BN> struct F16x3 {
-  static constexpr u32 A_BYTES = HG_M * HG_K * 2, B_BYTES = BN * HG_K * 2;
+  static constexpr int CTAS = BN == 256 ? 2 : 1, TM = CTAS * HG_M, COLS = BN / CTAS;   // tile rows; columns of B a CTA loads
+  static constexpr u32 A_BYTES = HG_M * HG_K * 2, B_BYTES = COLS * HG_K * 2;
   static constexpr u32 STAGE = 2 * A_BYTES + 2 * B_BYTES;
   static constexpr u32 BARS = 256, VECTORS = 8 * 128, STAGING = 8 * 4096;   // 128 bytes, a 4 KB block an epilogue warp
   static constexpr u32 FIT = (227 * 1024 - 1024 - BARS - VECTORS - STAGING) / STAGE;   // 1 KB to align the ring
@@ -129,20 +130,48 @@ template <bool MN> __device__ __forceinline__ u32 f16_desc_lo(u32 saddr) {
 template <bool MN> __host__ __device__ constexpr u32 f16_desc_hi() {
   return MN ? 1024u >> 4 | 1u << 14 | 2u << 29 : 512u >> 4 | 1u << 14 | 4u << 29;
 }
-// D f32, A and B f16, M = 128, N = n
-__host__ __device__ constexpr u32 idesc_f16(u32 n, u32 a_mn, u32 b_mn) {
-  return (1u << 4) | (a_mn << 15) | (b_mn << 16) | ((n >> 3) << 17) | ((u32)(HG_M >> 4) << 24);
+// D f32, A and B f16
+__host__ __device__ constexpr u32 idesc_f16(u32 m, u32 n, u32 a_mn, u32 b_mn) {
+  return (1u << 4) | (a_mn << 15) | (b_mn << 16) | ((n >> 3) << 17) | ((m >> 4) << 24);
 }
 __device__ __forceinline__ bool elect_one() {
   u32 p;
   asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(p));
   return p != 0;
 }
-template <u32 ID, u32 AH, u32 BH>
+template <int CTAS, u32 ID, u32 AH, u32 BH>
 __device__ __forceinline__ void mma_f16(u32 tmem, u32 a, u32 b, bool accumulate) {
-  asm volatile("{\n .reg .pred p;\n .reg .b64 x, y;\n setp.ne.b32 p, %3, 0;\n mov.b64 x, {%1, %5};\n mov.b64 y, {%2, %6};\n"
-               " tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %4, p;\n}"
-               :: "r"(tmem), "r"(a), "r"(b), "r"((u32)accumulate), "n"(ID), "n"(AH), "n"(BH) : "memory");
+  if constexpr (CTAS == 2)
+    asm volatile("{\n .reg .pred p;\n .reg .b64 x, y;\n setp.ne.b32 p, %3, 0;\n mov.b64 x, {%1, %5};\n mov.b64 y, {%2, %6};\n"
+                 " tcgen05.mma.cta_group::2.kind::f16 [%0], x, y, %4, p;\n}"
+                 :: "r"(tmem), "r"(a), "r"(b), "r"((u32)accumulate), "n"(ID), "n"(AH), "n"(BH) : "memory");
+  else
+    asm volatile("{\n .reg .pred p;\n .reg .b64 x, y;\n setp.ne.b32 p, %3, 0;\n mov.b64 x, {%1, %5};\n mov.b64 y, {%2, %6};\n"
+                 " tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %4, p;\n}"
+                 :: "r"(tmem), "r"(a), "r"(b), "r"((u32)accumulate), "n"(ID), "n"(AH), "n"(BH) : "memory");
+}
+
+// ---- a pair of CTAs (a cluster of two, the even one its leader) ----
+__device__ __forceinline__ u32 pair_rank() { u32 r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ void pair_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n barrier.cluster.wait.acquire;" ::: "memory");
+}
+// this CTA's shared-memory address in the leader
+__device__ __forceinline__ u32 in_leader(u32 addr) {
+  u32 r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+  return r;
+}
+// a tile into this CTA, its bytes counted by a barrier of the pair's
+__device__ __forceinline__ void pair_load_3d(u32 dst, const TmaDesc* map, u32 bar, int c0, int c1, int c2) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 "
+               "[%0], [%1, {%2, %3, %4}], [%5];"
+               :: "r"(dst), "l"(reinterpret_cast<u64>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar) : "memory");
+}
+// arrives at the same barrier of both CTAs when the pair's products so far are done
+__device__ __forceinline__ void pair_commit(u32 bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+               :: "r"(bar), "h"((unsigned short)3) : "memory");
 }
 __device__ __forceinline__ void tmem_ld32(u32 taddr, float (&r)[32]) {
   u32 v[32];
@@ -170,7 +199,7 @@ __device__ __forceinline__ F16Tile f16_tile(u32 u, u32 tm, u32 tn, u32 per) {
   if (SYM) {
     u32 i = 0;
     for (;; ++i) {
-      const u32 first = i * HG_M / BN, n = tn - first;
+      const u32 first = i * F16x3<BN>::TM / BN, n = tn - first;
       if (r < n) { nt = first + r; break; }
       r -= n;
     }
@@ -182,7 +211,7 @@ __device__ __forceinline__ F16Tile f16_tile(u32 u, u32 tm, u32 tn, u32 per) {
     mt = first + w % gsz;
     nt = w / gsz;
   }
-  T.m0 = (int)(mt * HG_M);
+  T.m0 = (int)(mt * F16x3<BN>::TM);
   T.n0 = (int)(nt * BN);
   return T;
 }
@@ -190,14 +219,14 @@ template <int BN, bool SYM>
 __device__ __forceinline__ u32 f16_tiles(u32 tm, u32 tn) {
   if (!SYM) return tm * tn;
   u32 n = 0;
-  for (u32 i = 0; i < tm; ++i) n += tn - i * HG_M / BN;
+  for (u32 i = 0; i < tm; ++i) n += tn - i * F16x3<BN>::TM / BN;
   return n;
 }
 
-// The work of one CTA, in order: whole tiles, then its run of the divided ones.
+// The work of one CTA or pair, in order: whole tiles, then its run of the divided ones.
 struct F16Work {
   u32 tiles, full, chunks, quantum, per;   // per: units of a divided tile
-  u32 grid, u;                             // CTAs; next whole tile
+  u32 grid, u;                             // CTAs (or pairs); next whole tile
   u64 at, end, total;                      // the run, in units over the divided tiles
   u32 tile, c0, c1;                        // the current piece: chunks c0 .. c1 of a tile
   __device__ __forceinline__ F16Work(u32 tiles_, u32 full_, u32 chunks_, u32 quantum_, u32 block, u32 grid_)
@@ -326,10 +355,12 @@ __device__ __forceinline__ void gemm_f16x3(const F16Job& J, u32* err, EPI& epi) 
   auto accf = [&](u32 b) { return bars + 8u * (2 * STAGES + b); };
   auto acce = [&](u32 b) { return bars + 8u * (2 * STAGES + 2 + b); };
   const u32 M = J.M, N = J.N;
-  const u32 tm = (M + HG_M - 1) / HG_M, tn = (N + BN - 1) / BN, kbs = (J.K + HG_K - 1) / HG_K;
+  constexpr u32 CTAS = S::CTAS, TM = S::TM;
+  const u32 rank = CTAS == 2 ? pair_rank() : 0, unit = J.block / CTAS;
+  const u32 tm = (M + TM - 1) / TM, tn = (N + BN - 1) / BN, kbs = (J.K + HG_K - 1) / HG_K;
   constexpr u32 CK = CHUNK / HG_K;   // stages of a chunk
   const u32 per = f16_tiles<BN, SYM>(tm, tn);
-  F16Work work(per * J.batch, J.full, (kbs + CK - 1) / CK, J.quantum, J.block, J.grid);
+  F16Work work(per * J.batch, J.full, (kbs + CK - 1) / CK, J.quantum, unit, J.grid / CTAS);
 
   if (threadIdx.x == 32 * 3) {
     asm volatile("prefetch.tensormap [%0];" :: "l"(reinterpret_cast<u64>(J.ma)) : "memory");
@@ -337,16 +368,23 @@ __device__ __forceinline__ void gemm_f16x3(const F16Job& J, u32* err, EPI& epi) 
   }
   if (threadIdx.x == 0) {
     for (u32 s = 0; s < STAGES; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
-    for (u32 b = 0; b < 2; ++b) { mbar_init(accf(b), 1); mbar_init(acce(b), 8); }
+    for (u32 b = 0; b < 2; ++b) { mbar_init(accf(b), 1); mbar_init(acce(b), 8 * CTAS); }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(tmem_slot)),
-                 "r"(S::TMEM) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    if constexpr (CTAS == 2) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(tmem_slot)),
+                   "r"(S::TMEM) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(tmem_slot)),
+                   "r"(S::TMEM) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
   }
   tc_fence_before();
   __syncthreads();
+  if constexpr (CTAS == 2) pair_sync();   // both CTAs' barriers are set up
   tc_fence_after();
   const u32 tmem = *tmem_slot;
   grid_dependency_sync();   // the set-up above touched this CTA's shared and tensor memory only
@@ -368,34 +406,37 @@ __device__ __forceinline__ void gemm_f16x3(const F16Job& J, u32* err, EPI& epi) 
           if (it >= STAGES && !wait(empty(s), phase ^ 1, 1)) { ok = false; break; }
           const u32 st = base + s * S::STAGE, sb = st + 2 * S::A_BYTES;
           const int kc = (int)(kb * HG_K);
+          const u32 bar = CTAS == 2 ? in_leader(full(s)) : full(s);
+          const int m0 = T.m0 + (int)rank * HG_M, n0 = T.n0 + (int)rank * S::COLS;
           auto load = [&](u32 dst, const TmaDesc* map, int col, int row) {
-            if (BLOCKED) tma_load_3d(dst, map, full(s), col & 255, row, 2 * (col >> 8));
-            else tma_load_3d(dst, map, full(s), col, row, 2 * T.bz);
+            const int c = BLOCKED ? col & 255 : col, z = BLOCKED ? 2 * (col >> 8) : 2 * T.bz;
+            if constexpr (CTAS == 2) pair_load_3d(dst, map, bar, c, row, z);
+            else tma_load_3d(dst, map, bar, c, row, z);
           };
           if (leader) {
-            mbar_expect_tx(full(s), S::STAGE);
+            if (rank == 0) mbar_expect_tx(full(s), CTAS * S::STAGE);
             // a box holds a tile's hi plane and, behind it, its lo plane
             if (A_MN) {
 #pragma unroll
-              for (int c = 0; c < HG_M / 64; ++c) load(st + c * HG_K * 256, J.ma, T.m0 + 64 * c, kc);
+              for (int c = 0; c < HG_M / 64; ++c) load(st + c * HG_K * 256, J.ma, m0 + 64 * c, kc);
             } else {
-              load(st, J.ma, kc, T.m0);
+              load(st, J.ma, kc, m0);
             }
             if (B_MN) {
 #pragma unroll
-              for (int c = 0; c < BN / 64; ++c) load(sb + c * HG_K * 256, J.mb, T.n0 + 64 * c, kc);
+              for (int c = 0; c < S::COLS / 64; ++c) load(sb + c * HG_K * 256, J.mb, n0 + 64 * c, kc);
             } else {
-              load(sb, J.mb, kc, T.n0);
+              load(sb, J.mb, kc, n0);
             }
           }
           __syncwarp();
           if (++s == STAGES) { s = 0; phase ^= 1; }
         }
       }
-      // wait (bounded) for the copies still in flight before this CTA may exit
-      for (u32 i = it > STAGES ? it - STAGES : 0; i < it; ++i) mbar_wait(full(i % STAGES), (i / STAGES) & 1, err, 2);
-    } else if (warp == 1) {
-      constexpr u32 ID = idesc_f16(BN, A_MN ? 1u : 0u, B_MN ? 1u : 0u), AH = f16_desc_hi<A_MN>(), BH = f16_desc_hi<B_MN>();
+      // wait (bounded) for the copies still in flight before this CTA (the leader: the pair) may exit
+      if (rank == 0) for (u32 i = it > STAGES ? it - STAGES : 0; i < it; ++i) mbar_wait(full(i % STAGES), (i / STAGES) & 1, err, 2);
+    } else if (warp == 1 && rank == 0) {
+      constexpr u32 ID = idesc_f16(TM, BN, A_MN ? 1u : 0u, B_MN ? 1u : 0u), AH = f16_desc_hi<A_MN>(), BH = f16_desc_hi<B_MN>();
       // hi to lo plane, and one K step on, in descriptor units of 16 bytes
       constexpr u32 AL = (A_MN ? HG_K * 128 : S::A_BYTES) >> 4, AK = (A_MN ? 2048 : 32) >> 4;
       constexpr u32 BL = (B_MN ? HG_K * 128 : S::B_BYTES) >> 4, BK = (B_MN ? 2048 : 32) >> 4;
@@ -417,23 +458,27 @@ __device__ __forceinline__ void gemm_f16x3(const F16Job& J, u32* err, EPI& epi) 
                 const u32 ah = da + AK * k, al = ah + AL, bh = db + BK * k, bl = bh + BL;
                 const bool on = k > 0 || kb != 0;
                 if (S::ACCS == 1) {
-                  mma_f16<ID, AH, BH>(acc, al, bh, on);
-                  mma_f16<ID, AH, BH>(acc, ah, bl, true);
-                  mma_f16<ID, AH, BH>(acc, ah, bh, true);
+                  mma_f16<CTAS, ID, AH, BH>(acc, al, bh, on);
+                  mma_f16<CTAS, ID, AH, BH>(acc, ah, bl, true);
+                  mma_f16<CTAS, ID, AH, BH>(acc, ah, bh, true);
                 } else {
-                  mma_f16<ID, AH, BH>(acc + BN, al, bh, on);
-                  mma_f16<ID, AH, BH>(acc, ah, bh, on);
-                  mma_f16<ID, AH, BH>(acc + (S::ACCS - 1) * BN, ah, bl, S::ACCS == 2 || on);
+                  mma_f16<CTAS, ID, AH, BH>(acc + BN, al, bh, on);
+                  mma_f16<CTAS, ID, AH, BH>(acc, ah, bh, on);
+                  mma_f16<CTAS, ID, AH, BH>(acc + (S::ACCS - 1) * BN, ah, bl, S::ACCS == 2 || on);
                 }
               }
-              mma_commit(empty(s));
+              if constexpr (CTAS == 2) pair_commit(empty(s));
+              else mma_commit(empty(s));
             }
             __syncwarp();
             da += S::STAGE >> 4;
             db += S::STAGE >> 4;
             if (++s == STAGES) { s = 0; phase ^= 1; da = a0; db = b0; }
           }
-          if (ok && leader) mma_commit(accf(buf));
+          if (ok && leader) {
+            if constexpr (CTAS == 2) pair_commit(accf(buf));
+            else mma_commit(accf(buf));
+          }
           __syncwarp();
         }
       }
@@ -456,6 +501,7 @@ __device__ __forceinline__ void gemm_f16x3(const F16Job& J, u32* err, EPI& epi) 
     bool ok = true;
     while (ok && work.next()) {
       e.T = f16_tile<BN, SYM>(work.tile, tm, tn, per);
+      e.T.m0 += (int)rank * HG_M;
       e.row = (u64)e.T.m0 + 32 * e.q + lane;
       epi.begin(e);   // its loads are on their way while the products run
       float v[NB][32];
@@ -470,20 +516,25 @@ __device__ __forceinline__ void gemm_f16x3(const F16Job& J, u32* err, EPI& epi) 
         f16_collect<BN, 0>(v, tmem + buf * S::ACCS * BN + ((u32)(32 * e.q) << 16) + (u32)e.c0);
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(acce(buf)) : "memory");
+        if (lane == 0) {
+          if constexpr (CTAS == 2)
+            asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" :: "r"(in_leader(acce(buf))) : "memory");
+          else
+            asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(acce(buf)) : "memory");
+        }
       }
       // this warp's part of the tile reaches into the output
       bool mine = ok && (u32)e.T.m0 + 32 * e.q < M && (u32)(e.T.n0 + e.c0) < N;
       if (mine && !work.whole()) {
-        // CTA c's slots: 2 c + 1 for the beginning of a tile, 2 c for a later part of one
-        constexpr u64 SLOT = (u64)8 * NB * 1024;
-        float* part = J.part + (u64)w * NB * 1024 + lane;
-        f16_partial_store<0>(v, part + (2 * J.block + (work.c0 == 0)) * SLOT);
+        // CTA (or pair) c's slots: 2 c + 1 for the beginning of a tile, 2 c for a later part of one
+        constexpr u64 SLOT = (u64)8 * NB * 1024 * CTAS;
+        float* part = J.part + (u64)(8 * rank + w) * NB * 1024 + lane;
+        f16_partial_store<0>(v, part + (2 * unit + (work.c0 == 0)) * SLOT);
         __threadfence();
         __syncwarp();
         const u64 first = (u64)(work.tile - work.full) * work.per;
         const u32 ca = work.owner(first), cb = work.owner(first + work.per - 1);
-        u32* count = J.counters + (work.tile - work.full) * 8 + w;
+        u32* count = J.counters + ((work.tile - work.full) * CTAS + rank) * 8 + w;
         u32 old = 0;
         if (lane == 0) old = atomicAdd(count, 1u);
         old = __shfl_sync(0xffffffffu, old, 0);
@@ -505,11 +556,20 @@ __device__ __forceinline__ void gemm_f16x3(const F16Job& J, u32* err, EPI& epi) 
   }
   tc_fence_before();
   __syncthreads();
+  if constexpr (CTAS == 2) pair_sync();   // neither CTA ends, nor gives up its tensor memory, while the other works
   if (warp == 1) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(S::TMEM) : "memory");
+    if constexpr (CTAS == 2)
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(S::TMEM) : "memory");
+    else
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(S::TMEM) : "memory");
   }
 }
+
+// a kernel's cluster by tile width
+#define TCB_F16_CLUSTER_256 __cluster_dims__(2, 1, 1)
+#define TCB_F16_CLUSTER_128
+#define TCB_F16_CLUSTER_64
 
 // ---- what the operators share ----
 

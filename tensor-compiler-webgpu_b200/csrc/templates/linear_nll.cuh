@@ -474,7 +474,8 @@ struct NllOut {
 }  // namespace tcb
 
 #define TCB_NLL_GEMM(NAME, BN, AMN, BMN, EPI, ...)                                                                          \
-  extern "C" __global__ void __launch_bounds__(tcb::HG_THREADS, 1) NAME##_##BN(const __grid_constant__ tcb::GemmParams P) { \
+  extern "C" __global__ void TCB_F16_CLUSTER_##BN                                                                         \
+      __launch_bounds__(tcb::HG_THREADS, 1) NAME##_##BN(const __grid_constant__ tcb::GemmParams P) {                        \
     tcb::EPI epi(__VA_ARGS__);                                                                                              \
     tcb::gemm_f16x3<BN, AMN, BMN, false, true, 256>(tcb::f16_job(P), reinterpret_cast<u32*>(P.a.p[15]), epi);               \
   }

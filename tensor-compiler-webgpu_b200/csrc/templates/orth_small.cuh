@@ -28,13 +28,13 @@ constexpr u32 OS_HI = 1024u >> 4 | 1u << 14 | 2u << 29;   // 8-row groups 1 KB a
 // accumulators of ACC columns (0: one).
 template <u32 N, bool BMN, u32 ACC>
 __device__ __forceinline__ void os_product(u32 tmem, u32 a, u32 b, u32 steps) {
-  constexpr u32 ID = idesc_f16(N, 0, BMN ? 1 : 0), L = OS_PLANE >> 4;
+  constexpr u32 ID = idesc_f16(128, N, 0, BMN ? 1 : 0), L = OS_PLANE >> 4;
   for (u32 k = 0; k < steps; ++k) {
     const u32 ka = (k >> 2) * OS_BLOCK + (k & 3) * 32;
     const u32 ah = os_lo<false>(a + ka), bh = os_lo<BMN>(b + (BMN ? k * 2048 : ka));
-    mma_f16<ID, OS_HI, OS_HI>(tmem + (ACC ? ACC : 0), ah + L, bh, k != 0);
-    mma_f16<ID, OS_HI, OS_HI>(tmem + 2 * ACC, ah, bh + L, ACC ? k != 0 : true);
-    mma_f16<ID, OS_HI, OS_HI>(tmem, ah, bh, ACC ? k != 0 : true);
+    mma_f16<1, ID, OS_HI, OS_HI>(tmem + (ACC ? ACC : 0), ah + L, bh, k != 0);
+    mma_f16<1, ID, OS_HI, OS_HI>(tmem + 2 * ACC, ah, bh + L, ACC ? k != 0 : true);
+    mma_f16<1, ID, OS_HI, OS_HI>(tmem, ah, bh, ACC ? k != 0 : true);
   }
 }
 

@@ -162,7 +162,7 @@ struct NsSymmetric {
     }
     store_split32(e, map, v, (int)col, e.T.m0 + 32 * e.q, e.T.bz);
     const u32 row0 = (u32)e.T.m0 + 32 * e.q;
-    if (row0 / BN < col / HG_M * HG_M / BN) {   // the mirror's tile is not computed
+    if (row0 / BN < col / F16x3<BN>::TM * F16x3<BN>::TM / BN) {   // the mirror's tile is not computed
       if (e.lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
       turn32(e, v);   // lane l: row l of the mirrored block
       store_split32(e, map, v, (int)row0, (int)col, e.T.bz);
@@ -213,7 +213,8 @@ struct NsApply {
 }  // namespace tcb
 
 #define TCB_NS_GEMM(NAME, BN, AMN, BMN, SYM, EPI)                                                                         \
-  extern "C" __global__ void __launch_bounds__(tcb::HG_THREADS, 1) NAME##_##BN(const __grid_constant__ tcb::GemmParams P) { \
+  extern "C" __global__ void TCB_F16_CLUSTER_##BN                                                                         \
+      __launch_bounds__(tcb::HG_THREADS, 1) NAME##_##BN(const __grid_constant__ tcb::GemmParams P) {                      \
     tcb::EPI epi(P);                                                                                                      \
     tcb::gemm_f16x3<BN, AMN, BMN, SYM, false, 128>(tcb::f16_job(P), reinterpret_cast<u32*>(P.a.p[15]), epi);              \
   }

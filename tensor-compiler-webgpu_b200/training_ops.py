@@ -31,8 +31,13 @@ def _up(n, k):
     return -(-n // k) * k
 
 
+def f16_ctas(bn):
+    """CTAs of a tile: a pair of SMs works on 256 x 256, each loading 128 rows of A and 128 columns of B."""
+    return 2 if bn == 256 else 1
+
+
 def _f16_stages(bn):
-    stage = 2 * F16_BM * F16_BK * 2 + 2 * bn * F16_BK * 2
+    stage = 2 * F16_BM * F16_BK * 2 + 2 * (bn // f16_ctas(bn)) * F16_BK * 2
     return min(8, (227 * 1024 - F16_EXTRA) // stage), stage
 
 
@@ -43,8 +48,9 @@ def f16_smem(bn):
 
 
 def f16_tiles(M, N, bn, symmetric):
-    tm, tn = math.ceil(M / F16_BM), math.ceil(N / bn)
-    return sum(tn - i * F16_BM // bn for i in range(tm)) if symmetric else tm * tn
+    rows = F16_BM * f16_ctas(bn)
+    tm, tn = math.ceil(M / rows), math.ceil(N / bn)
+    return sum(tn - i * rows // bn for i in range(tm)) if symmetric else tm * tn
 
 
 # Nanoseconds of a split-fp16 product by tile width, as measured with every SM busy: a K step of 16 of one tile;
@@ -62,18 +68,20 @@ def f16_plan(M, N, K, batch, chunk, symmetric=False):
     best = None
     steps = math.ceil(K / 16)
     for bn, (step, epi, once, part) in F16_COST.items():
-        if bn > 64 and N <= bn // 2:
+        ctas = f16_ctas(bn)
+        units = SM_COUNT // ctas
+        if (bn > 64 and N <= bn // 2) or M <= F16_BM * (ctas - 1):
             continue
         tiles = batch * f16_tiles(M, N, bn, symmetric)
-        plans = [(math.ceil(tiles / SM_COUNT) * (steps * step + epi), bn, min(SM_COUNT, tiles), tiles, 1)]
+        plans = [(math.ceil(tiles / units) * (steps * step + epi), bn, min(units, tiles) * ctas, tiles, 1)]
         for q in (1, 2, 4, 8, 16, 32, 64):
             per = math.ceil(K / (256 * q))
-            if tiles >= SM_COUNT or per == 1:
+            if tiles >= units or per == 1:
                 break
-            grid = min(SM_COUNT, tiles * per)
+            grid = min(units, tiles * per)
             run = math.ceil(tiles * per / grid)
             pieces = per if run == 1 else per // run + 2
-            plans.append((run * q * 16 * step + once + pieces * part + epi, bn, grid, 0, q * (256 // chunk)))
+            plans.append((run * q * 16 * step + once + pieces * part + epi, bn, grid * ctas, 0, q * (256 // chunk)))
         for p in plans:
             if best is None or p[0] < best[0]:
                 best = p
@@ -87,7 +95,7 @@ def f16_partial_bytes(grid, whole, tiles, bn):
 def _operand(off, plane, cols, rows, batch, pitch, mn, bn, region="scratch"):
     """The map of an operand's hi and lo planes, one behind the other for each matrix: boxes of 64 x F16_BK when
     its M or N index runs along the rows, else of F16_BK x (128 or the tile width)."""
-    box = (64 | F16 | PAIR, F16_BK) if mn else (F16_BK | F16 | PAIR, bn)
+    box = (64 | F16 | PAIR, F16_BK) if mn else (F16_BK | F16 | PAIR, bn // f16_ctas(bn))
     assert plane == batch * rows * pitch * 2
     return [(region, off, cols, rows, 2 * batch, pitch * 2, rows * pitch * 2, *box)]
 
@@ -103,7 +111,7 @@ def _pitch(cols):
 
 
 def _blocked_operand(region, off, rows, cols, pitch, mn, bn):
-    return _blocked(region, off, rows, cols, pitch, *((64, F16_BK) if mn else (F16_BK, bn)))
+    return _blocked(region, off, rows, cols, pitch, *((64, F16_BK) if mn else (F16_BK, bn // f16_ctas(bn))))
 
 
 def _at(index, off):

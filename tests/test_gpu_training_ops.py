@@ -340,6 +340,19 @@ def test_orthogonalize_stack_members_do_not_meet(pkg, mods, runner):
     assert np.array_equal(got[0], alone[0]) and np.array_equal(got[2], alone[2]) and np.isnan(got[1]).all()
 
 
+@pytest.mark.parametrize("divide", [False, True])
+@pytest.mark.parametrize("bn", [64, 128, 256])
+def test_every_tile_width_whole_and_divided(pkg, mods, runner, monkeypatch, bn, divide):
+    """The products by each tile width alone, their tiles whole or divided along K, at sizes with ragged edges."""
+    to = importlib.import_module(P + ".training_ops")
+    monkeypatch.setattr(to, "F16_COST", {bn: (100, 1000, 0, 0) if divide else (100, 1000, 10 ** 9, 0)})
+    for R, d, V in ((150, 140, 257), (300, 200, 700), (900, 513, 1300)):
+        check_nll(mods, runner, nll_case(pkg, R, d, V, seed=R), runs=2)
+    for shape in ((140, 150), (390, 130), (2, 257, 600), (2, 300, 520)):
+        x = np.random.default_rng(shape[-1]).standard_normal(shape).astype(np.float32).astype(np.float64)
+        check_orth(mods, runner, pkg, x)
+
+
 # ---------------------------------------------------------------- through the runner
 def test_runner_reads_every_node_with_canaries(pkg, mods, runner):
     """GpuRunner.run: a buffer per node, canaries behind each; several gradients of one launch among them."""
