@@ -264,13 +264,12 @@ def test_division_of_a_product(mods, M, N, K, batch, chunk, sym):
     """The device's division of tiles among CTAs, restated: every chunk of every tile once, the pieces of a
     divided tile found by the warp that adds them, no two in one slot."""
     pkg, cg, to, rt = mods
-    tile, ctas, whole, q = to.f16_plan(M, N, K, batch, chunk, sym)
-    assert ctas % tile.ctas == 0 and 1 <= ctas <= 148 and M > 128 * (tile.ctas - 1)
-    tiles, grid = batch * to.f16_tiles(M, N, tile, sym), ctas // tile.ctas   # pairs work as one
+    bn, grid, whole, q = to.f16_plan(M, N, K, batch, chunk, sym)
+    tiles = batch * to.f16_tiles(M, N, bn, sym)
     chunks = -(-K // chunk)
     per = -(-chunks // q)
     total = (tiles - whole) * per
-    assert (total == 0 or grid <= total) and (tiles - whole) * tile.ctas <= 148 and (tile.bn == 64 or N > tile.bn // 2)
+    assert 1 <= grid <= 148 and (total == 0 or grid <= total) and tiles - whole < 148 and (bn == 64 or N > bn // 2)
     seen, slots = {}, {}
     for c in range(grid):
         for t in range(c, whole, grid):
@@ -295,7 +294,7 @@ def test_division_of_a_product(mods, M, N, K, batch, chunk, sym):
             ca, cb = (((x + 1) * grid - 1) // total for x in (first, first + per - 1))
             assert [p[2] for p in pieces] == list(range(ca, cb + 1))
             assert [slots[2 * c + (c == ca)][1] for c in range(ca, cb + 1)] == pieces
-    assert to.f16_partial_bytes(ctas, whole, tiles, tile) >= (max(slots) + 1 if slots else 0) * 128 * tile.ctas * tile.bn * 4
+    assert to.f16_partial_bytes(grid, whole, tiles, bn) >= (max(slots) + 1 if slots else 0) * 128 * bn * 4
 
 
 @pytest.mark.parametrize("shape", [[1, 1], [64, 64], [100, 70], [3, 70, 300], [4095, 1000], [2, 2, 256, 1024]])
