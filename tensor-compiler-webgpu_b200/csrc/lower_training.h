@@ -209,68 +209,76 @@ static std::map<int, std::vector<int>> siblings(const Graph& g) {
 }
 
 // ---------------------------------------------------------------- split-fp16 products
-static i64 f16_ctas(i64 bn) { return bn == 256 ? 2 : 1; }
-static i64 f16_smem(i64 bn) {
-  i64 stage = 2 * F16_BM * F16_BK * 2 + 2 * (bn / f16_ctas(bn)) * F16_BK * 2;
+struct Tile {   // of a product: ctas * 128 rows x bn columns
+  i64 bn = 0, ctas = 1;
+  i64 cols() const { return bn / ctas; }   // of B, loaded by one CTA
+  std::string name() const { return std::to_string(bn) + (ctas == 2 ? "x2" : ""); }
+};
+static i64 f16_smem(const Tile& t) {
+  i64 stage = 2 * F16_BM * F16_BK * 2 + 2 * t.cols() * F16_BK * 2;
   i64 stages = std::min<i64>(8, (227 * 1024 - F16_EXTRA) / stage);
   return stages * stage + F16_EXTRA;
 }
-static i64 f16_tiles(i64 M, i64 N, i64 bn, bool symmetric) {
-  const i64 rows = F16_BM * f16_ctas(bn);
-  i64 tm = cdiv(M, rows), tn = cdiv(N, bn), t = 0;
+static i64 f16_tiles(i64 M, i64 N, const Tile& tile, bool symmetric) {
+  const i64 rows = F16_BM * tile.ctas;
+  i64 tm = cdiv(M, rows), tn = cdiv(N, tile.bn), t = 0;
   if (!symmetric) return tm * tn;
-  for (i64 i = 0; i < tm; ++i) t += tn - i * rows / bn;
+  for (i64 i = 0; i < tm; ++i) t += tn - i * rows / tile.bn;
   return t;
 }
 
-struct F16Plan { i64 bn = 0, grid = 0, whole = 0, quantum = 0; };
+struct F16Plan {
+  Tile tile;
+  i64 grid = 0, whole = 0, quantum = 0;
+};
 static F16Plan f16_plan(i64 M, i64 N, i64 K, i64 batch, i64 chunk, bool symmetric = false) {
-  static const i64 COST[3][5] = {{256, 290, 6000, 3000, 2500}, {128, 180, 3000, 1500, 1200}, {64, 140, 1500, 1000, 700}};
+  static const i64 COST[4][6] = {{256, 2, 275, 6600, 3000, 2500}, {128, 2, 173, 3600, 1500, 1600},
+                                 {128, 1, 180, 3000, 1500, 1200}, {64, 1, 140, 1500, 1000, 700}};
   F16Plan best;
   i64 cost = -1;
-  auto take = [&](i64 c, i64 bn, i64 grid, i64 whole, i64 q) {
+  auto take = [&](i64 c, const Tile& tile, i64 grid, i64 whole, i64 q) {
     if (cost >= 0 && c >= cost) return;
     cost = c;
-    best = {bn, grid, whole, q};
+    best = {tile, grid, whole, q};
   };
   const i64 steps = cdiv(K, 16);
   for (auto& row : COST) {
-    const i64 bn = row[0], step = row[1], epi = row[2], once = row[3], part = row[4];
-    const i64 ctas = f16_ctas(bn), units = SM_COUNT / ctas;
-    if ((bn > 64 && N <= bn / 2) || M <= F16_BM * (ctas - 1)) continue;
-    const i64 tiles = batch * f16_tiles(M, N, bn, symmetric);
-    take(cdiv(tiles, units) * (steps * step + epi), bn, std::min<i64>(units, tiles) * ctas, tiles, 1);
+    const Tile tile{row[0], row[1]};
+    const i64 step = row[2], epi = row[3], once = row[4], part = row[5], units = SM_COUNT / tile.ctas;
+    if ((tile.bn > 64 && N <= tile.bn / 2) || M <= F16_BM * (tile.ctas - 1)) continue;
+    const i64 tiles = batch * f16_tiles(M, N, tile, symmetric);
+    take(cdiv(tiles, units) * (steps * step + epi), tile, std::min<i64>(units, tiles) * tile.ctas, tiles, 1);
     for (i64 q = 1; q <= 64; q *= 2) {
       const i64 per = cdiv(K, 256 * q);
       if (tiles >= units || per == 1) break;
       const i64 grid = std::min<i64>(units, tiles * per), run = cdiv(tiles * per, grid);
       const i64 pieces = run == 1 ? per : per / run + 2;
-      take(run * q * 16 * step + once + pieces * part + epi, bn, grid * ctas, 0, q * (256 / chunk));
+      take(run * q * 16 * step + once + pieces * part + epi, tile, grid * tile.ctas, 0, q * (256 / chunk));
     }
   }
   return best;
 }
-static i64 f16_partial_bytes(const F16Plan& p, i64 tiles) { return p.whole == tiles ? 0 : 2 * p.grid * F16_BM * p.bn * 4; }
+static i64 f16_partial_bytes(const F16Plan& p, i64 tiles) { return p.whole == tiles ? 0 : 2 * p.grid * F16_BM * p.tile.bn * 4; }
 
-static Map f16_operand(i64 off, i64 cols, i64 rows, i64 batch, i64 pitch, bool mn, i64 bn) {
+static Map f16_operand(i64 off, i64 cols, i64 rows, i64 batch, i64 pitch, bool mn, i64 box_rows) {
   return {"scratch", off, cols, rows, 2 * batch, pitch * 2, rows * pitch * 2, (mn ? 64 : F16_BK) | F16_FLAG | PAIR_FLAG,
-          mn ? F16_BK : bn / f16_ctas(bn)};
+          mn ? F16_BK : box_rows};
 }
 static Map blocked(const std::string& region, i64 off, i64 rows, i64 cols, i64 pitch, i64 box_cols, i64 box_rows) {
   return {region, off, pitch, rows, 2 * cdiv(cols, 256), pitch * 2, rows * pitch * 2, box_cols | F16_FLAG | PAIR_FLAG, box_rows};
 }
-static Map blocked_operand(const std::string& region, i64 off, i64 rows, i64 cols, i64 pitch, bool mn, i64 bn) {
+static Map blocked_operand(const std::string& region, i64 off, i64 rows, i64 cols, i64 pitch, bool mn, i64 box_rows) {
   return mn ? blocked(region, off, rows, cols, pitch, 64, F16_BK)
-            : blocked(region, off, rows, cols, pitch, F16_BK, bn / f16_ctas(bn));
+            : blocked(region, off, rows, cols, pitch, F16_BK, box_rows);
 }
 
 static Call f16_gemm(const std::string& name, i64 M, i64 N, i64 K, i64 batch, const F16Plan& p, i64 part_at,
                      std::vector<Map> maps, const std::vector<i64>& params, i64 err, i64* partial, bool symmetric = false) {
-  const i64 tiles = batch * f16_tiles(M, N, p.bn, symmetric);
+  const i64 tiles = batch * f16_tiles(M, N, p.tile, symmetric);
   if (tiles >= ((i64)1 << 31)) throw Error(name + ": " + std::to_string(tiles) + " tiles");
   std::vector<i64> ps = {M | N << 32, K | batch << 32, p.whole | p.quantum << 32, part_at};
   ps.insert(ps.end(), params.begin(), params.end());
-  Call c = make_call(name + "_" + std::to_string(p.bn), {p.grid, 1, 1}, {384, 1, 1}, f16_smem(p.bn), ps);
+  Call c = make_call(name + "_" + p.tile.name(), {p.grid, 1, 1}, {384, 1, 1}, f16_smem(p.tile), ps);
   c.tma = std::move(maps);
   c.has_tma = true;
   c.err_offset = err;
@@ -318,7 +326,7 @@ static Launch nll_launch(const Graph& g, const std::vector<int>& ids) {
   for (int i : ids) (word_attr(g.nodes[i], "out") == "loss" ? loss : saved) = i;
   const NllSaved in = nll_saved(R, d, V);
   const F16Plan plan = f16_plan(R, V, d, 1, NLL_CHUNK);
-  const i64 halves = cdiv(V, plan.bn / 2);
+  const i64 halves = cdiv(V, plan.tile.bn / 2);
   Regions r;
   r.add(8 * AMAX_BLOCKS);
   const i64 err = r.add(NLL_CTRL_BYTES), zt = r.add(4 * R), part = r.add(8 * R * halves);
@@ -330,7 +338,7 @@ static Launch nll_launch(const Graph& g, const std::vector<int>& ids) {
   const std::string region = saved >= 0 ? "out" : "scratch";
   const i64 base = saved >= 0 ? 0 : saved_at;
   std::vector<Map> maps = {blocked_operand(region, base + in.h, R, d, nll_pitch(d), false, F16_BM),
-                           blocked_operand(region, base + in.w, d, V, nll_pitch(V), true, plan.bn)};
+                           blocked_operand(region, base + in.w, d, V, nll_pitch(V), true, plan.tile.cols())};
   const i64 blocks = std::max<i64>(1, std::min<i64>(AMAX_BLOCKS, cdiv(R * d + d * V, 2048)));
   const i64 units = d * cdiv(V, 1024) + R * cdiv(d, 1024);
   i64 partial = 0;
@@ -350,7 +358,7 @@ static Launch nll_launch(const Graph& g, const std::vector<int>& ids) {
     }
   Launch l = training_record(node, "linear-nll", nll_source(bool_attr(node, "bias")), std::move(calls),
                              r.end + up_to(partial, 256));
-  l.info = {{"rnv", arr({num(R), num(d), num(V)})}, {"bn", num(plan.bn)}, {"ctrl_bytes", num(up_to(NLL_CTRL_BYTES, 64))},
+  l.info = {{"rnv", arr({num(R), num(d), num(V)})}, {"tile", str(plan.tile.name())}, {"ctrl_bytes", num(up_to(NLL_CTRL_BYTES, 64))},
             {"path", str("tcgen05-f16x3")}};
   return l;
 }
@@ -382,8 +390,8 @@ static Launch nll_grad_launch(const Graph& g, const std::vector<int>& ids) {
     const std::vector<i64> params = cat(tail, {v0, (k ? NLL_ADD : 0) | (joined ? NLL_JOIN : 0) | (wb ? NLL_DB : 0)});
     const i64 w_at = in.w + (v0 ? 4 * d * v0 : 0);
     auto h = [&](bool mn) { return blocked_operand("in_at", in.h << 3 | 1, R, d, nll_pitch(d), mn, F16_BM); };
-    auto w = [&](bool mn, i64 bn) { return blocked_operand("in_at", w_at << 3 | 1, d, n, nll_pitch(V), mn, bn); };
-    auto z = [&](bool mn, i64 bn) { return blocked_operand("scratch", dz, R, n, nll_pitch(n), mn, bn); };
+    auto w = [&](bool mn, i64 box_rows) { return blocked_operand("in_at", w_at << 3 | 1, d, n, nll_pitch(V), mn, box_rows); };
+    auto z = [&](bool mn, i64 box_rows) { return blocked_operand("scratch", dz, R, n, nll_pitch(n), mn, box_rows); };
     auto add = [&](const std::string& name, i64 M, i64 N, i64 K, const F16Plan& p, std::vector<Map> maps) -> Call& {
       i64 nbytes = 0;
       calls.push_back(f16_gemm(name, M, N, K, 1, p, r.end, std::move(maps), params, err, &nbytes));
@@ -391,26 +399,26 @@ static Launch nll_grad_launch(const Graph& g, const std::vector<int>& ids) {
       return calls.back();
     };
     const F16Plan pz = f16_plan(R, n, d, 1, NLL_CHUNK);
-    Call& c = add("tcb_nll_dz", R, n, d, pz, {h(false), w(true, pz.bn), blocked("scratch", dz, R, n, nll_pitch(n), 32, 32)});
+    Call& c = add("tcb_nll_dz", R, n, d, pz, {h(false), w(true, pz.tile.cols()), blocked("scratch", dz, R, n, nll_pitch(n), 32, 32)});
     if (joined) c.ptr_params = {{14, want["b"]}};
     const F16Plan ph = f16_plan(R, d, n, 1, NLL_CHUNK), pw = f16_plan(d, n, R, 1, NLL_CHUNK);
-    if (wh && ww && std::max(ph.bn, pw.bn) <= 128 && ph.grid + pw.grid <= SM_COUNT) {
+    if (wh && ww && ph.tile.ctas == 1 && pw.tile.ctas == 1 && ph.grid + pw.grid <= SM_COUNT) {
       i64 hb = 0;
-      Call b = f16_gemm("tcb_nll_both", R, d, n, 1, ph, r.end, {z(false, F16_BM), w(false, ph.bn), h(true), z(true, pw.bn)}, params, err, &hb);
-      b.name = "tcb_nll_both_" + std::to_string(ph.bn) + "_" + std::to_string(pw.bn);
+      Call b = f16_gemm("tcb_nll_both", R, d, n, 1, ph, r.end, {z(false, F16_BM), w(false, ph.tile.cols()), h(true), z(true, pw.tile.cols())}, params, err, &hb);
+      b.name = "tcb_nll_both_" + ph.tile.name() + "_" + pw.tile.name();
       b.grid[0] = ph.grid + pw.grid;
-      b.smem = std::max(f16_smem(ph.bn), f16_smem(pw.bn));
+      b.smem = std::max(f16_smem(ph.tile), f16_smem(pw.tile));
       b.params[7] = pw.whole | pw.quantum << 32;
       b.params[8] = r.end + up_to(hb, 256);
       b.params.push_back(ph.grid);
       b.ptr_params = {{9, want["w"]}};
       to(b, "h");
-      partial = std::max(partial, up_to(hb, 256) + f16_partial_bytes(pw, f16_tiles(d, n, pw.bn, false)));
+      partial = std::max(partial, up_to(hb, 256) + f16_partial_bytes(pw, f16_tiles(d, n, pw.tile, false)));
       calls.push_back(std::move(b));
       continue;
     }
-    if (wh) to(add("tcb_nll_dh", R, d, n, ph, {z(false, F16_BM), w(false, ph.bn)}), "h");
-    if (ww) to(add("tcb_nll_dw", d, n, R, pw, {h(true), z(true, pw.bn)}), "w");
+    if (wh) to(add("tcb_nll_dh", R, d, n, ph, {z(false, F16_BM), w(false, ph.tile.cols())}), "h");
+    if (ww) to(add("tcb_nll_dw", d, n, R, pw, {h(true), z(true, pw.tile.cols())}), "w");
   }
   if (wb && !joined) {
     calls.push_back(make_call("tcb_nll_db", {cdiv(V, 32), 1, 1}, {256, 1, 1}, 0, cat(cat({0, 0, 0, 0}, tail), {0, 0})));
@@ -512,8 +520,8 @@ static Launch orth_launch(const Graph& g, const Node& node) {
   calls[0].err_offset = err;
   calls.push_back(make_call("tcb_orth_split", {std::max<i64>(1, std::min<i64>(m * cdiv(n, 1024), SM_COUNT * 8)), batch, 1},
                             {256, 1, 1}, 0, {parts, 0, 0, 0, m, n, x0}));
-  auto x_map = [&](i64 off, bool mn, i64 bn) { return f16_operand(off, n, m, batch, xp, mn, bn); };
-  auto s_map = [&](i64 off, i64 bn) { return f16_operand(off, s, s, batch, sp, false, bn); };
+  auto x_map = [&](i64 off, bool mn, i64 box_rows) { return f16_operand(off, n, m, batch, xp, mn, box_rows); };
+  auto s_map = [&](i64 off, i64 box_rows) { return f16_operand(off, s, s, batch, sp, false, box_rows); };
   auto out = [&](i64 off, i64 rs, i64 cs, i64 pitch) {
     return Map{"scratch", off, cs, rs, 2 * batch, pitch * 2, rs * pitch * 2, 32 | F16_FLAG | PAIR_FLAG, 32};
   };
@@ -528,15 +536,15 @@ static Launch orth_launch(const Graph& g, const Node& node) {
   for (i64 k = 0; k < steps; ++k) {
     const i64 cur = k % 2 ? x1 : x0, nxt = k % 2 ? x0 : x1;
     const std::vector<i64> params = {m, n, cur, nxt, s_at, p_at, k == steps - 1 ? 1 : 0};
-    add("tcb_orth_gram" + form, s, s, len, gram, {x_map(cur, tall, F16_BM), x_map(cur, tall, gram.bn), out(s_at, s, s, sp)}, params, true);
-    add("tcb_orth_poly", s, s, s, poly, {s_map(s_at, F16_BM), s_map(s_at, poly.bn), out(p_at, s, s, sp)}, params, true);
-    std::vector<Map> ab = tall ? std::vector<Map>{x_map(cur, false, F16_BM), s_map(p_at, app.bn)}
-                               : std::vector<Map>{s_map(p_at, F16_BM), x_map(cur, true, app.bn)};
+    add("tcb_orth_gram" + form, s, s, len, gram, {x_map(cur, tall, F16_BM), x_map(cur, tall, gram.tile.cols()), out(s_at, s, s, sp)}, params, true);
+    add("tcb_orth_poly", s, s, s, poly, {s_map(s_at, F16_BM), s_map(s_at, poly.tile.cols()), out(p_at, s, s, sp)}, params, true);
+    std::vector<Map> ab = tall ? std::vector<Map>{x_map(cur, false, F16_BM), s_map(p_at, app.tile.cols())}
+                               : std::vector<Map>{s_map(p_at, F16_BM), x_map(cur, true, app.tile.cols())};
     ab.push_back(out(nxt, m, n, xp));
     add("tcb_orth_apply" + form, m, n, s, app, std::move(ab), params, false);
   }
   Launch l = training_record(node, "orthogonalize", code, std::move(calls), r.end + up_to(partial, 256));
-  l.info = {{"mn", arr({num(batch), num(m), num(n)})}, {"bn", arr({num(gram.bn), num(poly.bn), num(app.bn)})},
+  l.info = {{"mn", arr({num(batch), num(m), num(n)})}, {"tiles", arr({str(gram.tile.name()), str(poly.tile.name()), str(app.tile.name())})},
             {"ctrl_bytes", num(up_to(CTRL_BYTES, 64))}, {"path", str("tcgen05-f16x3")}};
   return l;
 }

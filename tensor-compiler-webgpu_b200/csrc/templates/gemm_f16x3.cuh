@@ -20,16 +20,22 @@
 // instructions (a 64-wide product takes about 100 clocks in a chain, 32 by its size).
 //
 // Persistent, one CTA per SM, warps specialised: warp 0 loads the stage's four tiles by TMA, one lane of
-// warp 1 issues three tcgen05.mma.kind::f16 (M = 128, N = BN, K = 16) per K step into one of two TMEM
-// buffers, warps 4-11 collect the other: a quarter of the rows and half of the columns each, up to 128
+// warp 1 issues three tcgen05.mma.kind::f16 (M = 128 or, for a pair, 256, N = BN, K = 16) per K step into one of
+// two TMEM buffers, warps 4-11 collect the other: a quarter of the rows and half of the columns each, up to 128
 // sums a thread, on which the epilogue then runs 32 columns at a time.  They need more registers than an
 // even share (168), so the first warpgroup gives up most of its own: 40 + 2 x 232 = 3 x 168.  Either
 // operand may be K-major (64-byte rows) or MN-major (rows of 64 M or N values, 128 bytes), so no operand is
 // ever transposed in memory.  A symmetric product (SYM) computes the tiles on or above the diagonal only
 // and its epilogue mirrors them.
 //
-// What bounds it: 48 KB a stage of 32 K indices against 768 clocks of products at BN = 256, as many bytes a
-// clock as an SM takes from L2 at best (64, measured with boxes of 16 KB); narrower tiles ask for more.
+// Pairs (CTAS = 2): two SMs work on a tile of 256 rows, each loading 128 rows of A and half of B's columns, and
+// the even one's warp 1 issues the products of both (cta_group::2).  A stage of 32 K indices of a tile 256 wide
+// takes 768 clocks of products; one SM alone would load 48 KB in them, as many bytes a clock as it takes from L2
+// at best (64, measured with boxes of 16 KB), one of a pair 32 KB: 16384 x 1024 x 131072 with exponentials 10.9
+// ms alone, 9.2 in pairs.  A K step of 16 takes 290 to 305 ns then, 1.5 to 1.6 PFLOP/s of products.  128 wide a
+// pair is as fast as two SMs (166 to 200 ns a step), but draws less power: 4095 x 256 x 8192 forward and backward,
+// run for seconds, 269 us alone and 256 in pairs.  Full barriers are the even CTA's and count both CTAs' bytes,
+// empty and accumulator ones are each CTA's own, and both leave together.
 //
 // Work: where there are as many tiles as SMs or more, they go whole to the CTAs in turn, in grouped raster
 // order (full = tiles).  Fewer ones may be divided (full = 0): they are one line of units of `quantum` chunks,
@@ -109,14 +115,15 @@ __device__ __forceinline__ int scale_exponent(float m) {
 
 constexpr int HG_M = 128, HG_K = 32;
 constexpr u32 HG_THREADS = 384;
-template <int BN> struct F16x3 {
-  static constexpr int CTAS = BN == 256 ? 2 : 1, TM = CTAS * HG_M, COLS = BN / CTAS;   // tile rows; columns of B a CTA loads
+constexpr int f16_accs(int bn) { return bn == 256 ? 1 : bn == 128 ? 2 : 3; }   // accumulators of a TMEM buffer
+template <int BN, int CTAS> struct F16x3 {
+  static constexpr int TM = CTAS * HG_M, COLS = BN / CTAS;   // tile rows; columns of B a CTA loads
   static constexpr u32 A_BYTES = HG_M * HG_K * 2, B_BYTES = COLS * HG_K * 2;
   static constexpr u32 STAGE = 2 * A_BYTES + 2 * B_BYTES;
   static constexpr u32 BARS = 256, VECTORS = 8 * 128, STAGING = 8 * 4096;   // 128 bytes, a 4 KB block an epilogue warp
   static constexpr u32 FIT = (227 * 1024 - 1024 - BARS - VECTORS - STAGING) / STAGE;   // 1 KB to align the ring
   static constexpr u32 STAGES = FIT > 8 ? 8 : FIT;
-  static constexpr u32 ACCS = BN == 256 ? 1 : BN == 128 ? 2 : 3;     // accumulators of a TMEM buffer
+  static constexpr u32 ACCS = f16_accs(BN);
   static constexpr u32 TMEM = 512;                                   // columns allocated: 2 ACCS BN, a power of 2
 };
 
@@ -191,7 +198,7 @@ struct F16Tile { int m0, n0, bz; };
 
 // Tile u.  Grouped raster (8 tile rows per group) so the CTAs running together share operand panels in L2;
 // a symmetric product walks the tiles that reach the diagonal, row by row.
-template <int BN, bool SYM>
+template <int BN, int CTAS, bool SYM>
 __device__ __forceinline__ F16Tile f16_tile(u32 u, u32 tm, u32 tn, u32 per) {
   F16Tile T;
   T.bz = (int)(u / per);
@@ -199,7 +206,7 @@ __device__ __forceinline__ F16Tile f16_tile(u32 u, u32 tm, u32 tn, u32 per) {
   if (SYM) {
     u32 i = 0;
     for (;; ++i) {
-      const u32 first = i * F16x3<BN>::TM / BN, n = tn - first;
+      const u32 first = i * CTAS * HG_M / BN, n = tn - first;
       if (r < n) { nt = first + r; break; }
       r -= n;
     }
@@ -211,15 +218,15 @@ __device__ __forceinline__ F16Tile f16_tile(u32 u, u32 tm, u32 tn, u32 per) {
     mt = first + w % gsz;
     nt = w / gsz;
   }
-  T.m0 = (int)(mt * F16x3<BN>::TM);
+  T.m0 = (int)(mt * CTAS * HG_M);
   T.n0 = (int)(nt * BN);
   return T;
 }
-template <int BN, bool SYM>
+template <int BN, int CTAS, bool SYM>
 __device__ __forceinline__ u32 f16_tiles(u32 tm, u32 tn) {
   if (!SYM) return tm * tn;
   u32 n = 0;
-  for (u32 i = 0; i < tm; ++i) n += tn - i * F16x3<BN>::TM / BN;
+  for (u32 i = 0; i < tm; ++i) n += tn - i * CTAS * HG_M / BN;
   return n;
 }
 
@@ -273,7 +280,7 @@ struct F16Epi {
 template <int BN, int I, int NB>
 __device__ __forceinline__ void f16_collect(float (&v)[NB][32], u32 t) {
   if constexpr (I < NB) {
-    constexpr int ACCS = (int)F16x3<BN>::ACCS;
+    constexpr int ACCS = f16_accs(BN);
     float w[32];
     if constexpr (ACCS > 1) {   // the mixed terms, 2^-11 of the main ones, first
       tmem_ld32(t + BN + 32 * I, w);
@@ -340,9 +347,9 @@ __device__ __forceinline__ F16Job f16_job(const GemmParams& P) {
           reinterpret_cast<float*>(P.a.scratch + (u64)P.a.p[3]), reinterpret_cast<u32*>(P.a.p[15]) + 4};
 }
 
-template <int BN, bool A_MN, bool B_MN, bool SYM, bool BLOCKED, int CHUNK, class EPI>
+template <int BN, int CTAS, bool A_MN, bool B_MN, bool SYM, bool BLOCKED, int CHUNK, class EPI>
 __device__ __forceinline__ void gemm_f16x3(const F16Job& J, u32* err, EPI& epi) {
-  using S = F16x3<BN>;
+  using S = F16x3<BN, CTAS>;
   constexpr u32 STAGES = S::STAGES;
   extern __shared__ unsigned char smem_raw[];
   const u32 raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
@@ -355,11 +362,11 @@ __device__ __forceinline__ void gemm_f16x3(const F16Job& J, u32* err, EPI& epi) 
   auto accf = [&](u32 b) { return bars + 8u * (2 * STAGES + b); };
   auto acce = [&](u32 b) { return bars + 8u * (2 * STAGES + 2 + b); };
   const u32 M = J.M, N = J.N;
-  constexpr u32 CTAS = S::CTAS, TM = S::TM;
-  const u32 rank = CTAS == 2 ? pair_rank() : 0, unit = J.block / CTAS;
+  constexpr u32 TM = S::TM;
+  const u32 rank = CTAS == 2 ? pair_rank() : 0, unit = J.block / CTAS;   // a CTA, or a pair
   const u32 tm = (M + TM - 1) / TM, tn = (N + BN - 1) / BN, kbs = (J.K + HG_K - 1) / HG_K;
   constexpr u32 CK = CHUNK / HG_K;   // stages of a chunk
-  const u32 per = f16_tiles<BN, SYM>(tm, tn);
+  const u32 per = f16_tiles<BN, CTAS, SYM>(tm, tn);
   F16Work work(per * J.batch, J.full, (kbs + CK - 1) / CK, J.quantum, unit, J.grid / CTAS);
 
   if (threadIdx.x == 32 * 3) {
@@ -400,7 +407,7 @@ __device__ __forceinline__ void gemm_f16x3(const F16Job& J, u32* err, EPI& epi) 
       u32 it = 0, s = 0, phase = 0;
       bool ok = true;
       while (ok && work.next()) {
-        const F16Tile T = f16_tile<BN, SYM>(work.tile, tm, tn, per);
+        const F16Tile T = f16_tile<BN, CTAS, SYM>(work.tile, tm, tn, per);
         const u32 kend = work.c1 * CK < kbs ? work.c1 * CK : kbs;
         for (u32 kb = work.c0 * CK; kb < kend; ++kb, ++it) {
           if (it >= STAGES && !wait(empty(s), phase ^ 1, 1)) { ok = false; break; }
@@ -500,7 +507,7 @@ __device__ __forceinline__ void gemm_f16x3(const F16Job& J, u32* err, EPI& epi) 
     u32 j = 0;
     bool ok = true;
     while (ok && work.next()) {
-      e.T = f16_tile<BN, SYM>(work.tile, tm, tn, per);
+      e.T = f16_tile<BN, CTAS, SYM>(work.tile, tm, tn, per);
       e.T.m0 += (int)rank * HG_M;
       e.row = (u64)e.T.m0 + 32 * e.q + lane;
       epi.begin(e);   // its loads are on their way while the products run
@@ -566,10 +573,11 @@ __device__ __forceinline__ void gemm_f16x3(const F16Job& J, u32* err, EPI& epi) 
   }
 }
 
-// a kernel's cluster by tile width
-#define TCB_F16_CLUSTER_256 __cluster_dims__(2, 1, 1)
-#define TCB_F16_CLUSTER_128
-#define TCB_F16_CLUSTER_64
+// a kernel's cluster by its CTAs a tile
+#define TCB_F16_CLUSTER_1
+#define TCB_F16_CLUSTER_2 __cluster_dims__(2, 1, 1)
+// X(suffix of the names, BN, CTAS) for every tile
+#define TCB_F16_TILES(X) X(256x2, 256, 2) X(128x2, 128, 2) X(128, 128, 1) X(64, 64, 1)
 
 // ---- what the operators share ----
 

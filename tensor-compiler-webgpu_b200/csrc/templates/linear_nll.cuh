@@ -473,22 +473,20 @@ struct NllOut {
 
 }  // namespace tcb
 
-#define TCB_NLL_GEMM(NAME, BN, AMN, BMN, EPI, ...)                                                                          \
-  extern "C" __global__ void TCB_F16_CLUSTER_##BN                                                                         \
-      __launch_bounds__(tcb::HG_THREADS, 1) NAME##_##BN(const __grid_constant__ tcb::GemmParams P) {                        \
-    tcb::EPI epi(__VA_ARGS__);                                                                                              \
-    tcb::gemm_f16x3<BN, AMN, BMN, false, true, 256>(tcb::f16_job(P), reinterpret_cast<u32*>(P.a.p[15]), epi);               \
+#define TCB_NLL_GEMM(NAME, TILE, BN, CTAS, AMN, BMN, EPI, ...)                                                      \
+  extern "C" __global__ void TCB_F16_CLUSTER_##CTAS __launch_bounds__(tcb::HG_THREADS, 1)                           \
+      NAME##_##TILE(const __grid_constant__ tcb::GemmParams P) {                                                    \
+    tcb::EPI epi(__VA_ARGS__);                                                                                      \
+    tcb::gemm_f16x3<BN, CTAS, AMN, BMN, false, true, 256>(tcb::f16_job(P), reinterpret_cast<u32*>(P.a.p[15]), epi); \
   }
 // logits and dz: h K-major, W MN-major (its rows run along the vocabulary); dh: dz and W K-major (along the
 // vocabulary); dW: h^T and dz, both MN-major (along d and along the vocabulary)
-#define TCB_NLL_GEMMS(BN)                                                   \
-  TCB_NLL_GEMM(tcb_nll_logits, BN, false, true, NllForward<BN>, P.a)        \
-  TCB_NLL_GEMM(tcb_nll_dz, BN, false, true, NllDz, P)                       \
-  TCB_NLL_GEMM(tcb_nll_dh, BN, false, false, NllOut<false>, P.a, P.a.out)   \
-  TCB_NLL_GEMM(tcb_nll_dw, BN, true, true, NllOut<true>, P.a, P.a.out)
-TCB_NLL_GEMMS(256)
-TCB_NLL_GEMMS(128)
-TCB_NLL_GEMMS(64)
+#define TCB_NLL_GEMMS(TILE, BN, CTAS)                                                 \
+  TCB_NLL_GEMM(tcb_nll_logits, TILE, BN, CTAS, false, true, NllForward<BN>, P.a)      \
+  TCB_NLL_GEMM(tcb_nll_dz, TILE, BN, CTAS, false, true, NllDz, P)                     \
+  TCB_NLL_GEMM(tcb_nll_dh, TILE, BN, CTAS, false, false, NllOut<false>, P.a, P.a.out) \
+  TCB_NLL_GEMM(tcb_nll_dw, TILE, BN, CTAS, true, true, NllOut<true>, P.a, P.a.out)
+TCB_F16_TILES(TCB_NLL_GEMMS)
 
 // dh and dW in one launch where their CTAs find room side by side: the first p[14] CTAs are dh's, maps 2 and 3,
 // p[7] (plan), p[8] (partial sums) and p[9] (address) dW's.
@@ -501,13 +499,13 @@ __device__ __forceinline__ void nll_both(const tcb::GemmParams& P) {
   if (blockIdx.x < (u32)a.p[14]) {
     j.grid = (u32)a.p[14];
     NllOut<false> epi(a, a.out);
-    gemm_f16x3<BH, false, false, false, true, 256>(j, err, epi);
+    gemm_f16x3<BH, 1, false, false, false, true, 256>(j, err, epi);
   } else {
     j = F16Job{&P.maps[2], &P.maps[3], (u32)a.p[5], j.K, j.M, 1, (u32)a.p[7], (u32)((u64)a.p[7] >> 32),
                blockIdx.x - (u32)a.p[14], gridDim.x - (u32)a.p[14], reinterpret_cast<float*>(a.scratch + (u64)a.p[8]),
                j.counters + 8 * 148};
     NllOut<true> epi(a, (u64)a.p[9]);
-    gemm_f16x3<BW, true, true, false, true, 256>(j, err, epi);
+    gemm_f16x3<BW, 1, true, true, false, true, 256>(j, err, epi);
   }
 }
 #define TCB_NLL_BOTH(BH, BW)                                                                                          \

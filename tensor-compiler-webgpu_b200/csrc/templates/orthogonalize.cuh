@@ -137,7 +137,7 @@ namespace tcb {
 
 // S, or P = b S + c S S: written where computed and, when the tile across the diagonal is not computed,
 // mirrored there.
-template <int BN, bool POLY>
+template <int BN, int CTAS, bool POLY>
 struct NsSymmetric {
   const Args& a;
   const TmaDesc* map;
@@ -162,7 +162,7 @@ struct NsSymmetric {
     }
     store_split32(e, map, v, (int)col, e.T.m0 + 32 * e.q, e.T.bz);
     const u32 row0 = (u32)e.T.m0 + 32 * e.q;
-    if (row0 / BN < col / F16x3<BN>::TM * F16x3<BN>::TM / BN) {   // the mirror's tile is not computed
+    if (row0 / BN < col / (CTAS * HG_M) * (CTAS * HG_M) / BN) {   // the mirror's tile is not computed
       if (e.lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
       turn32(e, v);   // lane l: row l of the mirrored block
       store_split32(e, map, v, (int)row0, (int)col, e.T.bz);
@@ -212,21 +212,19 @@ struct NsApply {
 
 }  // namespace tcb
 
-#define TCB_NS_GEMM(NAME, BN, AMN, BMN, SYM, EPI)                                                                         \
-  extern "C" __global__ void TCB_F16_CLUSTER_##BN                                                                         \
-      __launch_bounds__(tcb::HG_THREADS, 1) NAME##_##BN(const __grid_constant__ tcb::GemmParams P) {                      \
-    tcb::EPI epi(P);                                                                                                      \
-    tcb::gemm_f16x3<BN, AMN, BMN, SYM, false, 128>(tcb::f16_job(P), reinterpret_cast<u32*>(P.a.p[15]), epi);              \
+#define TCB_NS_GEMM(NAME, TILE, BN, CTAS, AMN, BMN, SYM, EPI)                                                       \
+  extern "C" __global__ void TCB_F16_CLUSTER_##CTAS __launch_bounds__(tcb::HG_THREADS, 1)                           \
+      NAME##_##TILE(const __grid_constant__ tcb::GemmParams P) {                                                    \
+    tcb::EPI epi(P);                                                                                                \
+    tcb::gemm_f16x3<BN, CTAS, AMN, BMN, SYM, false, 128>(tcb::f16_job(P), reinterpret_cast<u32*>(P.a.p[15]), epi);  \
   }
-#define TCB_NS_S(BN) NsSymmetric<BN, false>
-#define TCB_NS_P(BN) NsSymmetric<BN, true>
+#define TCB_NS_S(BN, CTAS) NsSymmetric<BN, CTAS, false>
+#define TCB_NS_P(BN, CTAS) NsSymmetric<BN, CTAS, true>
 // wide: X X^T (both along n), P X (X along n); tall: X^T X, X P (P = P^T); S S (S = S^T)
-#define TCB_NS_GEMMS(BN)                                                     \
-  TCB_NS_GEMM(tcb_orth_gram_wide, BN, false, false, true, TCB_NS_S(BN))      \
-  TCB_NS_GEMM(tcb_orth_gram_tall, BN, true, true, true, TCB_NS_S(BN))        \
-  TCB_NS_GEMM(tcb_orth_poly, BN, false, false, true, TCB_NS_P(BN))           \
-  TCB_NS_GEMM(tcb_orth_apply_wide, BN, false, true, false, NsApply)          \
-  TCB_NS_GEMM(tcb_orth_apply_tall, BN, false, false, false, NsApply)
-TCB_NS_GEMMS(256)
-TCB_NS_GEMMS(128)
-TCB_NS_GEMMS(64)
+#define TCB_NS_GEMMS(TILE, BN, CTAS)                                                              \
+  TCB_NS_GEMM(tcb_orth_gram_wide, TILE, BN, CTAS, false, false, true, TCB_NS_S(BN, CTAS))         \
+  TCB_NS_GEMM(tcb_orth_gram_tall, TILE, BN, CTAS, true, true, true, TCB_NS_S(BN, CTAS))           \
+  TCB_NS_GEMM(tcb_orth_poly, TILE, BN, CTAS, false, false, true, TCB_NS_P(BN, CTAS))              \
+  TCB_NS_GEMM(tcb_orth_apply_wide, TILE, BN, CTAS, false, true, false, NsApply)                   \
+  TCB_NS_GEMM(tcb_orth_apply_tall, TILE, BN, CTAS, false, false, false, NsApply)
+TCB_F16_TILES(TCB_NS_GEMMS)

@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import math
 import struct
+from collections import namedtuple
 
 from .ir import TRAINING_OPS, linear_nll_saved, newton_schulz_scales, size
 
@@ -31,35 +32,43 @@ def _up(n, k):
     return -(-n // k) * k
 
 
-def f16_ctas(bn):
-    """CTAs of a tile: a pair of SMs works on 256 x 256, each loading 128 rows of A and 128 columns of B."""
-    return 2 if bn == 256 else 1
+class Tile(namedtuple("Tile", "bn ctas")):
+    """A product's tile: ctas * 128 rows x bn columns.  A pair of SMs loads 128 rows of A and half of B's columns
+    each."""
+    def __str__(self):
+        return f"{self.bn}x2" if self.ctas == 2 else str(self.bn)
+
+    @property
+    def cols(self):
+        """Columns of B a CTA loads."""
+        return self.bn // self.ctas
 
 
-def _f16_stages(bn):
-    stage = 2 * F16_BM * F16_BK * 2 + 2 * (bn // f16_ctas(bn)) * F16_BK * 2
+def _f16_stages(tile):
+    stage = 2 * F16_BM * F16_BK * 2 + 2 * tile.cols * F16_BK * 2
     return min(8, (227 * 1024 - F16_EXTRA) // stage), stage
 
 
-def f16_smem(bn):
+def f16_smem(tile):
     """Bytes of shared memory (tcb/gemm_f16x3.cuh)."""
-    stages, stage = _f16_stages(bn)
+    stages, stage = _f16_stages(tile)
     return stages * stage + F16_EXTRA
 
 
-def f16_tiles(M, N, bn, symmetric):
-    rows = F16_BM * f16_ctas(bn)
-    tm, tn = math.ceil(M / rows), math.ceil(N / bn)
-    return sum(tn - i * rows // bn for i in range(tm)) if symmetric else tm * tn
+def f16_tiles(M, N, tile, symmetric):
+    rows = F16_BM * tile.ctas
+    tm, tn = math.ceil(M / rows), math.ceil(N / tile.bn)
+    return sum(tn - i * rows // tile.bn for i in range(tm)) if symmetric else tm * tn
 
 
-# Nanoseconds of a split-fp16 product by tile width, as measured with every SM busy: a K step of 16 of one tile;
-# an epilogue; the exchange of a divided tile's partial sums, at all and for each part.
-F16_COST = {256: (290, 6000, 3000, 2500), 128: (180, 3000, 1500, 1200), 64: (140, 1500, 1000, 700)}
+# Nanoseconds of a split-fp16 product by tile, as measured with every SM busy: a K step of 16 of one tile; an
+# epilogue; the exchange of a divided tile's partial sums, at all and for each part.
+F16_COST = {Tile(256, 2): (275, 6600, 3000, 2500), Tile(128, 2): (173, 3600, 1500, 1600),
+            Tile(128, 1): (180, 3000, 1500, 1200), Tile(64, 1): (140, 1500, 1000, 700)}
 
 
 def f16_plan(M, N, K, batch, chunk, symmetric=False):
-    """(tile width, grid, whole tiles, quantum) of a product (tcb/gemm_f16x3.cuh), the cheapest by F16_COST.
+    """(tile, grid, whole tiles, quantum) of a product (tcb/gemm_f16x3.cuh), the cheapest by F16_COST.
 
     Tiles go whole to the SMs in waves, or, where they are fewer than the SMs, in pieces of `quantum` chains
     of `chunk` K indices.  Dividing the last wave of more tiles than that does not pay: the CTAs then no
@@ -67,13 +76,13 @@ def f16_plan(M, N, K, batch, chunk, symmetric=False):
     whole, 216 divided)."""
     best = None
     steps = math.ceil(K / 16)
-    for bn, (step, epi, once, part) in F16_COST.items():
-        ctas = f16_ctas(bn)
+    for tile, (step, epi, once, part) in F16_COST.items():
+        bn, ctas = tile
         units = SM_COUNT // ctas
         if (bn > 64 and N <= bn // 2) or M <= F16_BM * (ctas - 1):
             continue
-        tiles = batch * f16_tiles(M, N, bn, symmetric)
-        plans = [(math.ceil(tiles / units) * (steps * step + epi), bn, min(units, tiles) * ctas, tiles, 1)]
+        tiles = batch * f16_tiles(M, N, tile, symmetric)
+        plans = [(math.ceil(tiles / units) * (steps * step + epi), tile, min(units, tiles) * ctas, tiles, 1)]
         for q in (1, 2, 4, 8, 16, 32, 64):
             per = math.ceil(K / (256 * q))
             if tiles >= units or per == 1:
@@ -81,21 +90,21 @@ def f16_plan(M, N, K, batch, chunk, symmetric=False):
             grid = min(units, tiles * per)
             run = math.ceil(tiles * per / grid)
             pieces = per if run == 1 else per // run + 2
-            plans.append((run * q * 16 * step + once + pieces * part + epi, bn, grid * ctas, 0, q * (256 // chunk)))
+            plans.append((run * q * 16 * step + once + pieces * part + epi, tile, grid * ctas, 0, q * (256 // chunk)))
         for p in plans:
             if best is None or p[0] < best[0]:
                 best = p
     return best[1:]
 
 
-def f16_partial_bytes(grid, whole, tiles, bn):
-    return 0 if whole == tiles else 2 * grid * F16_BM * bn * 4
+def f16_partial_bytes(grid, whole, tiles, tile):
+    return 0 if whole == tiles else 2 * grid * F16_BM * tile.bn * 4
 
 
-def _operand(off, plane, cols, rows, batch, pitch, mn, bn, region="scratch"):
+def _operand(off, plane, cols, rows, batch, pitch, mn, box_rows, region="scratch"):
     """The map of an operand's hi and lo planes, one behind the other for each matrix: boxes of 64 x F16_BK when
-    its M or N index runs along the rows, else of F16_BK x (128 or the tile width)."""
-    box = (64 | F16 | PAIR, F16_BK) if mn else (F16_BK | F16 | PAIR, bn // f16_ctas(bn))
+    its M or N index runs along the rows, else of F16_BK x the rows of A or columns of B that a CTA loads."""
+    box = (64 | F16 | PAIR, F16_BK) if mn else (F16_BK | F16 | PAIR, box_rows)
     assert plane == batch * rows * pitch * 2
     return [(region, off, cols, rows, 2 * batch, pitch * 2, rows * pitch * 2, *box)]
 
@@ -110,8 +119,8 @@ def _pitch(cols):
     return min(256, _up(cols, 32))
 
 
-def _blocked_operand(region, off, rows, cols, pitch, mn, bn):
-    return _blocked(region, off, rows, cols, pitch, *((64, F16_BK) if mn else (F16_BK, bn // f16_ctas(bn))))
+def _blocked_operand(region, off, rows, cols, pitch, mn, box_rows):
+    return _blocked(region, off, rows, cols, pitch, *((64, F16_BK) if mn else (F16_BK, box_rows)))
 
 
 def _at(index, off):
@@ -121,14 +130,14 @@ def _at(index, off):
 
 def _gemm(name, M, N, K, batch, plan, part_at, maps, params, symmetric=False):
     from .codegen import KernelCall
-    bn, grid, whole, quantum = plan
-    tiles = batch * f16_tiles(M, N, bn, symmetric)
+    tile, grid, whole, quantum = plan
+    tiles = batch * f16_tiles(M, N, tile, symmetric)
     if tiles >= 1 << 31:
         raise ValueError(f"{name}: {tiles} tiles")
-    c = KernelCall(f"{name}_{bn}", (grid, 1, 1), (384, 1, 1), f16_smem(bn),
+    c = KernelCall(f"{name}_{tile}", (grid, 1, 1), (384, 1, 1), f16_smem(tile),
                    [M | N << 32, K | batch << 32, whole | quantum << 32, part_at, *params])
     c.tma = maps
-    return c, f16_partial_bytes(grid, whole, tiles, bn)
+    return c, f16_partial_bytes(grid, whole, tiles, tile)
 
 
 def siblings(graph):
@@ -198,8 +207,8 @@ def _nll_launch(graph, ids):
     (R, d), V = graph.nodes[node.inputs[0]].shape, graph.nodes[node.inputs[1]].shape[1]
     inner, floats = linear_nll_saved(R, d, V)
     plan = f16_plan(R, V, d, 1, NLL_CHUNK)
-    bn = plan[0]
-    halves = math.ceil(V / (bn // 2))
+    tile = plan[0]
+    halves = math.ceil(V / (tile.bn // 2))
     at, end = _regions(("amax", 8 * AMAX_BLOCKS), ("err", NLL_CTRL_BYTES), ("zt", 4 * R), ("part", 8 * R * halves),
                        ("loss", 0 if "loss" in by else 4 * R), ("saved", 0 if "saved" in by else 4 * floats))
     joined = _joined(math.ceil(R / 32), halves)
@@ -212,7 +221,7 @@ def _nll_launch(graph, ids):
         def saved(off):
             return "scratch", at["saved"] + off
     maps = (_blocked_operand(*saved(inner["h"]), R, d, _pitch(d), False, F16_BM) +
-            _blocked_operand(*saved(inner["w"]), d, V, _pitch(V), True, bn))
+            _blocked_operand(*saved(inner["w"]), d, V, _pitch(V), True, tile.cols))
     blocks = max(1, min(AMAX_BLOCKS, math.ceil((R * d + d * V) / 2048)))
     units = d * math.ceil(V / 1024) + R * math.ceil(d / 1024)
     gemm, partial = _gemm("tcb_nll_logits", R, V, d, 1, plan, end, maps, tail)
@@ -229,7 +238,7 @@ def _nll_launch(graph, ids):
                 c.out_node = by["saved"]
     return Launch(node.id, node.op, "linear-nll", None, node.inputs, nll_source(node.attrs["bias"]), calls,
                   scratch_bytes=end + _up(partial, 256),
-                  info={"rnv": (R, d, V), "bn": bn, "ctrl_bytes": _up(NLL_CTRL_BYTES, 64), "path": "tcgen05-f16x3"})
+                  info={"rnv": (R, d, V), "tile": str(tile), "ctrl_bytes": _up(NLL_CTRL_BYTES, 64), "path": "tcgen05-f16x3"})
 
 
 def _nll_grad_launch(graph, ids):
@@ -248,7 +257,7 @@ def _nll_grad_launch(graph, ids):
     def add(name, wrt, M, N, K, maps, params):
         nonlocal partial
         plan = f16_plan(M, N, K, 1, NLL_CHUNK)
-        c, nbytes = _gemm(name, M, N, K, 1, plan, end, maps(plan[0]), params)
+        c, nbytes = _gemm(name, M, N, K, 1, plan, end, maps(plan[0].cols), params)
         c.err_offset = at["err"]
         if wrt is not None and want[wrt] != node.id:
             c.out_node = want[wrt]
@@ -263,19 +272,19 @@ def _nll_grad_launch(graph, ids):
         def h(mn):
             return _blocked_operand("in_at", _at(1, inner["h"]), R, d, _pitch(d), mn, F16_BM)
 
-        def w(mn, bn):
-            return _blocked_operand("in_at", _at(1, w_at), d, n, _pitch(V), mn, bn)
+        def w(mn, box_rows):
+            return _blocked_operand("in_at", _at(1, w_at), d, n, _pitch(V), mn, box_rows)
 
-        def z(mn, bn):
-            return _blocked_operand("scratch", at["dz"], R, n, _pitch(n), mn, bn)
+        def z(mn, box_rows):
+            return _blocked_operand("scratch", at["dz"], R, n, _pitch(n), mn, box_rows)
         out = _blocked("scratch", at["dz"], R, n, _pitch(n), 32, 32)
-        add("tcb_nll_dz", None, R, n, d, lambda bn: h(False) + w(True, bn) + out, params)
+        add("tcb_nll_dz", None, R, n, d, lambda cols: h(False) + w(True, cols) + out, params)
         if joined:
             calls[-1].ptr_params = ((14, want["b"]),)
         ph, pw = f16_plan(R, d, n, 1, NLL_CHUNK), f16_plan(d, n, R, 1, NLL_CHUNK)
-        if "h" in want and "w" in want and max(ph[0], pw[0]) <= 128 and ph[1] + pw[1] <= SM_COUNT:
+        if "h" in want and "w" in want and ph[0].ctas == pw[0].ctas == 1 and ph[1] + pw[1] <= SM_COUNT:
             # both find room side by side
-            c, hb = _gemm("tcb_nll_both", R, d, n, 1, ph, end, z(False, F16_BM) + w(False, ph[0]) + h(True) + z(True, pw[0]), params)
+            c, hb = _gemm("tcb_nll_both", R, d, n, 1, ph, end, z(False, F16_BM) + w(False, ph[0].cols) + h(True) + z(True, pw[0].cols), params)
             wb = f16_partial_bytes(pw[1], pw[2], f16_tiles(d, n, pw[0], False), pw[0])
             c.name = f"tcb_nll_both_{ph[0]}_{pw[0]}"
             c.grid, c.smem = (ph[1] + pw[1], 1, 1), max(f16_smem(ph[0]), f16_smem(pw[0]))
@@ -289,9 +298,9 @@ def _nll_grad_launch(graph, ids):
             calls.append(c)
             continue
         if "h" in want:
-            add("tcb_nll_dh", "h", R, d, n, lambda bn: z(False, F16_BM) + w(False, bn), params)
+            add("tcb_nll_dh", "h", R, d, n, lambda cols: z(False, F16_BM) + w(False, cols), params)
         if "w" in want:
-            add("tcb_nll_dw", "w", d, n, R, lambda bn: h(True) + z(True, bn), params)
+            add("tcb_nll_dw", "w", d, n, R, lambda cols: h(True) + z(True, cols), params)
     if "b" in want and not joined:
         db = KernelCall("tcb_nll_db", (math.ceil(V / 32), 1, 1), (256, 1, 1), 0, [0, 0, 0, 0, *tail, 0, 0])
         if want["b"] != node.id:
@@ -428,23 +437,23 @@ def _orth_launch(graph, node):
                        [parts, 0, 0, 0, m, n, at["x0"]])
     calls, partial = [norm, split], 0
 
-    def x_map(off, mn, bn):
-        return _operand(off, xplane, n, m, batch, xp, mn, bn)
+    def x_map(off, mn, box_rows):
+        return _operand(off, xplane, n, m, batch, xp, mn, box_rows)
 
-    def s_map(off, bn):
-        return _operand(off, splane, s, s, batch, sp, False, bn)
+    def s_map(off, box_rows):
+        return _operand(off, splane, s, s, batch, sp, False, box_rows)
 
     def out(off, rows, cols, pitch):
         return [("scratch", off, cols, rows, 2 * batch, pitch * 2, rows * pitch * 2, 32 | F16 | PAIR, 32)]
     for k in range(a["steps"]):
         cur, nxt = (at["x0"], at["x1"]) if k % 2 == 0 else (at["x1"], at["x0"])
         params = [m, n, cur, nxt, at["s"], at["p"], int(k == a["steps"] - 1)]
-        ab = x_map(cur, False, F16_BM) + s_map(at["p"], app[0]) if tall else s_map(at["p"], F16_BM) + x_map(cur, True, app[0])
+        ab = x_map(cur, False, F16_BM) + s_map(at["p"], app[0].cols) if tall else s_map(at["p"], F16_BM) + x_map(cur, True, app[0].cols)
         for c, nbytes in (
                 _gemm("tcb_orth_gram_tall" if tall else "tcb_orth_gram_wide", s, s, max(m, n), batch, gram, end,
-                      x_map(cur, tall, F16_BM) + x_map(cur, tall, gram[0]) + out(at["s"], s, s, sp), params, True),
+                      x_map(cur, tall, F16_BM) + x_map(cur, tall, gram[0].cols) + out(at["s"], s, s, sp), params, True),
                 _gemm("tcb_orth_poly", s, s, s, batch, poly, end,
-                      s_map(at["s"], F16_BM) + s_map(at["s"], poly[0]) + out(at["p"], s, s, sp), params, True),
+                      s_map(at["s"], F16_BM) + s_map(at["s"], poly[0].cols) + out(at["p"], s, s, sp), params, True),
                 _gemm("tcb_orth_apply_tall" if tall else "tcb_orth_apply_wide", m, n, s, batch, app, end,
                       ab + out(nxt, m, n, xp), params)):
             c.err_offset = at["err"]
@@ -452,7 +461,7 @@ def _orth_launch(graph, node):
             partial = max(partial, nbytes)
     return Launch(node.id, node.op, "orthogonalize", None, node.inputs,
                   orth_source(a["steps"], a["coeffs"], a["eps"]), calls, scratch_bytes=end + _up(partial, 256),
-                  info={"mn": (batch, m, n), "bn": (gram[0], poly[0], app[0]), "ctrl_bytes": _up(CTRL_BYTES, 64), "path": "tcgen05-f16x3"})
+                  info={"mn": (batch, m, n), "tiles": (str(gram[0]), str(poly[0]), str(app[0])), "ctrl_bytes": _up(CTRL_BYTES, 64), "path": "tcgen05-f16x3"})
 
 
 def training_launch(graph, node, groups):

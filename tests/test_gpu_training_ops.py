@@ -341,11 +341,11 @@ def test_orthogonalize_stack_members_do_not_meet(pkg, mods, runner):
 
 
 @pytest.mark.parametrize("divide", [False, True])
-@pytest.mark.parametrize("bn", [64, 128, 256])
-def test_every_tile_width_whole_and_divided(pkg, mods, runner, monkeypatch, bn, divide):
-    """The products by each tile width alone, their tiles whole or divided along K, at sizes with ragged edges."""
+@pytest.mark.parametrize("bn,ctas", [(64, 1), (128, 1), (128, 2), (256, 2)])
+def test_every_tile_whole_and_divided(pkg, mods, runner, monkeypatch, bn, ctas, divide):
+    """The products by each tile alone, their tiles whole or divided along K, at sizes with ragged edges."""
     to = importlib.import_module(P + ".training_ops")
-    monkeypatch.setattr(to, "F16_COST", {bn: (100, 1000, 0, 0) if divide else (100, 1000, 10 ** 9, 0)})
+    monkeypatch.setattr(to, "F16_COST", {to.Tile(bn, ctas): (100, 1000, 0, 0) if divide else (100, 1000, 10 ** 9, 0)})
     for R, d, V in ((150, 140, 257), (300, 200, 700), (900, 513, 1300)):
         check_nll(mods, runner, nll_case(pkg, R, d, V, seed=R), runs=2)
     for shape in ((140, 150), (390, 130), (2, 257, 600), (2, 300, 520)):

@@ -258,18 +258,20 @@ def test_nll_maps_stay_inside(mods, R, d, V):
 @pytest.mark.parametrize("M,N,K,batch,chunk,sym", [(64, 50, 16384, 1, 256, False), (1, 1, 1, 1, 256, False), (57, 1365, 55301, 1, 256, False),
                                                    (256, 256, 1024, 4, 128, True), (1000, 1000, 4095, 1, 128, True),
                                                    (4095, 256, 8192, 1, 256, False), (8192, 1024, 4096, 1, 256, False),
+                                                   (1024, 512, 32000, 1, 256, False), (1300, 1300, 9000, 1, 128, True),
                                                    (18, 18, 3593, 14, 128, True), (300, 4099, 700, 1, 128, False),
                                                    (128, 2048, 12345, 1, 128, False)])
 def test_division_of_a_product(mods, M, N, K, batch, chunk, sym):
     """The device's division of tiles among CTAs, restated: every chunk of every tile once, the pieces of a
     divided tile found by the warp that adds them, no two in one slot."""
     pkg, cg, to, rt = mods
-    bn, grid, whole, q = to.f16_plan(M, N, K, batch, chunk, sym)
-    tiles = batch * to.f16_tiles(M, N, bn, sym)
+    tile, ctas, whole, q = to.f16_plan(M, N, K, batch, chunk, sym)
+    assert ctas % tile.ctas == 0 and 1 <= ctas <= 148 and M > 128 * (tile.ctas - 1)
+    tiles, grid = batch * to.f16_tiles(M, N, tile, sym), ctas // tile.ctas   # pairs work as one
     chunks = -(-K // chunk)
     per = -(-chunks // q)
     total = (tiles - whole) * per
-    assert 1 <= grid <= 148 and (total == 0 or grid <= total) and tiles - whole < 148 and (bn == 64 or N > bn // 2)
+    assert (total == 0 or grid <= total) and (tiles - whole) * tile.ctas <= 148 and (tile.bn == 64 or N > tile.bn // 2)
     seen, slots = {}, {}
     for c in range(grid):
         for t in range(c, whole, grid):
@@ -294,7 +296,7 @@ def test_division_of_a_product(mods, M, N, K, batch, chunk, sym):
             ca, cb = (((x + 1) * grid - 1) // total for x in (first, first + per - 1))
             assert [p[2] for p in pieces] == list(range(ca, cb + 1))
             assert [slots[2 * c + (c == ca)][1] for c in range(ca, cb + 1)] == pieces
-    assert to.f16_partial_bytes(grid, whole, tiles, bn) >= (max(slots) + 1 if slots else 0) * 128 * bn * 4
+    assert to.f16_partial_bytes(ctas, whole, tiles, tile) >= (max(slots) + 1 if slots else 0) * 128 * tile.ctas * tile.bn * 4
 
 
 @pytest.mark.parametrize("shape", [[1, 1], [64, 64], [100, 70], [3, 70, 300], [4095, 1000], [2, 2, 256, 1024]])
