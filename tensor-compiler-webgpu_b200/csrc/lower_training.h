@@ -18,6 +18,7 @@ constexpr i64 AMAX_BLOCKS = 4 * SM_COUNT, DZ_BYTES = (i64)128 << 20;
 constexpr i64 CTRL_BYTES = 4 * (4 + 8 * 2 * SM_COUNT);
 constexpr i64 JOIN_COUNTERS = 512, JOIN_PARTS = 4, NLL_CTRL_BYTES = CTRL_BYTES + 4 * JOIN_COUNTERS;
 constexpr i64 NLL_CHUNK = 256, NS_CHUNK = 128, NS_PARTS = 512;
+constexpr i64 NLL_ROWS = 16;
 constexpr i64 NLL_ADD = 1, NLL_JOIN = 2, NLL_NO_LOSS = 4, NLL_DB = 8;
 constexpr double F16_ROOM = 60000.0;
 
@@ -319,11 +320,32 @@ static std::vector<i64> cat(std::vector<i64> a, const std::vector<i64>& b) {
   return a;
 }
 
+// A few rows' loss alone (tcb/nll_rows.cuh).
+static Launch nll_rows_launch(const Graph& g, const Node& node, i64 R, i64 d, i64 V) {
+  const i64 rows = R <= 4 ? 4 : R <= 8 ? 8 : 16, blocks = cdiv(V, 128);
+  i64 parts = std::min<i64>({8, std::max<i64>(1, 4 * SM_COUNT / blocks), cdiv(d, 64)});
+  const i64 per = cdiv(d, parts);
+  parts = cdiv(d, per);
+  Regions r;
+  r.add(parts > 1 ? 4 * parts * R * V : 0);
+  const i64 zt = r.add(4 * R), stats = r.add(8 * R * cdiv(V, 32));
+  const std::vector<i64> params = {parts, per, zt, stats, R, d, V};
+  std::vector<Call> calls = {make_call("tcb_nll_rows_" + std::to_string(rows), {blocks, parts, 1}, {256, 1, 1}, 0, params)};
+  if (parts > 1) calls.push_back(make_call("tcb_nll_rows_add", {cdiv(V, 256), R, 1}, {256, 1, 1}, 0, params));
+  calls.push_back(make_call("tcb_nll_rows_finish", {R, 1, 1}, {1024, 1, 1}, 0, params));
+  std::string code = nll_source(bool_attr(node, "bias"));
+  code.replace(code.find("linear_nll.cuh"), 14, "nll_rows.cuh");
+  Launch l = training_record(node, "linear-nll", code, std::move(calls), r.end);
+  l.info = {{"rnv", arr({num(R), num(d), num(V)})}, {"parts", num(parts)}, {"path", str("fma")}};
+  return l;
+}
+
 static Launch nll_launch(const Graph& g, const std::vector<int>& ids) {
   const Node& node = g.nodes[ids[0]];
   const i64 R = in_shape(g, node, 0)[0], d = in_shape(g, node, 0)[1], V = in_shape(g, node, 1)[1];
   int loss = -1, saved = -1;
   for (int i : ids) (word_attr(g.nodes[i], "out") == "loss" ? loss : saved) = i;
+  if (saved < 0 && R <= NLL_ROWS) return nll_rows_launch(g, node, R, d, V);
   const NllSaved in = nll_saved(R, d, V);
   const F16Plan plan = f16_plan(R, V, d, 1, NLL_CHUNK);
   const i64 halves = cdiv(V, plan.tile.bn / 2);

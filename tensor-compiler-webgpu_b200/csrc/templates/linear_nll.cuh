@@ -32,24 +32,13 @@
 // in[]: h, W, (b), t forward; t, saved, the loss's cotangent backward.
 #pragma once
 #include "tcb/gemm_f16x3.cuh"
-
-#ifndef TCB_BIAS
-#define TCB_BIAS 1
-#endif
+#include "tcb/nll_common.cuh"
 
 namespace tcb {
 
 // flags: add to dh; join in the product's kernel; no loss; db wanted
 constexpr u32 NLL_ADD = 1, NLL_JOIN = 2, NLL_NO_LOSS = 4, NLL_DB = 8;
 constexpr u32 NLL_CTRL = F16_CTRL + 512;   // words of the control block: a counter more for each 32 rows or columns joined
-constexpr float NLL_LOG2E = 1.44269504f, NLL_LN2 = 0.693147181f, NLL_MAX = 3.402823466e38f;
-#define TCB_MINUS_INF bits(0xff800000u)
-
-__device__ __forceinline__ float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
 
 // At the start of the saved value; b log2(e) follows at 256 bytes, -inf beyond V up to a multiple of 256.
 struct NllScales { float down_h, down_w, z2; };
@@ -64,8 +53,7 @@ template <bool BACK> struct Nll {
   __device__ __forceinline__ const float* w() const { return reinterpret_cast<const float*>(a.in[1]); }
   // the row's class, or -1 when it takes no part
   __device__ __forceinline__ int target(u64 row) const {
-    const float t = ld1(reinterpret_cast<const float*>(a.in[BACK ? 0 : TCB_BIAS ? 3 : 2]) + row);
-    return t >= 0.0f && t < (float)V() ? (int)t : -1;
+    return nll_class(ld1(reinterpret_cast<const float*>(a.in[BACK ? 0 : TCB_BIAS ? 3 : 2]) + row), V());
   }
   __device__ __forceinline__ float cotangent(u64 row) const { return ld1(reinterpret_cast<const float*>(a.in[2]) + row); }
   template <class X> __device__ __forceinline__ X* scratch(u64 off) const { return reinterpret_cast<X*>(a.scratch + off); }
@@ -198,10 +186,8 @@ extern "C" __global__ void __launch_bounds__(256) tcb_nll_split(const tcb::Args 
     *n.scales() = NllScales{pow2(-kh), pow2(-kw), fminf(pow2(-kh) * pow2(-kw) * NLL_LOG2E, NLL_MAX)};
   const u64 V = n.V(), padded = (V + 255) / 256 * 256;
   for (u64 v = (u64)blockIdx.x * 256 + threadIdx.x; v < padded; v += (u64)gridDim.x * 256) {
-    float b = TCB_BIAS && v < V ? ld1(reinterpret_cast<const float*>(a.in[2]) + v) : 0.0f;
-    // a mask of the lowest float stays finite
-    if (fabsf(b) <= NLL_MAX) b = fmaxf(fminf(b * NLL_LOG2E, NLL_MAX), -NLL_MAX);
-    n.bias2()[v] = v < V ? b : TCB_MINUS_INF;
+    const float b = TCB_BIAS && v < V ? ld1(reinterpret_cast<const float*>(a.in[2]) + v) : 0.0f;
+    n.bias2()[v] = v < V ? nll_bias2(b) : TCB_MINUS_INF;
   }
   // the last blocks take h, about its share of the values
   const u64 hv = n.R() * n.d(), wv = n.d() * V;
@@ -254,11 +240,6 @@ __device__ __forceinline__ bool nll_last(const Args& a, u32 counter, u32 n, int 
     __threadfence();
   }
   return last;
-}
-__device__ __forceinline__ void nll_join(float& m, float& s, const float2& x) {
-  const float mx = fmaxf(m, x.x), safe = mx == TCB_MINUS_INF ? 0.0f : mx;
-  s = s * ex2(m - safe) + x.y * ex2(x.x - safe);
-  m = mx;
 }
 // Half tiles k, k + step, ... of a row joined, eight loads in flight.
 __device__ __forceinline__ void nll_join_tiles(const float2* part, u64 R, u64 row, u32 k, u32 step, u32 tiles, float& m,

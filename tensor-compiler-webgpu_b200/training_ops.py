@@ -1,6 +1,6 @@
 """Launches of the operators of a decoder's training step (ir.TRAINING_OPS).
 
-* ``linearNll`` / ``linearNllGrad``       -- tcb/linear_nll.cuh
+* ``linearNll`` / ``linearNllGrad``       -- tcb/linear_nll.cuh; a few rows' loss alone tcb/nll_rows.cuh
 * ``headNormRope`` / ``headNormRopeGrad`` -- tcb/head_norm_rope.cuh
 * ``orthogonalize``                       -- tcb/orthogonalize.cuh, tcb/orth_small.cuh
 
@@ -183,12 +183,35 @@ def nll_pieces(R, V):
     return wide, math.ceil(V / wide)
 
 
-def nll_source(bias):
+def nll_source(bias, rows=False):
     return f"""// cross entropy of a linear head, {'bias' if bias else 'no bias'}
 #include "tcb/common.cuh"
 #define TCB_BIAS {int(bias)}
-#include "tcb/linear_nll.cuh"
+#include "tcb/{'nll_rows' if rows else 'linear_nll'}.cuh"
 """
+
+
+NLL_ROWS = 16    # most rows of a loss without a backward that are worth reading W as it is
+
+
+def _nll_rows_launch(graph, node):
+    """A few rows' loss alone (tcb/nll_rows.cuh)."""
+    from .codegen import KernelCall, Launch
+    (R, d), V = graph.nodes[node.inputs[0]].shape, graph.nodes[node.inputs[1]].shape[1]
+    rows = next(k for k in (4, 8, 16) if R <= k)
+    blocks = math.ceil(V / 128)
+    # parts of d: blocks for every SM four times, at least 64 indices a part
+    parts = min(8, max(1, 4 * SM_COUNT // blocks), math.ceil(d / 64))
+    per = math.ceil(d / parts)
+    parts = math.ceil(d / per)
+    at, end = _regions(("sums", 4 * parts * R * V if parts > 1 else 0), ("zt", 4 * R), ("stats", 8 * R * math.ceil(V / 32)))
+    params = [parts, per, at["zt"], at["stats"], R, d, V]
+    calls = [KernelCall(f"tcb_nll_rows_{rows}", (blocks, parts, 1), (256, 1, 1), 0, params)]
+    if parts > 1:
+        calls.append(KernelCall("tcb_nll_rows_add", (math.ceil(V / 256), R, 1), (256, 1, 1), 0, params))
+    calls.append(KernelCall("tcb_nll_rows_finish", (R, 1, 1), (1024, 1, 1), 0, params))
+    return Launch(node.id, node.op, "linear-nll", None, node.inputs, nll_source(node.attrs["bias"], rows=True), calls,
+                  scratch_bytes=end, info={"rnv": (R, d, V), "parts": parts, "path": "fma"})
 
 
 def _regions(*parts):
@@ -205,6 +228,8 @@ def _nll_launch(graph, ids):
     by = {graph.nodes[i].attrs["out"]: i for i in ids}
     node = graph.nodes[ids[0]]
     (R, d), V = graph.nodes[node.inputs[0]].shape, graph.nodes[node.inputs[1]].shape[1]
+    if "saved" not in by and R <= NLL_ROWS:
+        return _nll_rows_launch(graph, node)
     inner, floats = linear_nll_saved(R, d, V)
     plan = f16_plan(R, V, d, 1, NLL_CHUNK)
     tile = plan[0]

@@ -119,7 +119,7 @@ def training_sources():
     the usual head layouts and the default Newton-Schulz coefficients."""
     from . import training_ops as to
     from .ir import NEWTON_SCHULZ
-    codes = {to.nll_source(bias) for bias in (False, True)}
+    codes = {to.nll_source(bias, rows) for bias in (False, True) for rows in (False, True)}
     codes |= {to.orth_source(steps, NEWTON_SCHULZ, 1e-7, small) for steps in (1, 2, 5) for small in (None, *to.ORTH_SMALL)}
     for D in (16, 32, 48, 64, 80, 96, 128, 192, 256):
         codes |= {to.head_source(D, rot, pairs) for rot in (D, D // 2) for pairs in (False, True)}

@@ -340,6 +340,73 @@ def test_orthogonalize_stack_members_do_not_meet(pkg, mods, runner):
     assert np.array_equal(got[0], alone[0]) and np.array_equal(got[2], alone[2]) and np.isnan(got[1]).all()
 
 
+def nll_loss_case(pkg, R, d, V, bias=True, seed=0):
+    g = pkg.ir.Graph()
+    y = g.linear_nll(g.input("h", [R, d]), g.input("w", [d, V]), g.input("b", [V]) if bias else None, g.input("t", [R]))
+    rng = np.random.default_rng(seed)
+    x = {"h": f32(rng.standard_normal((R, d))), "w": f32(rng.standard_normal((d, V)) * 2 / np.sqrt(d)),
+         "t": rng.integers(0, V, R).astype(np.float64)}
+    if bias:
+        x["b"] = f32(rng.standard_normal(V) * 0.1)
+    return g, y, x
+
+
+def few_rows_bound(h, w, b, t):
+    """A few rows' loss on the CUDA cores: a term passes through at most d / 8 fused steps of a warp (an eighth and
+    one more of each 256 indices), 8 + 8 sums of warps and parts, one more of the bias, each off by half a step of
+    the sums so far.  Sums of exponentials: 4 terms of each of V / 4096 steps, 40 joins of two roundings,
+    exponentials of 2 steps."""
+    loss, _, ok = ref.nll(h, w, b, t)
+    (R, d), V = h.shape, w.shape[1]
+    z = np.abs(np.where(ok[:, None], h, 0.0)) @ np.abs(w) + (0.0 if b is None else np.abs(b))
+    top = (d / 8 + d / 256 + 20) * ref.U * z.max(1)
+    return loss, 2 * top + ref.U * (4 * (V / 4096 + 1) + 2 * (V / 4096 + 40) + 8) + 6 * ref.U * (np.abs(loss) + z.max(1))
+
+
+@pytest.mark.parametrize("R,d,V", [(1, 1, 1), (1, 64, 5000), (3, 70, 7), (4, 513, 4096), (5, 1000, 129), (8, 33, 128), (16, 257, 10001),
+                                   (15, 16, 3), (16, 2048, 1000), (7, 300, 5003), (17, 300, 5003), (33, 300, 5003)])
+@pytest.mark.parametrize("bias", [True, False])
+def test_nll_loss_of_a_few_rows(pkg, mods, runner, R, d, V, bias):
+    g, y, x = nll_loss_case(pkg, R, d, V, bias, seed=R)
+    a = (x["h"], x["w"], x.get("b"), x["t"])
+    loss, bound = few_rows_bound(*a)
+    if R > 16:   # more than the CUDA cores' form takes
+        bound = ref.nll_bounds(*a, np.zeros(R))[0]
+    within(run_graph(mods, runner, g, x, [y], runs=2)[0], loss, bound, "loss")
+
+
+def test_nll_loss_of_a_few_rows_masks(pkg, mods, runner):
+    """Padding rows with NaN in h, classes out of the vocabulary, a target among them."""
+    case = nll_loss_case(pkg, 6, 40, 700)
+    x = case[2]
+    x["b"][100:600], x["b"][650:] = -np.inf, -3.4028234663852886e38
+    x["t"][:] = [3, -1, 99, 700, 620, 200]
+    x["h"][1] = np.nan
+    got = run_graph(mods, runner, case[0], x, [case[1]])[0]
+    assert got[1] == 0 and got[3] == 0 and got[5] == np.inf
+    live = np.r_[0:100, 600:650]
+    keep = np.array([0, 2, 4])
+    within(got[keep], *few_rows_bound(x["h"][keep], x["w"][:, live], x["b"][live], np.array([3.0, 99.0, 120.0])), "loss")
+
+
+def test_nll_loss_of_a_few_rows_unaligned_weight(pkg, mods, runner):
+    """W where the caller has it, 4 bytes past a 128-bit boundary: the scalar loads."""
+    rt, cg = mods
+    g, y, x = nll_loss_case(pkg, 5, 65, 260)
+    ids = {n.attrs["name"]: n.id for n in g.inputs()}
+    buf = rt.DeviceBuffer(runner, 4 * 65 * 260 + 16)
+    prog = rt.Program(runner, g, cg.lower_fused(g, keep=[y]), keep=[y], place={ids["w"]: buf.ptr + 4})
+    try:
+        for name, i in ids.items():
+            prog.write(i, x[name])
+        prog.run()
+        got = prog.read(y).ravel()
+    finally:
+        prog.free()
+        buf.free()
+    within(got, *few_rows_bound(x["h"], x["w"], x["b"], x["t"]), "loss")
+
+
 @pytest.mark.parametrize("divide", [False, True])
 @pytest.mark.parametrize("bn,ctas", [(64, 1), (128, 1), (128, 2), (256, 2)])
 def test_every_tile_whole_and_divided(pkg, mods, runner, monkeypatch, bn, ctas, divide):
