@@ -189,8 +189,9 @@ extern "C" __global__ void __launch_bounds__(256) tcb_nll_split(const tcb::Args 
     const float b = TCB_BIAS && v < V ? ld1(reinterpret_cast<const float*>(a.in[2]) + v) : 0.0f;
     n.bias2()[v] = v < V ? nll_bias2(b) : TCB_MINUS_INF;
   }
-  // the last blocks take h, about its share of the values
-  const u64 hv = n.R() * n.d(), wv = n.d() * V;
+  // the last blocks take h, about its share of the pieces of rows (of the values, W's 600 rows of 3 fell to one
+  // block: 203 us)
+  const u64 hv = n.R() * ((n.d() + 1023) / 1024), wv = n.d() * ((V + 1023) / 1024);
   u64 hb = gridDim.x * hv / (hv + wv);
   hb = hb < 1 ? 1 : hb > gridDim.x - 1 ? gridDim.x - 1 : hb;
   const u64 wb = gridDim.x - hb;
@@ -322,6 +323,7 @@ struct NllForward {
 };
 
 // Backward epilogue: logits to dz, split for the products that read it; its column sums for db.
+template <int BN>
 struct NllDz {
   const Args& a;
   const TmaDesc* map;
@@ -381,6 +383,17 @@ struct NllDz {
       add2(v[j], v[j + 1], -lse, -lse);
       v[j] = ex2(v[j]);
       v[j + 1] = ex2(v[j + 1]);
+    }
+    if (BN == 64 && n.V() <= 32) {
+      // The whole row is here: made to add up to 1.  ex2 is low by 4e-8 of a row's sum on average, measured, which
+      // the sum of many rows keeps while their gradients of a few classes cancel (db of 4096 rows and 2 classes:
+      // 3.7e-6 off); with more classes each keeps less of it.
+      float s = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 32; ++j) s += v[j];
+      s = 1.0f - s;   // exact
+#pragma unroll
+      for (int j = 0; j < 32; j += 2) fma2(v[j], v[j + 1], s, s, v[j], v[j + 1]);
     }
     if (__any_sync(0xffffffffu, mine != 0u)) {   // in one block of 8 at 8192 classes
 #pragma unroll
@@ -464,7 +477,7 @@ struct NllOut {
 // vocabulary); dW: h^T and dz, both MN-major (along d and along the vocabulary)
 #define TCB_NLL_GEMMS(TILE, BN, CTAS)                                                 \
   TCB_NLL_GEMM(tcb_nll_logits, TILE, BN, CTAS, false, true, NllForward<BN>, P.a)      \
-  TCB_NLL_GEMM(tcb_nll_dz, TILE, BN, CTAS, false, true, NllDz, P)                     \
+  TCB_NLL_GEMM(tcb_nll_dz, TILE, BN, CTAS, false, true, NllDz<BN>, P)                 \
   TCB_NLL_GEMM(tcb_nll_dh, TILE, BN, CTAS, false, false, NllOut<false>, P.a, P.a.out) \
   TCB_NLL_GEMM(tcb_nll_dw, TILE, BN, CTAS, true, true, NllOut<true>, P.a, P.a.out)
 TCB_F16_TILES(TCB_NLL_GEMMS)

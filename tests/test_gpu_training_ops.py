@@ -174,6 +174,18 @@ def test_nll_pieces(pkg, mods, runner, monkeypatch):
     check_nll(mods, runner, nll_case(pkg, 200, 40, 900, seed=8))
 
 
+@pytest.mark.parametrize("V", [2, 5, 32])
+def test_nll_few_classes_add_up_to_one(pkg, mods, runner, V):
+    """A row's probabilities add up to 1, so its gradients of the logits to 0: what each row has left are a few
+    roundings of half a step (2^-25) that do not lean to one side.  Their mean over 8192 rows has a standard deviation
+    below 4 * 2^-25 / 90 = 1.3e-9; a lean of the exponential itself, 4e-8, would stand out."""
+    case = nll_case(pkg, 8192, 40, V, seed=V)
+    x = case[3]
+    x["d0"][:] = 1.0
+    out = run_graph(mods, runner, case[0], x, [case[1], *case[2].values()])
+    assert abs(out[3].astype(np.float64).sum()) / 8192 <= 1e-8
+
+
 def test_nll_is_deterministic_and_replays(pkg, mods, runner):
     case = nll_case(pkg, 700, 80, 3001, seed=9)
     keep = [case[1], *case[2].values()]
@@ -444,9 +456,13 @@ def small_graphs(pkg):
     yield graph, [y, *grads.values()], x
     graph, y, grads, x = nll_case(pkg, 700, 260, 3000, bias=False)
     yield graph, [y, *grads.values()], x
+    graph, y, grads, x = nll_case(pkg, 1500, 520, 2600)   # tiles of pairs of SMs
+    yield graph, [y, *grads.values()], x
+    graph, y, x = nll_loss_case(pkg, 6, 300, 5000)
+    yield graph, [y], x
     graph, y, grads, x = head_case(pkg, 2, 21, 3, 20, 20, True)
     yield graph, [y, *grads.values()], x
-    for shape in ([2, 70, 33], [3, 200, 300]):
+    for shape in ([2, 70, 33], [3, 200, 300], [520, 4000]):
         graph, y = orth_case(pkg, shape)
         yield graph, [y], {"x": f32(np.random.default_rng(1).standard_normal(shape))}
 
