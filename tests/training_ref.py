@@ -1,6 +1,6 @@
 """A float64 evaluation of whole graphs in numpy, with the training operators written from their formulas.
 
-The checker of the training-operator tests: nothing here shares code with the package.  Beside each
+The oracle of the training-operator tests: nothing here shares code with the package.  Beside each
 operator stands the bound of its float32 kernel's error, by counting roundings (U is half a float32 step).
 """
 import math
@@ -203,7 +203,7 @@ def evaluate(graph, inputs):
         elif op == "transpose":
             r = v[0].transpose(a["perm"])
         elif op == "linearNll":
-            # (opaque: the checker's gradients go back to the operands)
+            # (opaque: the oracle's gradients go back to the operands)
             r = np.zeros(n.shape) if a["out"] == "saved" else nll(v[0], v[1], v[2] if a["bias"] else None, v[-1])[0]
         elif op == "linearNllGrad":
             ops = [vals[i] for i in graph.nodes[n.inputs[1]].inputs]
