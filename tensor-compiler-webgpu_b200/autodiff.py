@@ -70,11 +70,16 @@ def _linear_nll_rule(G, n, gy, need):
 
 
 def _head_norm_rope_rule(G, n, gy, need):
+    if need[2]:
+        raise GradientError("headNormRope has no gradient with respect to its positions; wrap them in stopGradient "
+                            "where it is meant to be zero")
     return [G.emit("headNormRopeGrad", [*n.inputs, gy], {**n.attrs, "wrt": k}) if want else None
             for k, want in zip(("x", "gain"), need)] + [None]
 
 
-# Rules told which inputs' gradients are wanted: one launch computes all of a node's, and only those.
+# Rules told which inputs' gradients are wanted (an input from which a `wrt` node is reached without passing
+# one of these, whose gradient is zero): one launch computes all of a node's, and only those.
+ZERO_GRADIENT = ("step", "stopGradient")
 SELECTIVE = (_linear_nll_rule, _head_norm_rope_rule)
 
 RULES = {
@@ -126,6 +131,10 @@ def grad(graph, outputs, wrt, rules=None, prefix="d"):
         if any(depends[i] for i in node.inputs):
             depends[node.id] = True
 
+    wanted = [False] * forward_count
+    for node in graph.nodes:
+        wanted[node.id] = node.id in wrt or (node.op not in ZERO_GRADIENT and any(wanted[i] for i in node.inputs))
+
     cot = [None] * forward_count
 
     def accumulate(nid, contribution):
@@ -150,7 +159,7 @@ def grad(graph, outputs, wrt, rules=None, prefix="d"):
         if rule is None:
             raise GradientError(f"no gradient rule for '{node.op}'")
         if rule in SELECTIVE:
-            contributions = rule(G, node, cot[nid], [depends[i] for i in node.inputs])
+            contributions = rule(G, node, cot[nid], [wanted[i] for i in node.inputs])
         else:
             contributions = rule(G, node, cot[nid])
         for k, inp in enumerate(node.inputs):
