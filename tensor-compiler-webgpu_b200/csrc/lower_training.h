@@ -55,6 +55,12 @@ static std::string word_attr(const Node& n, const std::string& name) {
 static void expect(const Node& n, bool ok, const std::string& what) {
   if (!ok) refuse(n, what);
 }
+// eps as the kernel takes it, a float32: one above 0 must stay so, or a zero norm is divided by zero.
+static void check_eps(const Node& n) {
+  const double eps = number_attr(n, "eps");
+  expect(n, eps >= 0 && std::isfinite((float)eps) && (eps == 0 || (float)eps > 0),
+         "eps must be 0 or a positive float32");
+}
 static const std::vector<i64>& in_shape(const Graph& g, const Node& n, size_t k) {
   expect(n, k < n.inputs.size(), "too few inputs");
   return g.nodes[n.inputs[k]].shape;
@@ -144,8 +150,7 @@ static void check_training(const Graph& g, const Node& n) {
     const i64 r = int_attr(n, "rotary");
     expect(n, r >= 0 && r <= x[3] && r % 2 == 0, "rotary must be an even part of a head");
     bool_attr(n, "interleaved");
-    const float eps = (float)number_attr(n, "eps");
-    expect(n, eps >= 0 && std::isfinite(eps), "eps must be a number of at least 0");
+    check_eps(n);
     expect(n, number_attr(n, "base") > 0, "base must be a number above 0");
     const Shape y = bool_attr(n, "headsFirst") ? Shape{x[0], x[2], x[1], x[3]} : x;
     if (back) {
@@ -167,8 +172,9 @@ static void check_training(const Graph& g, const Node& n) {
     expect(n, steps >= 1 && steps <= 32, "steps must be 1 to 32");
     const Value& co = attr(n, "coeffs");
     expect(n, co.is_array() && co.arr.size() == 3, "coeffs must be three numbers");
-    for (auto& v : co.arr) expect(n, v.is_number() && std::isfinite(v.num), "coeffs must be three numbers");
-    expect(n, number_attr(n, "eps") >= 0, "eps must be a number of at least 0");
+    for (auto& v : co.arr)
+      expect(n, v.is_number() && std::isfinite((float)v.num), "coeffs must be three float32 numbers");
+    check_eps(n);
     const double c[3] = {co.arr[0].num, co.arr[1].num, co.arr[2].num};
     int k[3];
     newton_schulz_scales(n, steps, c, k);

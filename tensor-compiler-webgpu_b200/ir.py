@@ -149,7 +149,18 @@ def infer_shape(op, shapes, attrs):
 
 
 def _number(v):
-    return isinstance(v, (int, float)) and not isinstance(v, bool) and math.isfinite(v)
+    if not isinstance(v, (int, float)) or isinstance(v, bool):
+        return False
+    try:
+        return math.isfinite(float(v))
+    except OverflowError:   # an int beyond every float
+        return False
+
+
+def _check_eps(op, eps):
+    """eps as the kernel takes it, a float32: one above 0 must stay so, or a zero norm is divided by zero."""
+    if not _number(eps) or eps < 0 or not math.isfinite(f32(eps)) or (eps > 0 and f32(eps) == 0):
+        raise ShapeError(f"{op}: eps must be 0 or a positive float32, got {eps!r}")
 
 
 def linear_nll_saved(R, d, V):
@@ -221,8 +232,7 @@ def _infer_head(op, shapes, attrs):
     for name in ("interleaved", "headsFirst"):
         if not isinstance(attrs.get(name), bool):
             raise ShapeError(f"{op}: {name} must be true or false")
-    if not _number(attrs.get("eps")) or f32(attrs["eps"]) < 0 or not math.isfinite(f32(attrs["eps"])):
-        raise ShapeError(f"{op}: eps must be a number of at least 0")
+    _check_eps(op, attrs.get("eps"))
     if not _number(attrs.get("base")) or attrs["base"] <= 0:
         raise ShapeError(f"{op}: base must be a number above 0")
     out = [B, H, T, D] if attrs["headsFirst"] else [B, T, H, D]
@@ -288,10 +298,9 @@ def _infer_orthogonalize(op, shapes, attrs):
     steps, co, eps = attrs.get("steps"), attrs.get("coeffs"), attrs.get("eps")
     if not _is_int(steps) or not 1 <= steps <= 32:
         raise ShapeError(f"{op}: steps must be 1 to 32, got {steps!r}")
-    if not isinstance(co, (list, tuple)) or len(co) != 3 or not all(_number(v) for v in co):
-        raise ShapeError(f"{op}: coeffs must be three numbers, got {co!r}")
-    if not _number(eps) or eps < 0:
-        raise ShapeError(f"{op}: eps must be a number of at least 0, got {eps!r}")
+    if not isinstance(co, (list, tuple)) or len(co) != 3 or not all(_number(v) and math.isfinite(f32(v)) for v in co):
+        raise ShapeError(f"{op}: coeffs must be three float32 numbers, got {co!r}")
+    _check_eps(op, eps)
     newton_schulz_scales(steps, co)
     return list(x)
 

@@ -51,3 +51,66 @@ def test_stopped_inputs_of_a_node_cost_nothing(pkg):
     G = pkg.autodiff.grad(g, [y], [h, w])
     assert [n.attrs["wrt"] for n in G.graph.nodes if n.op == "linearNllGrad"] == ["h"]
     assert G.graph.nodes[G.grads[1]].op == "const"
+
+
+# ---------------------------------------------------------------- numbers that a float32 does not hold
+def _lower(rt, js):
+    """(status, message) of the library's lowering of a graph's JSON."""
+    import ctypes
+    import json
+    out = ctypes.c_void_p()
+    status = rt.lib().tc_lower_json(json.dumps(js).encode(), b"{}", ctypes.byref(out))
+    message = rt.lib().tc_last_error().decode() if status else ""
+    if not status:
+        rt.lib().tc_lowered_free(out)
+    return status, message
+
+
+def _orth(g, **kw):
+    return g.orthogonalize(g.input("x", [4, 4]), **kw)
+
+
+def _head(g, **kw):
+    return g.head_norm_rope(g.input("x", [1, 3, 2, 4]), g.input("gain", [4]), g.input("pos", [3]), **kw)
+
+
+@pytest.mark.parametrize("build", [_orth, _head])
+@pytest.mark.parametrize("eps", [1e-46, 1e39, 1e300, 10 ** 400, -1e-46])
+def test_eps_is_a_float32(pkg, build, eps):
+    """The kernels take eps as a float32: a positive one that rounds to 0 would divide a zero norm by zero, one
+    beyond the range would make every value 0."""
+    rt = importlib.import_module(P + ".runtime")
+    g = pkg.ir.Graph()
+    with pytest.raises(pkg.ir.ShapeError, match="eps"):
+        build(g, eps=eps)
+    g = pkg.ir.Graph()
+    y = build(g)
+    js = g.to_json()
+    if abs(eps) < 1e308:
+        js["nodes"][y]["attrs"]["eps"] = eps
+        status, message = _lower(rt, js)
+        assert status == 1 and "eps" in message
+        with pytest.raises(pkg.ir.ShapeError, match="eps"):
+            pkg.ir.Graph.from_json(js)
+
+
+@pytest.mark.parametrize("eps", [0, 0.0, 1e-45, 3e38])
+def test_eps_at_the_ends_is_taken(pkg, eps):
+    rt = importlib.import_module(P + ".runtime")
+    for build in (_orth, _head):
+        g = pkg.ir.Graph()
+        build(g, eps=eps)
+        assert _lower(rt, g.to_json()) == (0, "")
+
+
+def test_coefficients_are_float32(pkg):
+    rt = importlib.import_module(P + ".runtime")
+    g = pkg.ir.Graph()
+    with pytest.raises(pkg.ir.ShapeError, match="coeffs"):
+        _orth(g, steps=1, coeffs=(1e39, 0.0, 0.0))
+    g = pkg.ir.Graph()
+    y = _orth(g, steps=1)
+    js = g.to_json()
+    js["nodes"][y]["attrs"]["coeffs"] = [1e39, 0, 0]
+    status, message = _lower(rt, js)
+    assert status == 1 and "coeffs" in message
