@@ -21,6 +21,7 @@ constexpr i64 NLL_CHUNK = 256, NS_CHUNK = 128, NS_PARTS = 512;
 constexpr i64 NLL_ROWS = 16;
 constexpr i64 NLL_ADD = 1, NLL_JOIN = 2, NLL_NO_LOSS = 4, NLL_DB = 8;
 constexpr double F16_ROOM = 60000.0;
+constexpr i64 MAX_DIM = (i64)1 << 30, MAX_VALUES = (i64)1 << 40;
 
 static i64 up_to(i64 n, i64 k) { return cdiv(n, k) * k; }
 static i64 nll_pitch(i64 cols) { return std::min<i64>(256, up_to(cols, 32)); }
@@ -113,8 +114,15 @@ static void newton_schulz_scales(const Node& n, i64 steps, const double co[3], i
 
 // Shapes and attributes, as the Python host's infer_shape checks them.
 static void check_training(const Graph& g, const Node& n) {
-  for (int i : n.inputs) {
-    for (i64 d : g.nodes[i].shape) expect(n, d >= 1, "operand of an empty shape");
+  for (size_t k = 0; k < n.inputs.size(); ++k) {
+    // (the saved value of linearNllGrad has one axis of any length)
+    const i64 most = n.op == "linearNllGrad" && k == 1 ? MAX_VALUES : MAX_DIM;
+    i64 values = 1;
+    for (i64 d : g.nodes[n.inputs[k]].shape) {
+      expect(n, d >= 1, "operand of an empty shape");
+      expect(n, d <= most && values <= MAX_VALUES / d, "operand beyond 2^30 an axis or 2^40 values");
+      values *= d;
+    }
   }
   Shape want;
   if (n.op == "linearNll") {
@@ -132,7 +140,7 @@ static void check_training(const Graph& g, const Node& n) {
     const bool bias = bool_attr(n, "bias");
     expect(n, n.inputs.size() == 3, "wrong number of inputs");
     const i64 d = int_attr(n, "d"), V = int_attr(n, "V");
-    expect(n, d >= 1 && V >= 1 && V <= ((i64)1 << 24), "d and V must be the weight's sizes");
+    expect(n, d >= 1 && d <= MAX_DIM && V >= 1 && V <= ((i64)1 << 24), "d and V must be the weight's sizes");
     const Shape& t = in_shape(g, n, 0);
     expect(n, t.size() == 1 && in_shape(g, n, 2) == t && in_shape(g, n, 1) == Shape{nll_saved(t[0], d, V).floats},
            "targets, saved value and cotangent do not belong together");

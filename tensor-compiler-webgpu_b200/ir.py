@@ -25,6 +25,8 @@ TRAINING_OPS = ("linearNll", "linearNllGrad", "headNormRope", "headNormRopeGrad"
 OPS += TRAINING_OPS
 MAX_CLASSES = 1 << 24    # class indices and positions are whole numbers in float32
 MAX_HEAD = 512
+# Of an operand of theirs: the kernels count rows and columns in 31 bits, both hosts bytes in 63.
+MAX_DIM, MAX_VALUES = 1 << 30, 1 << 40
 
 
 class ShapeError(ValueError):
@@ -185,7 +187,7 @@ def _infer_nll(op, shapes, attrs):
         if len(shapes) != 3:
             raise ShapeError(f"{op}: takes 3 inputs, got {len(shapes)}")
         d, V, wrt = attrs.get("d"), attrs.get("V"), attrs.get("wrt")
-        if not _is_int(d) or not _is_int(V) or d < 1 or not 1 <= V <= MAX_CLASSES:
+        if not _is_int(d) or not _is_int(V) or not 1 <= d <= MAX_DIM or not 1 <= V <= MAX_CLASSES:
             raise ShapeError(f"{op}: d and V must be the weight's sizes, got {d!r} and {V!r}")
         t, saved, gy = shapes
         if len(t) != 1 or list(gy) != list(t) or list(saved) != [linear_nll_saved(t[0], d, V)[1]]:
@@ -306,6 +308,9 @@ def _infer_orthogonalize(op, shapes, attrs):
 
 
 def _infer_training(op, shapes, attrs):
+    for s in shapes:
+        if any(d > MAX_DIM for d in s) and not (op == "linearNllGrad" and s is shapes[1]) or size(s) > MAX_VALUES:
+            raise ShapeError(f"{op}: an operand of shape {fmt(s)}, beyond {MAX_DIM} an axis or {MAX_VALUES} values")
     if op in ("linearNll", "linearNllGrad"):
         return _infer_nll(op, shapes, attrs)
     if op in ("headNormRope", "headNormRopeGrad"):

@@ -114,3 +114,48 @@ def test_coefficients_are_float32(pkg):
     js["nodes"][y]["attrs"]["coeffs"] = [1e39, 0, 0]
     status, message = _lower(rt, js)
     assert status == 1 and "coeffs" in message
+
+
+# ---------------------------------------------------------------- sizes beyond any device
+def _big(pkg, which):
+    g = pkg.ir.Graph()
+    if which == "orth-square":
+        g.orthogonalize(g.input("x", [1 << 32, 1 << 32]))
+    elif which == "orth-long":
+        g.orthogonalize(g.input("x", [1 << 31, 4]))
+    elif which == "nll-rows":
+        g.linear_nll(g.input("h", [1 << 62, 1]), g.input("w", [1, 5]), None, g.input("t", [1 << 62]))
+    elif which == "nll-wide":
+        g.linear_nll(g.input("h", [5, 1 << 24]), g.input("w", [1 << 24, 1 << 24]), None, g.input("t", [5]))
+    elif which == "head-batch":
+        g.head_norm_rope(g.input("x", [1 << 33, 1 << 33, 3, 8]), g.input("gain", [8]), g.input("pos", [1 << 33]))
+    else:
+        g.head_norm_rope(g.input("x", [1, 1 << 33, 3, 8]), g.input("gain", [8]), g.input("pos", [1 << 33]))
+    return g
+
+
+@pytest.mark.parametrize("which", ["orth-square", "orth-long", "nll-rows", "nll-wide", "head-batch", "head-tokens"])
+def test_sizes_beyond_any_device_are_refused(pkg, monkeypatch, which):
+    """Counts that leave 64 bits (a product of two sides became 0, and the process died dividing by it) or the 31
+    bits of a kernel's rows and columns: refused by both hosts."""
+    rt = importlib.import_module(P + ".runtime")
+    with pytest.raises(pkg.ir.ShapeError, match="beyond"):
+        _big(pkg, which)
+    monkeypatch.setattr(pkg.ir, "MAX_DIM", 1 << 70)
+    monkeypatch.setattr(pkg.ir, "MAX_VALUES", 1 << 200)
+    js = _big(pkg, which).to_json()
+    status, message = _lower(rt, js)
+    assert status == 1 and "beyond" in message
+
+
+def test_a_gradient_of_sizes_beyond_any_device_is_refused(pkg):
+    rt = importlib.import_module(P + ".runtime")
+    g = pkg.ir.Graph()
+    y = g.linear_nll(g.input("h", [5, 3]), g.input("w", [3, 4]), None, g.input("t", [5]))
+    js = pkg.autodiff.grad(g, [y], [0]).graph.to_json()
+    node = next(n for n in js["nodes"] if n["op"] == "linearNllGrad")
+    node["attrs"]["d"] = 1 << 45
+    status, message = _lower(rt, js)
+    assert status == 1 and "sizes" in message
+    with pytest.raises(pkg.ir.ShapeError, match="sizes"):
+        pkg.ir.Graph.from_json(js)
