@@ -2,16 +2,16 @@
 
 The step is split where the reference's step builder exposes the gradients
 (src/m3b/step.js:18-31): a gradient graph (forward + loss + autodiff
-backward) run on this rank's shard of the batch, then an Adam graph
-(src/m3b/adam.js:24-48) run identically on every rank, so parameters stay
-replicated.  Every gradient -- laid out back to back in one flat device buffer
+backward) run on this rank's shard of the batch, then the optimizer's graph
+(Adam, src/m3b/adam.js:24-48, or Muon) run identically on every rank, so parameters
+stay replicated.  Every gradient -- laid out back to back in one flat device buffer
 that the gradient graph writes directly -- is sum-allreduced over
 NVLink/NVSwitch and scaled by 1/W (each rank's loss divides by its local row
 count, src/m3b/model.js:127-130, so the average of the rank gradients is the
 full-batch gradient).  The buffer is ordered by when the backward finishes each
 gradient and cut into a few contiguous buckets; each bucket's allreduce runs on
-a collective stream while the rest of the backward computes, and the Adam graph
-waits for all of them.  World size 1 skips the collective.
+a collective stream while the rest of the backward computes, and the optimizer's
+graph waits for all of them.  World size 1 skips the collective.
 
 Process plumbing (rank, world, the NCCL unique id) goes through
 torch.distributed's gloo group on the host; the collective itself is the
@@ -136,7 +136,7 @@ class DPTrainer:
         self.flat = rt.DeviceBuffer(runner, max(total, 256))
         self.flat_floats = total // 4
         rt.check(rt.lib().tc_memset32(runner.ctx, self.flat.ptr, 0, max(total, 256) // 4))  # padding, zero grads
-        # parameters: one buffer each, shared by both graphs (the Adam graph's outputs are copied back)
+        # parameters: one buffer each, shared by both graphs (the update graph's outputs are copied back)
         self.params = {n: rt.DeviceBuffer(runner, size(shapes[n]) * 4) for n in names}
         place_g = {iid: self.params[n].ptr for iid, n in zip(input_ids, names)}
         # a gradient the graph gives as a constant zero (no dependence) is still written by its launch
@@ -170,7 +170,7 @@ class DPTrainer:
         for n in names:
             self.params[n].upload(np.asarray(params[n], dtype=np.float32))
         if state is None:
-            state = _steps.adam_initial_state(names, shapes)
+            state = _steps.initial_state(names, shapes, opt)
         for k in state_names:
             self.adam_prog.write(fa.index[ad["inputs"][k]], state[k])
         cot = fg.graph.input_id(gs["cotangent"])
@@ -183,7 +183,7 @@ class DPTrainer:
             self.adam_prog.capture()
 
     def step_device(self):
-        """One step with x, y already on the device: gradients, allreduce, Adam (asynchronous)."""
+        """One step with x, y already on the device: gradients, allreduce, update (asynchronous)."""
         self.grad_prog.run()   # with buckets, the allreduces run inside it
         if self.comm is not None and self.comm.world > 1 and self.buckets == 1:
             self.comm.allreduce_mean(self.flat.ptr, self.flat_floats, prescaled=self.prescaled)

@@ -418,14 +418,16 @@ def build_grad3b(V, B, cfg=CONFIG):
 
 
 def build_adam_graph(V, cfg=CONFIG, opt=ADAM_3B):
-    """Adam alone, its gradients as inputs named ``g:<param>`` (the graph after the allreduce)."""
+    """The optimizer's update alone (Adam, or by `opt` Muon), its gradients as inputs named ``g:<param>`` (the graph
+    after the allreduce)."""
     g = Graph()
     names = param_names(V, cfg)
     shapes = param_shapes(V, cfg)
     ids = {n: g.input(n, shapes[n]) for n in names}
     grads = {n: g.input(f"g:{n}", shapes[n]) for n in names}
-    state = {name: g.input(name, shape) for name, shape in adam_state_spec(names, shapes)}
-    outputs = adam_update(g, names, ids, grads, state, opt)
+    state = {name: g.input(name, shape) for name, shape in state_spec(names, shapes, opt)}
+    update = muon_update if opt["kind"] == "muon" else adam_update
+    outputs = update(g, names, ids, grads, state, opt)
     inputs = {**ids, **{f"g:{n}": grads[n] for n in names}, **state}
     return {"graph": g, "names": names, "inputs": inputs, "outputs": outputs}
 

@@ -159,3 +159,45 @@ def test_a_gradient_of_sizes_beyond_any_device_is_refused(pkg):
     assert status == 1 and "sizes" in message
     with pytest.raises(pkg.ir.ShapeError, match="sizes"):
         pkg.ir.Graph.from_json(js)
+
+
+# ---------------------------------------------------------------- Muon after the allreduce
+def _tiny_step(pkg, opt, **kw):
+    s = pkg.steps
+    cfg = s.make_config(T=6, d=8, H=2, L=1, ff=32, targets="index", rope=100.0, **kw)
+    return s, cfg, s.build_step3b(11, 2, cfg, opt=opt)
+
+
+def test_the_update_graph_is_the_steps_update(pkg):
+    """Gradients in, parameters and state out: what the whole step makes of the same gradients, for both optimizers."""
+    rng = np.random.default_rng(0)
+    for opt in (pkg.steps.ADAM_3B, pkg.steps.MUON_3B):
+        s, cfg, step = _tiny_step(pkg, opt)
+        up = s.build_adam_graph(11, cfg, opt)
+        shapes = s.param_shapes(11, cfg)
+        inputs = {n: rng.standard_normal(shapes[n]) for n in step["names"]}
+        inputs |= {n: np.asarray(0.9) if n.endswith("Pow") else np.abs(rng.standard_normal(sh))
+                   for n, sh in s.state_spec(step["names"], shapes, opt)}
+        inputs |= {"x": np.eye(11)[rng.integers(0, 11, 12)], "y": rng.integers(-1, 11, 12), step["cotangent"]: 1.0}
+        vals = ref.evaluate(step["graph"], inputs)
+        got = ref.evaluate(up["graph"], {**inputs, **{f"g:{n}": vals[i] for n, i in step["grads"].items()}})
+        assert set(up["outputs"]) == set(step["outputs"])
+        for n, i in step["outputs"].items():
+            assert np.allclose(got[up["outputs"][n]], vals[i], rtol=1e-12, atol=1e-14), n
+
+
+def test_data_parallel_trainer_takes_muon(pkg, monkeypatch):
+    """The trainer's two programs over Muon's state: every launch reads values still in place."""
+    from test_program_plan import Recorder, _replay
+    rt = importlib.import_module(P + ".runtime")
+    dp = importlib.import_module(P + ".dp")
+    rec = Recorder(rt.lib())
+    monkeypatch.setattr(rt, "lib", lambda: rec)
+    monkeypatch.setattr(rt.GpuRunner, "pipeline", lambda self, code: rt.Module(hash(code) & 0xFFFF, self))
+    s, cfg, step = _tiny_step(pkg, pkg.steps.MUON_3B)
+    params = s.init_params_normal(11, 0, 0.02, cfg)
+    tr = dp.DPTrainer(rt.GpuRunner(1, 0), 11, 2, cfg, params, opt=s.MUON_3B, capture=False)
+    _replay(tr.grad_prog, tr.fg.graph)
+    _replay(tr.adam_prog, tr.fa.graph)
+    assert sorted(tr.state_names) == sorted(step["stateNames"])
+    assert any(lau.kind == "orthogonalize" for lau in tr.adam_prog.launches)
