@@ -344,7 +344,10 @@ def adam_update(B, names, ids, grads, state, opt, sabotage=None):
 
 
 # ---------------------------------------------------------------- Muon
-MUON_3B = {"kind": "muon", "lr": 2e-2, "momentum": 0.95, "steps": 5, "weightDecay": 0, "adam": ADAM_3B}
+MUON = {"kind": "muon", "lr": 2e-2, "momentum": 0.95, "steps": 5, "weightDecay": 0, "adam": ADAM_3B}
+# The settings with Muon's shape factor turned round (rows / columns of a weight as it is stored, [in, out] here,
+# where Muon's definition has fan-out / fan-in): for runs that were begun with it.
+MUON_3B = {**MUON, "factor": "rows/columns"}
 MUON_KEYS = ("wq", "wk", "wv", "wo", "w1", "w2")
 
 
@@ -366,19 +369,24 @@ def initial_state(names, shapes, opt=ADAM_3B):
 
 
 def muon_update(B, names, ids, grads, state, opt):
-    """Momentum with Nesterov's look ahead, orthogonalised: W [m, n] -= lr sqrt(max(1, m / n)) orth(g + mu buf),
-    after decoupled weight decay.  Parameters that are not a block's weight matrix get Adam."""
+    """Momentum with Nesterov's look ahead, orthogonalised: W -= lr sqrt(max(1, fan-out / fan-in)) orth(g + mu buf),
+    after decoupled weight decay.  A weight here is [fan-in, fan-out] (x W); `opt["factor"]` "rows/columns" takes
+    the ratio the other way round.  Parameters that are not a block's weight matrix get Adam."""
     c = B.const
+    factor = opt.get("factor", "fan-out/fan-in")
+    if factor not in ("fan-out/fan-in", "rows/columns"):
+        raise ValueError(f"muon: factor must be 'fan-out/fan-in' or 'rows/columns', got {factor!r}")
     mu = muon_names(names)
     outputs = adam_update(B, [n for n in names if n not in mu], ids, grads, state, opt["adam"])
     for p in mu:
         buf = B.add(B.mul(c(opt["momentum"]), state[f"{p}.buf"]), grads[p])
         o = B.orthogonalize(B.add(grads[p], B.mul(c(opt["momentum"]), buf)), steps=opt["steps"])
         m, n = B.shape(ids[p])
+        ratio = n / m if factor == "fan-out/fan-in" else m / n
         w = ids[p]
         if opt["weightDecay"]:
             w = B.mul(w, c(1 - opt["lr"] * opt["weightDecay"]))
-        outputs[p] = B.sub(w, B.mul(c(opt["lr"] * math.sqrt(max(1.0, m / n))), o))
+        outputs[p] = B.sub(w, B.mul(c(opt["lr"] * math.sqrt(max(1.0, ratio))), o))
         outputs[f"{p}.buf"] = buf
     return outputs
 

@@ -171,7 +171,7 @@ def _tiny_step(pkg, opt, **kw):
 def test_the_update_graph_is_the_steps_update(pkg):
     """Gradients in, parameters and state out: what the whole step makes of the same gradients, for both optimizers."""
     rng = np.random.default_rng(0)
-    for opt in (pkg.steps.ADAM_3B, pkg.steps.MUON_3B):
+    for opt in (pkg.steps.ADAM_3B, pkg.steps.MUON):
         s, cfg, step = _tiny_step(pkg, opt)
         up = s.build_adam_graph(11, cfg, opt)
         shapes = s.param_shapes(11, cfg)
@@ -194,10 +194,31 @@ def test_data_parallel_trainer_takes_muon(pkg, monkeypatch):
     rec = Recorder(rt.lib())
     monkeypatch.setattr(rt, "lib", lambda: rec)
     monkeypatch.setattr(rt.GpuRunner, "pipeline", lambda self, code: rt.Module(hash(code) & 0xFFFF, self))
-    s, cfg, step = _tiny_step(pkg, pkg.steps.MUON_3B)
+    s, cfg, step = _tiny_step(pkg, pkg.steps.MUON)
     params = s.init_params_normal(11, 0, 0.02, cfg)
-    tr = dp.DPTrainer(rt.GpuRunner(1, 0), 11, 2, cfg, params, opt=s.MUON_3B, capture=False)
+    tr = dp.DPTrainer(rt.GpuRunner(1, 0), 11, 2, cfg, params, opt=s.MUON, capture=False)
     _replay(tr.grad_prog, tr.fg.graph)
     _replay(tr.adam_prog, tr.fa.graph)
     assert sorted(tr.state_names) == sorted(step["stateNames"])
     assert any(lau.kind == "orthogonalize" for lau in tr.adam_prog.launches)
+
+
+def test_muon_scales_by_fan_out_over_fan_in(pkg):
+    """Muon's factor is sqrt(max(1, fan-out / fan-in)), whatever way round a weight is stored: here w1 is
+    [d, 4 d] and gets 2, w2 [4 d, d] gets 1."""
+    s = pkg.steps
+    opt = {**s.MUON, "momentum": 0.0}
+    g = pkg.ir.Graph()
+    shapes = {"b0.w1": [4, 16], "b0.w2": [16, 4], "b0.wq": [4, 4]}
+    ids = {n: g.input(n, sh) for n, sh in shapes.items()}
+    grads = {n: g.input(f"g:{n}", sh) for n, sh in shapes.items()}
+    state = {n: g.input(n, sh) for n, sh in s.state_spec(list(shapes), shapes, opt)}
+    out = s.muon_update(g, list(shapes), ids, grads, state, opt)
+    rng = np.random.default_rng(1)
+    inputs = {n.attrs["name"]: rng.standard_normal(n.shape) for n in g.inputs()} | {"beta1Pow": 0.9, "beta2Pow": 0.9}
+    vals = ref.evaluate(g, inputs)
+    for n, factor in (("b0.w1", 2.0), ("b0.w2", 1.0), ("b0.wq", 1.0)):
+        o = ref.newton_schulz(inputs[f"g:{n}"], 5, (3.4445, -4.7750, 2.0315), 1e-7)
+        assert np.allclose(inputs[n] - vals[out[n]], 0.02 * factor * o, rtol=1e-9, atol=1e-12), n
+    with pytest.raises(ValueError, match="factor"):
+        s.muon_update(g, list(shapes), ids, grads, state, {**opt, "factor": "fan"})
