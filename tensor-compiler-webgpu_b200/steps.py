@@ -11,7 +11,11 @@ whose default is that same CONFIG.
 Beyond the reference, ``cfg`` may ask for ``"rope": base`` (queries and keys
 normalised per head and turned by position, in place of the learned positions)
 and ``"targets": "index"`` (``y`` holds each token's class, -1 for none, and the
-loss never makes the logits), and ``opt`` may be of kind ``"muon"``.
+loss never makes the logits), and ``opt`` may be of kind ``"muon"``.  With index
+targets the loss is the sum of the tokens' losses over B*T, tokens without a
+class counted in the divisor (it is the same on every rank and in every
+micro-batch, so gradients add up; scale the cotangent by B*T / count for a mean
+over the others), and the key ``"logits"`` holds the per-token losses [B*T].
 """
 from __future__ import annotations
 
@@ -122,6 +126,14 @@ def build_mlp_step(dims, batch, opt=None, hidden="relu", sabotage=None):
 
 # ---------------------------------------------------------------- transformer (src/m3b/model.js)
 CONFIG = {"T": 64, "d": 64, "H": 4, "dh": 16, "L": 2, "ff": 256, "eps": 1e-5, "mask": -1e4}
+
+
+def index_targets(cfg):
+    """Whether y holds classes; any other word than these two is refused."""
+    targets = cfg.get("targets", "one-hot")
+    if targets not in ("one-hot", "index"):
+        raise ValueError(f"targets must be 'one-hot' or 'index', got {targets!r}")
+    return targets == "index"
 
 
 def make_config(**kw):
@@ -286,7 +298,7 @@ def build_forward(V, B, cfg=CONFIG, bug=None):
     ids = {name: g.input(name, shape) for name, shape, _ in param_spec(V, cfg)}
     ids["x"] = g.input("x", [B * T, V])
     scores = []
-    if cfg.get("targets") == "index":   # no logits: the per-token losses stand in their place
+    if index_targets(cfg):   # no logits: the per-token losses stand in their place
         ids["y"] = g.input("y", [B * T])
         each = g.linear_nll(hidden_of(g, ids, V, B, cfg, bug, scores), ids["head"], ids["headb"], ids["y"])
         loss = g.div(g.sum(each, 0), g.const(B * T))
@@ -445,7 +457,7 @@ def encode_batch(seqs, V, T, targets="one-hot"):
     "index" y holds the classes themselves, [B*T]."""
     import numpy as np
     B = len(seqs)
-    if targets == "index":
+    if index_targets({"targets": targets}):
         x, _ = encode_batch(seqs, V, T)
         return x, np.asarray([s[1:T + 1] for s in seqs], np.float32).reshape(-1)
     x = np.zeros((B * T, V), dtype=np.float32)

@@ -222,3 +222,13 @@ def test_muon_scales_by_fan_out_over_fan_in(pkg):
         assert np.allclose(inputs[n] - vals[out[n]], 0.02 * factor * o, rtol=1e-9, atol=1e-12), n
     with pytest.raises(ValueError, match="factor"):
         s.muon_update(g, list(shapes), ids, grads, state, {**opt, "factor": "fan"})
+
+
+def test_unknown_targets_are_refused(pkg):
+    """A word that is neither form of the targets built the one-hot model before."""
+    s = pkg.steps
+    with pytest.raises(ValueError, match="targets"):
+        s.build_forward(7, 1, s.make_config(T=4, d=8, H=2, L=1, ff=16, targets="indices"))
+    with pytest.raises(ValueError, match="targets"):
+        s.encode_batch([[0, 1, 2, 3, 4]], 7, 4, "indices")
+    s.build_forward(7, 1, s.make_config(T=4, d=8, H=2, L=1, ff=16))
