@@ -179,6 +179,12 @@ i64 info_int(const Launch& l, const char* key, i64 dflt) {
   return dflt;
 }
 
+// Calls that clear their launch's control block in scratch, which other launches write to.  A program's private
+// block is zero from the start, and an error in it has to last until it is read.
+bool clears_control(const Call& c) {
+  return c.name == "tcb_gemm_prep" || c.name == "tcb_split_a" || c.name == "tcb_nll_amax" || c.name == "tcb_orth_norm";
+}
+
 // The argument block and tensor-map descriptors of one call (the Python host's runtime.issue).
 struct Issued {
   tc_args args;
@@ -202,7 +208,7 @@ int prepare_call(const Call& c, const std::vector<uint64_t>& ins, uint64_t out, 
   }
   if (c.err_offset >= 0) {
     while (params.size() < 16) params.push_back(0);
-    params[15] = (i64)(err_ptr ? err_ptr : scratch + (uint64_t)c.err_offset);
+    params[15] = (i64)(!err_ptr ? scratch + (uint64_t)c.err_offset : clears_control(c) ? 0 : err_ptr);
   }
   if (ins.size() > TC_MAX_OPERANDS || params.size() > TC_MAX_PARAMS)
     return tcb_detail::fail_msg(TC_ERR_INVALID, "call " + c.name + ": too many operands or parameters");

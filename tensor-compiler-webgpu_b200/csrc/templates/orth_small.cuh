@@ -8,7 +8,9 @@
 // S S, P) and across them (X in P X) alike.  Rows beyond the short side and columns beyond the long one are
 // zero; what the 128-row instruction reads below TCB_ROWS only makes rows that nobody looks at.
 //
-// grid: matrices; in[0] -> out; p[0] m, p[1] n, p[2] steps, p[15] the error word.
+// grid: matrices; in[0] -> out; p[0] m, p[1] n, p[2] steps, p[15] the error word.  No block looks at the word: only
+// a wait of 2 s that ran out writes it.  In scratch, at its start, it holds what other launches left, and the first
+// block clears it; a resident program's own word stays until it is read.
 #pragma once
 #include "tcb/gemm_f16x3.cuh"
 
@@ -91,7 +93,7 @@ extern "C" __global__ void __launch_bounds__(256, 1) tcb_orth_small(const tcb::A
   tc_fence_after();
   const u32 tmem = tmem_slot;
   grid_dependency_sync();
-  if (blockIdx.x == 0 && threadIdx.x == 0 && err) *err = 0u;
+  if (blockIdx.x == 0 && threadIdx.x == 0 && err && (u64)a.p[15] == a.scratch) *err = 0u;
 
   const u32 m = (u32)a.p[0], n = (u32)a.p[1], count = m * n;
   const bool tall = m > n;
@@ -141,7 +143,8 @@ extern "C" __global__ void __launch_bounds__(256, 1) tcb_orth_small(const tcb::A
       }
       __syncwarp();
     }
-    ok = __syncthreads_and(mbar_wait(done, phase, err, 1)) != 0;   // the same for every thread
+    ok = __syncthreads_and(mbar_wait(done, phase, nullptr, 1)) != 0;   // the same for every thread
+    if (!ok && threadIdx.x == 0 && err) atomicCAS(err, 0u, 1u);
     phase ^= 1;
     tc_fence_after();
   };

@@ -256,11 +256,17 @@ def _map_desc(call, scratch, ins=(), out=0):
     return (ctypes.c_uint64 * len(vals))(*vals)
 
 
+# Calls that clear their launch's control block in scratch, which other launches write to.  A program's private
+# block is zero from the start, and an error in it has to last until it is read.
+CLEARING = ("tcb_gemm_prep", "tcb_split_a", "tcb_nll_amax", "tcb_orth_norm")
+
+
 def issue(call, mod, ins, out, scratch, plan=None, err_ptr=None, ptrs=None):
     """Launch one KernelCall now (plan None) or append it to a native plan.
 
     A call with an error word gets its address in p[15]: `err_ptr` when given (a resident program's own
-    word for that launch), else its slot in the scratch buffer.  `ptrs` (node id -> device address)
+    word for that launch; none for a call that would only clear it, CLEARING), else its slot in the scratch
+    buffer.  `ptrs` (node id -> device address)
     resolves a call's `out_node` and `ptr_params` (a launch with a second output).
     """
     params = list(call.params)
@@ -273,7 +279,10 @@ def issue(call, mod, ins, out, scratch, plan=None, err_ptr=None, ptrs=None):
     if call.err_offset is not None:
         while len(params) < 16:
             params.append(0)
-        params[15] = err_ptr if err_ptr is not None else scratch + call.err_offset
+        if err_ptr is None:
+            params[15] = scratch + call.err_offset
+        else:
+            params[15] = 0 if call.name in CLEARING else err_ptr
     args = make_args(ins, out, scratch, params)
     g, b = _u32x3(call.grid), _u32x3(call.block)
     if call.tma:
@@ -709,8 +718,7 @@ class Program:
         # a private control block (error word + split-tile arrival counters) per launch that has one:
         # launches share scratch, so not there.  The blocks start zeroed and stay so -- a bounded wait
         # writes the error word only when it runs out (check_errors zeroes them again), the counters
-        # return to zero as each split tile completes -- so the one-block clearing launch
-        # (tcb_gemm_prep) that a one-off run needs is left out of the plan.
+        # return to zero as each split tile completes -- so nothing in the plan clears them (CLEARING).
         self.err_slot = {}
         off = 0
         for k, lau in enumerate(self.launches):

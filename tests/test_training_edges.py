@@ -232,3 +232,45 @@ def test_unknown_targets_are_refused(pkg):
     with pytest.raises(ValueError, match="targets"):
         s.encode_batch([[0, 1, 2, 3, 4]], 7, 4, "indices")
     s.build_forward(7, 1, s.make_config(T=4, d=8, H=2, L=1, ff=16))
+
+
+# ---------------------------------------------------------------- a resident program's error words
+def _graphs_with_waits(pkg):
+    """(graph, kept nodes): a launch of each kind that has a control block."""
+    g = pkg.ir.Graph()
+    h, w, b = g.input("h", [300, 260]), g.input("w", [260, 700]), g.input("b", [700])
+    y = g.linear_nll(h, w, b, g.input("t", [300]))
+    G = pkg.autodiff.grad(g, [y], [h, w, b])
+    yield G.graph, [y, *G.grads]
+    for shape in ([3, 64, 50], [3, 200, 300]):
+        g = pkg.ir.Graph()
+        yield g, [g.orthogonalize(g.input("x", shape))]
+    g = pkg.ir.Graph()
+    yield g, [g.matmul(g.input("a", [512, 4096]), g.input("b", [4096, 512]))]
+
+
+def test_replays_leave_the_error_words_alone(pkg, monkeypatch):
+    """What clears a control block in reused scratch does not get a resident program's private one, so an error
+    stays until it is read, however many runs come between; what waits gets it."""
+    from test_program_plan import Recorder
+    rt = importlib.import_module(P + ".runtime")
+    cg = importlib.import_module(P + ".codegen")
+    real = rt.lib()
+    rec = Recorder(real)
+    monkeypatch.setattr(rt.GpuRunner, "pipeline", lambda self, code: rt.Module(hash(code) & 0xFFFF, self))
+    kinds = set()
+    for graph, keep in _graphs_with_waits(pkg):
+        low = cg.lower(graph, matmul="tiled")
+        monkeypatch.setattr(rt, "lib", lambda: rec)
+        prog = rt.Program(rt.GpuRunner(1, 0), graph, low, keep=keep)
+        monkeypatch.setattr(rt, "lib", lambda: real)
+        issued = [(c, e) for (c, e) in zip([c for lau in prog.launches for c in rt.program_calls(lau)], rec.plans[prog.plan.value])]
+        lo, hi = prog.errs.ptr, prog.errs.ptr + prog.errs_bytes
+        for c, (_, name, _, args, maps) in issued:
+            assert c.name == name
+            if c.err_offset is None:
+                continue
+            waits = bool(maps) or name == "tcb_orth_small"
+            kinds.add((name.split("_")[1], waits))
+            assert lo <= args["p"][15] < hi if waits else args["p"][15] == 0, name
+    assert kinds >= {("nll", True), ("nll", False), ("orth", True), ("orth", False), ("gemm", True)}
