@@ -375,7 +375,7 @@ struct tc_program {
   std::map<int, uint64_t> ptrs;
   std::vector<int> err_words;   // byte offsets of the launches' error words in `errs`
   tc_buf* errs = nullptr;
-  uint64_t errs_ptr = 0;
+  uint64_t errs_ptr = 0, errs_bytes = 0;
   tc_plan* plan = nullptr;
   int launches = 0;
   ~tc_program() {
@@ -502,6 +502,7 @@ int tc_program_create(tc_ctx* ctx, tc_lowered* l, const int32_t* keep, int n_kee
     }
   }
   uint64_t errs_bytes = std::max<uint64_t>(64, off);
+  p->errs_bytes = errs_bytes;
   if (int s = tc_alloc(ctx, errs_bytes, 0, &p->errs)) return s;
   p->bufs.push_back(p->errs);
   p->errs_ptr = ptr_of(p->errs);
@@ -573,14 +574,15 @@ int tc_program_check(tc_program* p) {
   if (!p) return tcb_detail::fail_msg(TC_ERR_INVALID, "tc_program_check: null program");
   if (p->err_words.empty()) return TC_OK;
   if (int s = tc_sync(p->ctx, 600000)) return s;
+  std::vector<uint32_t> w(p->errs_bytes / 4);
+  if (int s = tc_memcpy_dtoh(p->ctx, w.data(), p->errs_ptr, p->errs_bytes)) return s;
+  if (int s = tc_sync(p->ctx, 600000)) return s;
   for (int off : p->err_words) {
-    uint32_t w = 0;
-    if (int s = tc_memcpy_dtoh(p->ctx, &w, p->errs_ptr + (uint64_t)off, 4)) return s;
-    if (int s = tc_sync(p->ctx, 600000)) return s;
-    if (w) {
-      tc_memset32(p->ctx, p->errs_ptr + (uint64_t)off, 0, 1);
-      return tcb_detail::fail_msg(TC_ERR_TIMEOUT, "a tensor-core launch's bounded wait ran out (code " + std::to_string(w) + ")");
-    }
+    const uint32_t code = w[(size_t)off / 4];
+    if (!code) continue;
+    // a launch that gave up left arrivals uncounted: all counters back to zero for the next run, not the words alone
+    if (int s = tc_memset32(p->ctx, p->errs_ptr, 0, p->errs_bytes / 4)) return s;
+    return tcb_detail::fail_msg(TC_ERR_TIMEOUT, "a tensor-core launch's bounded wait ran out (code " + std::to_string(code) + ")");
   }
   return TC_OK;
 }

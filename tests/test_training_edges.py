@@ -274,3 +274,39 @@ def test_replays_leave_the_error_words_alone(pkg, monkeypatch):
             kinds.add((name.split("_")[1], waits))
             assert lo <= args["p"][15] < hi if waits else args["p"][15] == 0, name
     assert kinds >= {("nll", True), ("nll", False), ("orth", True), ("orth", False), ("gemm", True)}
+
+
+@pytest.fixture(scope="module")
+def check_program(pkg, tmp_path_factory):
+    import os
+    import subprocess
+    from conftest import ROOT
+    rt = importlib.import_module(P + ".runtime")
+    rt.lib()
+    exe = str(tmp_path_factory.mktemp("check") / "check_program")
+    lib = os.path.join(ROOT, P)
+    subprocess.run(["gcc", "-O1", "-rdynamic", "-o", exe, os.path.join(ROOT, "tests", "c", "check_program.c"),
+                    "-I" + os.path.join(ROOT, "include"), "-L" + lib, "-ltcb200", "-Wl,-rpath," + lib], check=True)
+    return exe
+
+
+def test_the_library_clears_whole_control_blocks(pkg, check_program, tmp_path):
+    """tc_program_check after a wait that ran out: every arrival counter is zeroed with the error words, so the next
+    run does not take a part of a tile for the last; and no planned call clears a private block before."""
+    import json
+    import os
+    import subprocess
+    for k, (graph, keep) in enumerate(_graphs_with_waits(pkg)):
+        path = tmp_path / f"{k}.json"
+        path.write_text(json.dumps(graph.to_json()))
+        r = subprocess.run([check_program, str(path), ",".join(map(str, keep))], capture_output=True, text=True, timeout=60,
+                           env={**os.environ, "TCB_KERNEL_CACHE": str(tmp_path / "cubins")})
+        assert r.returncode == 0, r.stderr
+        *calls, last = r.stdout.splitlines()
+        rt = importlib.import_module(P + ".runtime")
+        for line in calls:
+            _, name, off = line.split()
+            assert name not in rt.CLEARING or off == "-1", line
+        assert any(int(line.split()[2]) >= 0 for line in calls)
+        words = last.split()
+        assert words[:4] == ["check", "5", "left", "0"] and words[-2:] == ["again", "0"], last
