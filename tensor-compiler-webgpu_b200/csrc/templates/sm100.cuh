@@ -30,7 +30,10 @@ __device__ __forceinline__ bool mbar_try(u32 bar, u32 parity) {
                : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
   return ok != 0;
 }
-// Bounded wait: false (and the error word set) if the barrier phase never completes.
+// Bounded wait: false (and the error word set) if the barrier phase never completes, or the word is set already.
+// Whoever gives up leaves after 1 ms more: copies and products in flight, which take microseconds, have then ended,
+// and a CTA neither exits nor frees its tensor memory under them.
+constexpr u32 SETTLE_NS = 1000000u;
 __device__ __forceinline__ bool mbar_wait(u32 bar, u32 parity, u32* err, u32 code) {
   if (mbar_try(bar, parity)) return true;
   const u64 t0 = now_ns();
@@ -38,6 +41,7 @@ __device__ __forceinline__ bool mbar_wait(u32 bar, u32 parity, u32* err, u32 cod
     if (mbar_try(bar, parity)) return true;
     if ((it & 255) == 0 && (now_ns() - t0 > WAIT_NS || (err && *(volatile u32*)err))) {
       if (err) atomicCAS(err, 0u, code);
+      for (const u64 t1 = now_ns(); now_ns() - t1 < SETTLE_NS;) { }
       return false;
     }
   }
