@@ -1,0 +1,90 @@
+"""The training operators on the B200 at the edges of what a call may ask: confident rows, masks at the end of the
+range, mixed magnitudes, memory left by other launches."""
+import importlib
+
+import numpy as np
+import pytest
+
+import training_ref as ref
+from test_gpu_training_ops import check_nll, check_orth, f32, mods, nll_case, nll_loss_case, run_graph, small_graphs, within  # noqa: F401
+from test_training_edges import _graphs_with_waits
+
+pytestmark = pytest.mark.gpu
+P = "tensor-compiler-webgpu_b200"
+U = ref.U
+
+
+# ---------------------------------------------------------------- memory that other launches left
+def test_one_off_runs_over_what_others_left_in_scratch(pkg, mods, runner):
+    """The runner's scratch full of ones' bits (error words, counters, partial sums): a one-off run clears what it
+    relies on, and gives what a resident program gives."""
+    rt, cg = mods
+    for graph, keep, x in small_graphs(pkg):
+        want = run_graph(mods, runner, graph, x, keep)
+        low = cg.lower(graph, matmul="tiled")
+        need = max(lau.scratch_bytes for lau in low["launches"])
+        ptr = runner.scratch(need)
+        rt.check(rt.lib().tc_memset32(runner.ctx, ptr, 0xFFFFFFFF, need // 4))
+        out = runner.run(graph, low, x)
+        for i, w in zip(keep, want):
+            assert np.array_equal(out["values"][i].reshape(w.shape), w), graph.nodes[i].op
+    g = pkg.ir.Graph()   # many matrices on one SM each
+    y = g.orthogonalize(g.input("x", [400, 20, 30]))
+    x = {"x": f32(np.random.default_rng(2).standard_normal((400, 20, 30)))}
+    want = run_graph(mods, runner, g, x, [y])[0]
+    rt.check(rt.lib().tc_memset32(runner.ctx, runner.scratch(256), 0xFFFFFFFF, 64))
+    assert np.array_equal(runner.run(g, cg.lower(g), x)["values"][y].reshape(want.shape), want)
+
+
+@pytest.mark.parametrize("capture", [False, True])
+def test_control_blocks_are_not_cleared_by_a_run(pkg, mods, runner, capture):
+    """The words beside a resident launch's error word, which nothing reads, last through its runs: an error there
+    would too."""
+    rt, cg = mods
+    for graph, keep in _graphs_with_waits(pkg):
+        prog = rt.Program(runner, graph, cg.lower(graph, matmul="tiled"), keep=keep, capture=capture)
+        try:
+            rng = np.random.default_rng(3)
+            for n in graph.inputs():
+                prog.write(n.id, rng.random(n.shape) if n.attrs["name"] != "t" else np.zeros(n.shape))
+            mark = np.array([0, 11, 12, 13], np.uint32)
+            for off in prog.err_slot.values():
+                rt.check(rt.lib().tc_memcpy_htod(runner.ctx, prog.errs.ptr + off, mark.ctypes.data, 16))
+            runner.sync()
+            for _ in range(2):
+                prog.run()
+            prog.check_errors()
+            words = prog.errs.download(prog.errs_bytes // 4, np.uint32)
+            for off in prog.err_slot.values():
+                assert np.array_equal(words[off // 4:off // 4 + 4], mark)
+                assert not words[off // 4 + 4:off // 4 + 16].any()   # the counters are back at zero
+        finally:
+            prog.free()
+
+
+# ---------------------------------------------------------------- Muon, data parallel
+def test_data_parallel_trainer_with_muon(pkg, runner):
+    """One rank of the data-parallel trainer with Muon against the single trainer: losses as the gradient programs'
+    orders of sums allow, and the weights after three steps."""
+    rt = importlib.import_module(P + ".runtime")
+    dp = importlib.import_module(P + ".dp")
+    s, V, B = pkg.steps, 300, 3
+    cfg = s.make_config(T=40, d=64, H=4, L=1, ff=128, targets="index", rope=10000.0)
+    params = {n: np.asarray(v, np.float32) for n, v in s.init_params_normal(V, 0, 0.05, cfg).items()}
+    step = s.build_step3b(V, B, cfg, opt=s.MUON)
+    state = s.initial_state(step["names"], s.param_shapes(V, cfg), s.MUON)
+    one = rt.FusedTrainer(runner, rt.fused_step(step, matmul="tiled"), params, state)
+    many = dp.DPTrainer(runner, V, B, cfg, params, opt=s.MUON)
+    try:
+        for t in range(3):
+            toks = np.random.default_rng(t).integers(0, V, (B, cfg["T"] + 1))
+            x, y = s.encode_batch([list(map(int, r)) for r in toks], V, cfg["T"], "index")
+            a, b = one.train(x.reshape(-1), y), many.train(x.reshape(-1), y)
+            assert abs(a - b) <= 1e-4 * abs(a), t
+        names = s.muon_names(step["names"])
+        u, v = one.read(names), many.read(names)
+        for n in names:   # three updates of norm about lr sqrt(short side) each, equal to 1 % of one
+            assert np.linalg.norm(u[n] - v[n]) <= 1e-2 * s.MUON["lr"] * np.sqrt(min(s.param_shapes(V, cfg)[n])), n
+    finally:
+        one.destroy()
+        many.destroy()
