@@ -73,7 +73,7 @@ static NllSaved nll_saved(i64 R, i64 d, i64 V) {
   auto blocked = [](i64 n) { return n <= 256 ? up_to(n, 32) : up_to(n, 256); };
   NllSaved s;
   s.lse = up_to(256 + 4 * up_to(V, 256), 256);
-  s.h = up_to(s.lse + 4 * R, 256);
+  s.h = up_to(s.lse + 8 * R, 256);
   s.w = up_to(s.h + 4 * R * blocked(d), 256);
   s.floats = up_to(s.w + 4 * d * blocked(V), 256) / 4;
   return s;
@@ -246,7 +246,7 @@ struct F16Plan {
   Tile tile;
   i64 grid = 0, whole = 0, quantum = 0;
 };
-static F16Plan f16_plan(i64 M, i64 N, i64 K, i64 batch, i64 chunk, bool symmetric = false) {
+static F16Plan f16_plan(i64 M, i64 N, i64 K, i64 batch, i64 chunk, bool symmetric = false, const Tile* only = nullptr) {
   static const i64 COST[4][6] = {{256, 2, 275, 6600, 3000, 2500}, {128, 2, 173, 3600, 1500, 1600},
                                  {128, 1, 180, 3000, 1500, 1200}, {64, 1, 140, 1500, 1000, 700}};
   F16Plan best;
@@ -260,12 +260,14 @@ static F16Plan f16_plan(i64 M, i64 N, i64 K, i64 batch, i64 chunk, bool symmetri
   for (auto& row : COST) {
     const Tile tile{row[0], row[1]};
     const i64 step = row[2], epi = row[3], once = row[4], part = row[5], units = SM_COUNT / tile.ctas;
-    if ((tile.bn > 64 && N <= tile.bn / 2) || M <= F16_BM * (tile.ctas - 1)) continue;
+    if (only ? tile.bn != only->bn || tile.ctas != only->ctas
+             : (tile.bn > 64 && N <= tile.bn / 2) || M <= F16_BM * (tile.ctas - 1))
+      continue;
     const i64 tiles = batch * f16_tiles(M, N, tile, symmetric);
     take(cdiv(tiles, units) * (steps * step + epi), tile, std::min<i64>(units, tiles) * tile.ctas, tiles, 1);
     for (i64 q = 1; q <= 64; q *= 2) {
       const i64 per = cdiv(K, 256 * q);
-      if (tiles >= units || per == 1) break;
+      if (only || tiles >= units || per == 1) break;
       const i64 grid = std::min<i64>(units, tiles * per), run = cdiv(tiles * per, grid);
       const i64 pieces = run == 1 ? per : per / run + 2;
       take(run * q * 16 * step + once + pieces * part + epi, tile, grid * tile.ctas, 0, q * (256 / chunk));
@@ -403,6 +405,7 @@ static Launch nll_grad_launch(const Graph& g, const std::vector<int>& ids) {
   const Node& node = g.nodes[ids[0]];
   const i64 R = in_shape(g, node, 0)[0], d = int_attr(node, "d"), V = int_attr(node, "V");
   const NllSaved in = nll_saved(R, d, V);
+  const F16Plan fwd = f16_plan(R, V, d, 1, NLL_CHUNK);
   const i64 most = std::max<i64>(256, DZ_BYTES / (4 * R) / 256 * 256);
   const i64 piece = std::min<i64>(up_to(cdiv(V, cdiv(V, most)), 256), up_to(V, 32)), pieces = cdiv(V, piece);
   std::map<std::string, int> want;
@@ -434,7 +437,8 @@ static Launch nll_grad_launch(const Graph& g, const std::vector<int>& ids) {
       partial = std::max(partial, nbytes);
       return calls.back();
     };
-    const F16Plan pz = f16_plan(R, n, d, 1, NLL_CHUNK);
+    // the forward's own plan, or its tile
+    const F16Plan pz = pieces == 1 ? fwd : f16_plan(R, n, d, 1, NLL_CHUNK, false, &fwd.tile);
     Call& c = add("tcb_nll_dz", R, n, d, pz, {h(false), w(true, pz.tile.cols()), blocked("scratch", dz, R, n, nll_pitch(n), 32, 32)});
     if (joined) c.ptr_params = {{14, want["b"]}};
     const F16Plan ph = f16_plan(R, d, n, 1, NLL_CHUNK), pw = f16_plan(d, n, R, 1, NLL_CHUNK);

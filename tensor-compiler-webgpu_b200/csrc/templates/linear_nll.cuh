@@ -14,9 +14,11 @@
 // of log 2: z2 = log2(e) z is one fma from the sums, its exponential one ex2 (2^-22 relative, as far off as the
 // operands' split).
 // What the backward needs of it is saved in one opaque value (NllSaved): the scales, b log2(e), each
-// row's log2 of the sum, and h and W as split for the tensor core, 4 bytes a value.
+// row's maximum m and sum s of exponentials below it, and h and W as split for the tensor core, 4 bytes a value.
+// m and s stay two floats: m + log2(s) in one is off by half a step of m, 4e-6 at logits of 100, and so would be
+// the gradient of a row whose target is all but certain (and that row's dz would not add up to 0).
 // Backward: the vocabulary is walked in pieces (a bounded workspace).  A piece's logits are computed
-// again, turned into dz in the epilogue -- as fp16 hi / lo, what the two products after it read;
+// again in the forward's order, turned into dz = (2^(z2 - m) - s [v = t]) g / s in the epilogue -- as fp16 hi / lo, what the two products after it read;
 // |dz| <= |g_i|, so its scale is known before -- and dh += dz W_piece^T and dW_piece = h^T dz follow.
 // db's column sums are taken in the dz epilogue, and added up there (or by tcb_nll_db) in the same way.
 //
@@ -62,7 +64,7 @@ template <bool BACK> struct Nll {
   }
   __device__ __forceinline__ NllScales* scales() const { return saved<NllScales>(0); }
   __device__ __forceinline__ float* bias2() const { return saved<float>(256); }
-  __device__ __forceinline__ float* lse2() const { return saved<float>((u64)a.p[8]); }
+  __device__ __forceinline__ float2* stats() const { return saved<float2>((u64)a.p[8]); }   // m, s of every row
   __device__ __forceinline__ float* amax() const { return scratch<float>(0); }
   __device__ __forceinline__ float2* g_scale() const { return scratch<float2>(0); }   // up, down (backward)
 };
@@ -261,7 +263,7 @@ __device__ __forceinline__ void nll_write(const Nll<false>& n, u64 row, float m,
   if (!((u32)a.p[13] & NLL_NO_LOSS))
     reinterpret_cast<float*>(a.p[14] ? (u64)a.p[7] : a.out)[row] =
         n.target(row) >= 0 ? (m - __ldcg(n.scratch<float>((u64)a.p[11]) + row)) * NLL_LN2 + logf(s) : 0.0f;
-  n.lse2()[row] = m + log2f(s);
+  n.stats()[row] = make_float2(m, s);
 }
 
 // Forward epilogue: a row's maximum and sum of exponentials over the half tile's columns, the target's
@@ -329,7 +331,7 @@ struct NllDz {
   const TmaDesc* map;
   const float* bias2;
   float* part_row;   // where this lane's column sums go
-  float z2, up, down, lse, g, bias;
+  float z2, up, down, m, s, g, bias;
   int t;
   __device__ __forceinline__ explicit NllDz(const GemmParams& P) : a(P.a), map(&P.maps[2]) {}
   // The cotangent's scale: each CTA's epilogue warps look through all of it behind the first product.
@@ -366,8 +368,9 @@ struct NllDz {
     const Nll<true> n(a);
     const u64 row = e.row < n.R() ? e.row : n.R() - 1;
     t = n.target(row);
-    lse = n.lse2()[row];
-    g = n.cotangent(row) * up;
+    m = n.stats()[row].x;
+    s = n.stats()[row].y;
+    g = n.cotangent(row) * up / s;
     if (e.row != row) t = -1;
     part_row = n.template scratch<float>((u64)a.p[11]) + ((u64)e.T.m0 / 32 + e.q) * n.V() + (u64)a.p[12] + e.lane;
     bias = bias2[nll_column(e, e.c0)];
@@ -380,24 +383,13 @@ struct NllDz {
     const u32 mine = nll_bit(t, col);
 #pragma unroll
     for (int j = 0; j < 32; j += 2) {
-      add2(v[j], v[j + 1], -lse, -lse);
+      add2(v[j], v[j + 1], -m, -m);
       v[j] = ex2(v[j]);
       v[j + 1] = ex2(v[j + 1]);
     }
-    if (BN == 64 && n.V() <= 32) {
-      // The whole row is here: made to add up to 1.  ex2 is low by 4e-8 of a row's sum on average, measured, which
-      // the sum of many rows keeps while their gradients of a few classes cancel (db of 4096 rows and 2 classes:
-      // 3.7e-6 off); with more classes each keeps less of it.
-      float s = 0.0f;
-#pragma unroll
-      for (int j = 0; j < 32; ++j) s += v[j];
-      s = 1.0f - s;   // exact
-#pragma unroll
-      for (int j = 0; j < 32; j += 2) fma2(v[j], v[j + 1], s, s, v[j], v[j + 1]);
-    }
     if (__any_sync(0xffffffffu, mine != 0u)) {   // in one block of 8 at 8192 classes
 #pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] = (mine >> j) & 1 ? v[j] - 1.0f : v[j];
+      for (int j = 0; j < 32; ++j) v[j] = (mine >> j) & 1 ? v[j] - s : v[j];
     }
 #pragma unroll
     for (int j = 0; j < 32; j += 2) mul2(v[j], v[j + 1], g, g);

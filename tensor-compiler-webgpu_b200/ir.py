@@ -167,14 +167,14 @@ def _check_eps(op, eps):
 
 def linear_nll_saved(R, d, V):
     """The value linearNll saves for its backward: byte offsets of its parts (the scales at 0, the scaled bias
-    at 256) and its size in floats.  h and W are held as fp16 pairs in blocks of 256 columns."""
+    at 256; "lse": each row's largest logit and sum of exponentials below it) and its size in floats.  h and W are held as fp16 pairs in blocks of 256 columns."""
     def up(n, k):
         return -(-n // k) * k
 
     def blocked(n):
         return up(n, 32) if n <= 256 else up(n, 256)
     lse = up(256 + 4 * up(V, 256), 256)
-    h = up(lse + 4 * R, 256)
+    h = up(lse + 8 * R, 256)
     w = up(h + 4 * R * blocked(d), 256)
     return {"lse": lse, "h": h, "w": w}, up(w + 4 * d * blocked(V), 256) // 4
 

@@ -67,8 +67,9 @@ F16_COST = {Tile(256, 2): (275, 6600, 3000, 2500), Tile(128, 2): (173, 3600, 150
             Tile(128, 1): (180, 3000, 1500, 1200), Tile(64, 1): (140, 1500, 1000, 700)}
 
 
-def f16_plan(M, N, K, batch, chunk, symmetric=False):
-    """(tile, grid, whole tiles, quantum) of a product (tcb/gemm_f16x3.cuh), the cheapest by F16_COST.
+def f16_plan(M, N, K, batch, chunk, symmetric=False, only=None):
+    """(tile, grid, whole tiles, quantum) of a product (tcb/gemm_f16x3.cuh), the cheapest by F16_COST; with
+    `only` whole tiles of that kind.
 
     Tiles go whole to the SMs in waves, or, where they are fewer than the SMs, in pieces of `quantum` chains
     of `chunk` K indices.  Dividing the last wave of more tiles than that does not pay: the CTAs then no
@@ -79,13 +80,13 @@ def f16_plan(M, N, K, batch, chunk, symmetric=False):
     for tile, (step, epi, once, part) in F16_COST.items():
         bn, ctas = tile
         units = SM_COUNT // ctas
-        if (bn > 64 and N <= bn // 2) or M <= F16_BM * (ctas - 1):
+        if tile != only if only else (bn > 64 and N <= bn // 2) or M <= F16_BM * (ctas - 1):
             continue
         tiles = batch * f16_tiles(M, N, tile, symmetric)
         plans = [(math.ceil(tiles / units) * (steps * step + epi), tile, min(units, tiles) * ctas, tiles, 1)]
         for q in (1, 2, 4, 8, 16, 32, 64):
             per = math.ceil(K / (256 * q))
-            if tiles >= units or per == 1:
+            if only or tiles >= units or per == 1:
                 break
             grid = min(units, tiles * per)
             run = math.ceil(tiles * per / grid)
@@ -279,9 +280,14 @@ def _nll_grad_launch(graph, ids):
     joined = "b" in want and _joined(math.ceil(V / 32), math.ceil(R / 32))
     calls, partial = [], 0
 
-    def add(name, wrt, M, N, K, maps, params):
+    # A piece's logits are the forward's, bit for bit: by its own plan where the piece is all of the vocabulary, else
+    # by its tile (several pieces have more tiles than there are SMs: neither divides them).  Computed in another
+    # order they would be off by roundings of the logits' size, and a row's largest no longer the one subtracted.
+    forward = f16_plan(R, V, d, 1, NLL_CHUNK)
+
+    def add(name, wrt, M, N, K, maps, params, plan=None):
         nonlocal partial
-        plan = f16_plan(M, N, K, 1, NLL_CHUNK)
+        plan = plan or f16_plan(M, N, K, 1, NLL_CHUNK)
         c, nbytes = _gemm(name, M, N, K, 1, plan, end, maps(plan[0].cols), params)
         c.err_offset = at["err"]
         if wrt is not None and want[wrt] != node.id:
@@ -303,7 +309,8 @@ def _nll_grad_launch(graph, ids):
         def z(mn, box_rows):
             return _blocked_operand("scratch", at["dz"], R, n, _pitch(n), mn, box_rows)
         out = _blocked("scratch", at["dz"], R, n, _pitch(n), 32, 32)
-        add("tcb_nll_dz", None, R, n, d, lambda cols: h(False) + w(True, cols) + out, params)
+        add("tcb_nll_dz", None, R, n, d, lambda cols: h(False) + w(True, cols) + out, params,
+            forward if pieces == 1 else f16_plan(R, n, d, 1, NLL_CHUNK, only=forward[0]))
         if joined:
             calls[-1].ptr_params = ((14, want["b"]),)
         ph, pw = f16_plan(R, d, n, 1, NLL_CHUNK), f16_plan(d, n, R, 1, NLL_CHUNK)

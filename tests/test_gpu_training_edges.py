@@ -14,6 +14,72 @@ P = "tensor-compiler-webgpu_b200"
 U = ref.U
 
 
+# ---------------------------------------------------------------- rows whose target is all but certain
+def _dz_bound(x, p, onehot):
+    """dz of a row (cotangent 1) from logits off by up to ez each: p (1 - p) 2 ez, since what all logits share is
+    subtracted with the maximum; the sum of exponentials off by es, which moves a probability by es p (1 - p); and
+    the exponential's 2^-22, the subtraction of s, the division and the product, half a step each."""
+    h, w, b = x["h"], x["w"], x["b"]
+    d, V = w.shape
+    ez = (ref.product_bound(d, 256) * U * (np.abs(h) @ np.abs(w) + np.abs(b)).max(1)
+          + 2.0 ** -39 * d * np.abs(h).max() * np.abs(w).max())[:, None]
+    es = U * (32 + 2 * (11 + V / 64) + 8)
+    return (2 * ez + es) * p * (1 - p) + 8 * U * p * (1 - p) + 4 * U * (p + onehot) * 2 + 2.0 ** -39
+
+
+@pytest.mark.parametrize("R,d,V,level,pieces", [(40, 16, 33, 0.0, 1), (300, 40, 300, 100.0, 1), (300, 40, 300, -1000.0, 1),
+                                                (200, 40, 900, 100.0, 4), (150, 600, 500, 100.0, 1), (1500, 64, 2600, 300.0, 1)])
+def test_nll_confident_rows(pkg, mods, runner, monkeypatch, R, d, V, level, pieces):
+    """A row's dz, read as db under a cotangent of that row alone, where the target has a probability of 1 - 1e-2 to
+    1 - 1e-13 and all logits stand far from 0: the gradient's error is of the probabilities' size, not of the logits'."""
+    to = importlib.import_module(P + ".training_ops")
+    if pieces > 1:
+        monkeypatch.setattr(to, "DZ_BYTES", 4 * R * 256)
+        assert to.nll_pieces(R, V)[1] == pieces
+    graph, y, grads, x = nll_case(pkg, R, d, V, wrt="b", seed=V)
+    rng = np.random.default_rng(R)
+    x["w"] = f32(rng.standard_normal((d, V)))
+    t = x["t"].astype(int)
+    margin = np.linspace(8, 34, R)      # the target's logit above the rest's noise
+    x["h"] = f32(0.05 * rng.standard_normal((R, d)) + x["w"].T[t] * (margin / (x["w"].T[t] ** 2).sum(1))[:, None])
+    x["b"] = f32(level + 0.1 * rng.standard_normal(V))
+    _, p, _ = ref.nll(x["h"], x["w"], x["b"], x["t"])
+    onehot = np.zeros_like(p)
+    onehot[np.arange(R), t] = 1.0
+    bound = _dz_bound(x, p, onehot)
+    for r in (0, R // 3, R // 2, 2 * R // 3, R - 1):
+        x["d0"] = (np.arange(R) == r).astype(np.float64)
+        db = run_graph(mods, runner, graph, x, [grads["b"]])[0]
+        within(db, p[r] - onehot[r], bound[r], f"dz of row {r}")
+
+
+@pytest.mark.parametrize("V", [33, 65, 300, 5000])
+def test_nll_gradients_of_a_row_add_up_to_zero(pkg, mods, runner, V):
+    """The mean over 8192 rows of what dz adds up to.  The forward takes an exponential against its half tile's
+    maximum and one to move that sum to the row's, the backward one against the row's: at most 2^-22 each (the
+    exponential's bound), and a half step for each of s, the division and the product."""
+    graph, y, grads, x = nll_case(pkg, 8192, 40, V, seed=V, wrt="b")
+    x["d0"][:] = 1.0
+    db = run_graph(mods, runner, graph, x, [grads["b"]])[0].astype(np.float64)
+    assert abs(db.sum()) / 8192 <= 3 * 2.0 ** -22 + 3 * U
+
+
+# ---------------------------------------------------------------- masks at the end of the range
+LOWEST = -3.4028234663852886e38
+
+
+def test_nll_every_class_at_the_lowest_float(pkg, mods, runner):
+    """A bias that masks every class leaves them alike, as adding it in float32 or float64 does: p = 1 / V."""
+    R, V = 40, 100
+    graph, y, grads, x = nll_case(pkg, R, 24, V, seed=1, wrt="b")
+    x["b"][:] = LOWEST
+    loss, db = run_graph(mods, runner, graph, x, [y, grads["b"]])
+    want = np.full(V, x["d0"].sum() / V)
+    np.subtract.at(want, x["t"].astype(int), x["d0"])
+    assert np.allclose(loss, np.log(V), rtol=8 * U)
+    assert np.allclose(db, want, rtol=0, atol=(R + 8) * U * x["d0"].sum())
+
+
 # ---------------------------------------------------------------- memory that other launches left
 def test_one_off_runs_over_what_others_left_in_scratch(pkg, mods, runner):
     """The runner's scratch full of ones' bits (error words, counters, partial sums): a one-off run clears what it
