@@ -262,7 +262,7 @@ __device__ __forceinline__ void nll_write(const Nll<false>& n, u64 row, float m,
   const Args& a = n.a;
   if (!((u32)a.p[13] & NLL_NO_LOSS))
     reinterpret_cast<float*>(a.p[14] ? (u64)a.p[7] : a.out)[row] =
-        n.target(row) >= 0 ? (m - __ldcg(n.scratch<float>((u64)a.p[11]) + row)) * NLL_LN2 + logf(s) : 0.0f;
+        nll_loss(m, s, __ldcg(n.scratch<float>((u64)a.p[11]) + row), n.target(row), reinterpret_cast<const float*>(a.in[2]));
   n.stats()[row] = make_float2(m, s);
 }
 

@@ -27,5 +27,13 @@ __device__ __forceinline__ void nll_join(float& m, float& s, const float2& x) {
   s = s * ex2(m - safe) + x.y * ex2(x.x - safe);
   m = mx;
 }
+// A row's loss from its maximum, its sum of exponentials and the target's logit (units of log 2); bias: all of it,
+// not read without one.  A bias below -2.36e38, a mask of the lowest float say, leaves the range in units of log 2
+// and stands at its end, beyond what the others' logits can move: that target's loss takes the bias itself.
+__device__ __forceinline__ float nll_loss(float m, float s, float z, int t, const float* bias) {
+  if (t < 0) return 0.0f;
+  if (TCB_BIAS && z <= -NLL_MAX && m > z) return fmaf(m, NLL_LN2, logf(s)) - __ldg(bias + t);
+  return (m - z) * NLL_LN2 + logf(s);
+}
 
 }  // namespace tcb

@@ -179,6 +179,6 @@ extern "C" __global__ void __launch_bounds__(1024) tcb_nll_rows_finish(const tcb
     for (int k = 1; k < 32; ++k) nll_join(m, s, sh[k]);
     const int t = nll_class(ld1(reinterpret_cast<const float*>(a.in[TCB_BIAS ? 3 : 2]) + row), V);
     const float z = __ldcg(reinterpret_cast<const float*>(a.scratch + (u64)a.p[2]) + row);
-    reinterpret_cast<float*>(a.out)[row] = t >= 0 ? (m - z) * NLL_LN2 + logf(s) : 0.0f;
+    reinterpret_cast<float*>(a.out)[row] = nll_loss(m, s, z, t, reinterpret_cast<const float*>(a.in[2]));
   }
 }

@@ -68,6 +68,31 @@ def test_nll_gradients_of_a_row_add_up_to_zero(pkg, mods, runner, V):
 LOWEST = -3.4028234663852886e38
 
 
+@pytest.mark.parametrize("R,train", [(6, False), (40, False), (40, True)])
+@pytest.mark.parametrize("bias", [LOWEST, -3e38, -2.5e38, -2e38, -1e30])
+def test_nll_target_masked_by_a_finite_bias(pkg, mods, runner, R, train, bias):
+    """A target that a finite bias masks: its loss is that bias's size, also where log2(e) times it leaves the range
+    of float32.  The bound: half a step of the product by log2(e), of the one by log 2 and of the result, and of both
+    constants."""
+    if train:
+        graph, y, grads, x = nll_case(pkg, R, 24, 200, seed=R)
+    else:
+        graph, y, x = nll_loss_case(pkg, R, 24, 200, seed=R)
+        grads = {}
+    x["b"][150:] = bias
+    x["t"][:] = np.arange(R) % 150
+    x["t"][1] = 170
+    out = run_graph(mods, runner, graph, x, [y, *grads.values()])
+    want, p, _ = ref.nll(x["h"], x["w"], x["b"], x["t"])
+    assert abs(out[0][1] - want[1]) <= 6 * U * abs(bias)
+    keep = np.arange(R) != 1
+    assert np.allclose(out[0][keep], want[keep], rtol=1e-4, atol=1e-5)
+    if train:
+        want = ref.nll_grad(x["h"], x["w"], x["b"], x["t"], x["d0"])
+        for k, got in zip(grads, out[1:]):
+            assert np.allclose(got, want[k], rtol=1e-3, atol=1e-5), k
+
+
 def test_nll_every_class_at_the_lowest_float(pkg, mods, runner):
     """A bias that masks every class leaves them alike, as adding it in float32 or float64 does: p = 1 / V."""
     R, V = 40, 100
