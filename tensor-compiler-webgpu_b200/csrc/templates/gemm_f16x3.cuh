@@ -4,7 +4,7 @@
 //
 // An operand value x, scaled by a power of two s so that the largest one lies in [2^14, 2^15), is held
 // as hi = fp16(x s) and lo = fp16(x s - hi): 22 significant bits, or an absolute error of 2^-25 where lo
-// is subnormal, 2^-40 of the operand's largest value.  A product is
+// is subnormal, up to 2^-39 of the operand's largest value.  A product is
 //   A.B ~= A_lo.B_hi + A_hi.B_lo + A_hi.B_hi     (A_lo.B_lo, below 2^-22 of a term, dropped)
 // scaled back, exactly, in the epilogue.  The operands carry what the 3xTF32 split's do (tcb/gemm_tc.cuh:
 // 11 + 11 bits too) at twice the rate and half the bytes: hi and lo together take the 4 bytes of the float

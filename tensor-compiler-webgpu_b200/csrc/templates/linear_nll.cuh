@@ -22,9 +22,11 @@
 // |dz| <= |g_i|, so its scale is known before -- and dh += dz W_piece^T and dW_piece = h^T dz follow.
 // db's column sums are taken in the dz epilogue, and added up there (or by tcb_nll_db) in the same way.
 //
-// dz below 2^-40 of the largest |g_i| rounds to zero, and keeps fewer than 22 bits below 2^-18 of it: the
-// gradient of a class whose probability is that small in every row has that absolute accuracy, which is
-// beneath the float32 rounding of the sums it enters.
+// Range: h, W and dz have one scale each.  A value keeps 22 bits down to 2^-18 of its operand's largest, an absolute
+// 2^-39 of the largest below that, and nothing under that.  Results are therefore accurate as float32 in norm; by
+// element they are not where small values meet small ones only: dW's column of a class that is improbable in every row
+// (dz of 1e-8 of the largest is off by 1e-4 of itself, 1e-12 is lost), dh of a row whose cotangent is as small beside
+// the largest, the logits of the other rows beside one row of h with far larger values.
 //
 // p[] of every kernel: [0..3] the product's (split: [0] blocks of the amax launch; finish: [0] half tiles of a
 // row), [4] R, [5] d, [6] V, [7] byte offset of the saved value in scratch (when nobody asks for a backward;

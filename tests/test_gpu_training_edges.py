@@ -105,6 +105,22 @@ def test_nll_every_class_at_the_lowest_float(pkg, mods, runner):
     assert np.allclose(db, want, rtol=0, atol=(R + 8) * U * x["d0"].sum())
 
 
+# ---------------------------------------------------------------- mixed magnitudes
+@pytest.mark.parametrize("what", ["rows", "cotangents", "classes"])
+def test_nll_mixed_magnitudes(pkg, mods, runner, what):
+    """One scale for the whole of h, of W and of dz: beside its own 22 bits a value keeps 2^-39 of its operand's
+    largest, and every result stands within what that makes of it."""
+    case = nll_case(pkg, 130, 48, 200, seed=11)
+    x = case[3]
+    if what == "rows":
+        x["h"] = f32(x["h"] * 10.0 ** np.linspace(-9, 1, 130)[:, None])
+    elif what == "cotangents":
+        x["d0"] = f32(10.0 ** np.linspace(-20, 0, 130))
+    else:
+        x["b"] = f32(np.linspace(-60, 0, 200))
+    check_nll(mods, runner, case)
+
+
 # ---------------------------------------------------------------- memory that other launches left
 def test_one_off_runs_over_what_others_left_in_scratch(pkg, mods, runner):
     """The runner's scratch full of ones' bits (error words, counters, partial sums): a one-off run clears what it
