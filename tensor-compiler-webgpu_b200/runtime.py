@@ -469,8 +469,8 @@ def run_local(runner, graph, lowered, values, canary=False):
     """Node-local run (src/gpu/harness-m3b.js:86): each launch on float32 reference operands.
 
     `values` are reference values per node (any float dtype); each launch's
-    operands are uploaded rounded to float32, and its own output is read back.
-    Returns a list with the output of every launched node (None elsewhere).
+    operands are uploaded rounded to float32, and its own outputs are read back.
+    Returns a list with the value of every launched node (None elsewhere).
     """
     out = [None] * len(graph.nodes)
     for lau in lowered["launches"]:
@@ -478,19 +478,24 @@ def run_local(runner, graph, lowered, values, canary=False):
         try:
             ins = []
             for i in lau.inputs:
+                if values[i] is None:
+                    raise ValueError(f"launch for node {lau.node}: no value for its operand, node {i}")
                 b = DeviceBuffer(runner, max(1, size(graph.nodes[i].shape)) * 4)
-                b.upload(np.asarray(values[i], dtype=np.float32).reshape(-1))
                 bufs.append(b)
+                b.upload(np.asarray(values[i], dtype=np.float32).reshape(-1))
                 ins.append(b.ptr)
-            n = size(graph.nodes[lau.node].shape)
-            ob = DeviceBuffer(runner, max(1, n) * 4, ((-(-n // WG)) * WG + WG - n) * 4 if canary else 0)
-            bufs.append(ob)
-            sc = runner.launch(lau, ins, ob.ptr)
+            made = {}
+            for i in getattr(lau, "nodes", [lau.node]):
+                n = size(graph.nodes[i].shape)
+                made[i] = DeviceBuffer(runner, max(1, n) * 4, ((-(-n // WG)) * WG + WG - n) * 4 if canary else 0)
+                bufs.append(made[i])
+            sc = runner.launch(lau, ins, made[lau.node].ptr, {i: b.ptr for i, b in made.items()})
             runner.sync()
             runner.check_errors(lau, sc)
-            out[lau.node] = ob.download(n)
-            if canary and not ob.canary_intact():
-                raise TcError(1, f"launch for node {lau.node} wrote past its output")
+            for i, b in made.items():
+                out[i] = b.download(size(graph.nodes[i].shape))
+                if canary and not b.canary_intact():
+                    raise TcError(1, f"launch for node {lau.node} wrote past its output, node {i}")
         finally:
             for b in bufs:
                 b.free()

@@ -96,11 +96,12 @@ class Bench:
             rt.check(rt.lib().tc_memset32(self.runner.ctx, scratch.ptr, 0, scratch_bytes // 4))
         h = rt.ctypes.c_void_p()
         rt.check(rt.lib().tc_plan_create(self.runner.ctx, rt.ctypes.byref(h)))
+        at = {i: b.ptr for i, b in enumerate(bufs)}   # a launch's further outputs (graph_program's buffers are nodes)
         for d in program["dispatches"]:
             mod = self.pipeline(d["code"])
-            ptrs = [bufs[i].ptr for i in d["bindings"]]
+            ptrs = [at[i] for i in d["bindings"]]
             for call in d["calls"]:
-                rt.issue(call, mod, ptrs[:-1], ptrs[-1], scratch.ptr if scratch else 0, plan=h)
+                rt.issue(call, mod, ptrs[:-1], ptrs[-1], scratch.ptr if scratch else 0, plan=h, ptrs=at)
         return {"program": program, "buffers": bufs, "scratch": scratch, "plan": h}
 
     def reset(self, prepared):

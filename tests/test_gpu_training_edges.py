@@ -195,3 +195,18 @@ def test_data_parallel_trainer_with_muon(pkg, runner):
     finally:
         one.destroy()
         many.destroy()
+
+
+def test_node_local_runs_of_launches_with_several_outputs(pkg, mods, runner):
+    """run_local: both gradients of a head norm in one launch, each read back; an operand that has no value by the
+    definition (what the loss saves) is asked for by name."""
+    rt, cg = mods
+    from test_training_edges import _multi_output
+    (nll, vals), (head, hv) = _multi_output(pkg)
+    out = rt.run_local(runner, head, cg.lower(head), hv, canary=True)
+    for n in head.nodes:
+        if n.op == "headNormRopeGrad":
+            assert np.allclose(out[n.id].reshape(n.shape), hv[n.id], rtol=1e-5, atol=1e-5)
+    vals[next(n.id for n in nll.nodes if n.attrs.get("out") == "saved")] = None
+    with pytest.raises(ValueError, match="no value"):
+        rt.run_local(runner, nll, cg.lower(nll), vals)

@@ -310,3 +310,43 @@ def test_the_library_clears_whole_control_blocks(pkg, check_program, tmp_path):
         assert any(int(line.split()[2]) >= 0 for line in calls)
         words = last.split()
         assert words[:4] == ["check", "5", "left", "0"] and words[-2:] == ["again", "0"], last
+
+
+# ---------------------------------------------------------------- launches with several outputs, by every host
+def _multi_output(pkg):
+    """(graph, values of its nodes in 64 bits): a loss with its gradients, a head norm with both of its."""
+    rng = np.random.default_rng(4)
+    g = pkg.ir.Graph()
+    h, w = g.input("h", [30, 8]), g.input("w", [8, 20])
+    y = g.linear_nll(h, w, None, g.input("t", [30]))
+    G = pkg.autodiff.grad(g, [y], [h, w]).graph
+    yield G, ref.evaluate(G, {"h": rng.standard_normal((30, 8)), "w": rng.standard_normal((8, 20)), "t": rng.integers(0, 20, 30),
+                              "d0": rng.random(30)})
+    g = pkg.ir.Graph()
+    x, gain = g.input("x", [2, 5, 3, 8]), g.input("gain", [8])
+    G = pkg.autodiff.grad(g, [g.head_norm_rope(x, gain, g.input("pos", [5]))], [x, gain]).graph
+    yield G, ref.evaluate(G, {"x": rng.standard_normal((2, 5, 3, 8)), "gain": rng.standard_normal(8), "pos": np.arange(5),
+                              "d0": rng.standard_normal((2, 3, 5, 8))})
+
+
+def test_timed_programs_of_launches_with_several_outputs(pkg, monkeypatch):
+    """A graph timed (timing.graph_program): every output of a launch goes to its own node's buffer."""
+    from test_program_plan import Recorder
+    rt, cg, timing = (importlib.import_module(f"{P}.{m}") for m in ("runtime", "codegen", "timing"))
+    rec = Recorder(rt.lib())
+    for G, vals in _multi_output(pkg):
+        low = cg.lower(G)
+        prog = timing.graph_program(G, low, {n.attrs["name"]: vals[n.id] for n in G.inputs()}, [])
+        with monkeypatch.context() as m:
+            m.setattr(rt, "lib", lambda: rec)
+            m.setattr(rt.GpuRunner, "pipeline", lambda self, code: rt.Module(1, self))
+            bench = object.__new__(timing.Bench)
+            bench.runner, bench.counts = rt.GpuRunner(1, 0), {}
+            bench.pipeline, bench._count = bench.runner.pipeline, lambda what: None
+            made = bench.prepare(prog)
+        multi = [lau for lau in low["launches"] if len(getattr(lau, "nodes", [])) > 1]
+        assert multi
+        used = {v for e in rec.plans[made["plan"].value] for v in (e[3]["out"], *e[3]["p"])}
+        for lau in multi:
+            for i in lau.nodes:
+                assert made["buffers"][i].ptr in used
