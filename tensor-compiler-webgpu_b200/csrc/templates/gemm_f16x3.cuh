@@ -396,6 +396,7 @@ __device__ __forceinline__ void gemm_f16x3(const F16Job& J, u32* err, EPI& epi) 
   const u32 tmem = *tmem_slot;
   grid_dependency_sync();   // the set-up above touched this CTA's shared and tensor memory only
 
+  bool ok = true;   // this thread's waits have not given up
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     // Both warps run their loops whole and one elected lane issues: the operands of the copies and products are
@@ -405,7 +406,6 @@ __device__ __forceinline__ void gemm_f16x3(const F16Job& J, u32* err, EPI& epi) 
     auto wait = [&](u32 bar, u32 parity, u32 code) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, code)) != 0; };
     if (warp == 0) {
       u32 it = 0, s = 0, phase = 0;
-      bool ok = true;
       while (ok && work.next()) {
         const F16Tile T = f16_tile<BN, CTAS, SYM>(work.tile, tm, tn, per);
         const u32 kend = work.c1 * CK < kbs ? work.c1 * CK : kbs;
@@ -441,7 +441,7 @@ __device__ __forceinline__ void gemm_f16x3(const F16Job& J, u32* err, EPI& epi) 
         }
       }
       // wait (bounded) for the copies still in flight before this CTA (the leader: the pair) may exit
-      if (rank == 0) for (u32 i = it > STAGES ? it - STAGES : 0; i < it; ++i) mbar_wait(full(i % STAGES), (i / STAGES) & 1, err, 2);
+      if (rank == 0) for (u32 i = it > STAGES ? it - STAGES : 0; i < it; ++i) ok &= mbar_wait(full(i % STAGES), (i / STAGES) & 1, err, 2);
     } else if (warp == 1 && rank == 0) {
       constexpr u32 ID = idesc_f16(TM, BN, A_MN ? 1u : 0u, B_MN ? 1u : 0u), AH = f16_desc_hi<A_MN>(), BH = f16_desc_hi<B_MN>();
       // hi to lo plane, and one K step on, in descriptor units of 16 bytes
@@ -449,7 +449,6 @@ __device__ __forceinline__ void gemm_f16x3(const F16Job& J, u32* err, EPI& epi) 
       constexpr u32 BL = (B_MN ? HG_K * 128 : S::B_BYTES) >> 4, BK = (B_MN ? 2048 : 32) >> 4;
       const u32 a0 = f16_desc_lo<A_MN>(base), b0 = f16_desc_lo<B_MN>(base + 2 * S::A_BYTES);
       u32 j = 0, s = 0, phase = 0, da = a0, db = b0;   // j counts chunks
-      bool ok = true;
       while (ok && work.next()) {
         for (u32 c = work.c0; ok && c < work.c1; ++c, ++j) {
           const u32 k1 = (c + 1) * CK < kbs ? CK : kbs - c * CK, buf = j & 1;
@@ -505,7 +504,6 @@ __device__ __forceinline__ void gemm_f16x3(const F16Job& J, u32* err, EPI& epi) 
     e.vec = reinterpret_cast<float*>(gbase + (vectors - base)) + w * 32;
     epi.start(e.gstage - w * 4096);
     u32 j = 0;
-    bool ok = true;
     while (ok && work.next()) {
       e.T = f16_tile<BN, CTAS, SYM>(work.tile, tm, tn, per);
       e.T.m0 += (int)rank * HG_M;
@@ -562,7 +560,7 @@ __device__ __forceinline__ void gemm_f16x3(const F16Job& J, u32* err, EPI& epi) 
     epi.done(e);
   }
   tc_fence_before();
-  __syncthreads();
+  sync_settled(!ok);
   if constexpr (CTAS == 2) pair_sync();   // neither CTA ends, nor gives up its tensor memory, while the other works
   if (warp == 1) {
     tc_fence_after();

@@ -336,6 +336,7 @@ extern "C" __global__ void __launch_bounds__((TCB_FS_A || TCB_FS_B) ? 320 : 192,
   // kernel's tail (programmatic dependent launch); every global access comes after this wait
   grid_dependency_sync();
 
+  bool gave_up = false;   // a wait of this thread
   if (warp == 0) {
     if (lane == 0) {
       u32 it = 0;
@@ -344,7 +345,7 @@ extern "C" __global__ void __launch_bounds__((TCB_FS_A || TCB_FS_B) ? 320 : 192,
         const Tile T = decode(t);
         for (u32 kb = 0; kb < T.kb; ++kb, ++it) {
           const int s = it % STAGES;
-          if (it >= (u32)STAGES && !mbar_wait(empty(s), ((it / STAGES) - 1) & 1, err, 1)) { ok = false; break; }
+          if (it >= (u32)STAGES && !mbar_wait(empty(s), ((it / STAGES) - 1) & 1, err, 1)) { ok = false; gave_up = true; break; }
           const u32 st = base + s * STAGE_BYTES;
           const int kc = (int)((T.kb0 + kb) * GB_K);
           // maps: [0] A_hi or raw A, [1] A_lo, [2] B_hi or raw B, [3] B_lo; an MN-major raw tile is GB_K
@@ -369,7 +370,8 @@ extern "C" __global__ void __launch_bounds__((TCB_FS_A || TCB_FS_B) ? 320 : 192,
         }
       }
       // drain: wait (bounded) for the copies still in flight before this CTA may exit
-      for (u32 i = it > (u32)STAGES ? it - STAGES : 0; i < it; ++i) mbar_wait(full(i % STAGES), (i / STAGES) & 1, err, 2);
+      for (u32 i = it > (u32)STAGES ? it - STAGES : 0; i < it; ++i)
+        gave_up |= !mbar_wait(full(i % STAGES), (i / STAGES) & 1, err, 2);
     }
   } else if (warp == 1) {
     if (lane == 0) {
@@ -382,13 +384,13 @@ extern "C" __global__ void __launch_bounds__((TCB_FS_A || TCB_FS_B) ? 320 : 192,
       for (u32 t = blockIdx.x; ok && t < S::UNITS; t += S::GRID, ++j) {
         const Tile T = decode(t);
         const u32 buf = j & 1;
-        if (j >= 2 && !mbar_wait(acce(buf), ((j >> 1) - 1) & 1, err, 5)) break;
+        if (j >= 2 && !mbar_wait(acce(buf), ((j >> 1) - 1) & 1, err, 5)) { gave_up = true; break; }
         tc_fence_after();
         const u32 acc = tmem + buf * BN;
         for (u32 kb = 0; kb < T.kb; ++kb, ++it) {
           const int s = it % STAGES;
-          if (!mbar_wait(full(s), (it / STAGES) & 1, err, 3)) { ok = false; break; }
-          if (FS && !mbar_wait(conv(s), (it / STAGES) & 1, err, 7)) { ok = false; break; }
+          if (!mbar_wait(full(s), (it / STAGES) & 1, err, 3)) { ok = false; gave_up = true; break; }
+          if (FS && !mbar_wait(conv(s), (it / STAGES) & 1, err, 7)) { ok = false; gave_up = true; break; }
           tc_fence_after();
           const u32 st = base + s * STAGE_BYTES;
 #pragma unroll
@@ -418,7 +420,7 @@ extern "C" __global__ void __launch_bounds__((TCB_FS_A || TCB_FS_B) ? 320 : 192,
       const Tile T = decode(t);
       for (u32 kb = 0; kb < T.kb; ++kb, ++it) {
         const int s = it % STAGES;
-        if (!mbar_wait(full(s), (it / STAGES) & 1, err, 6)) { ok = false; break; }
+        if (!mbar_wait(full(s), (it / STAGES) & 1, err, 6)) { ok = false; gave_up = true; break; }
         unsigned char* st = gbase + s * STAGE_BYTES;
         if (FA) {
           const float4* ra = reinterpret_cast<const float4*>(st);
@@ -470,7 +472,7 @@ extern "C" __global__ void __launch_bounds__((TCB_FS_A || TCB_FS_B) ? 320 : 192,
     for (u32 t = blockIdx.x; t < S::UNITS; t += S::GRID, ++j) {
       const Tile T = decode(t);
       const u32 buf = j & 1;
-      if (!mbar_wait(accf(buf), (j >> 1) & 1, err, 4)) break;
+      if (!mbar_wait(accf(buf), (j >> 1) & 1, err, 4)) { gave_up = true; break; }
       tc_fence_after();
       const u64 row = (u64)T.m0 + 32 * q + lane;
       if (S::TAIL > 1 && T.tail >= 0) {
@@ -609,7 +611,7 @@ extern "C" __global__ void __launch_bounds__((TCB_FS_A || TCB_FS_B) ? 320 : 192,
     if (TCB_TMA_STORE && lane == 0) bulk_wait_all();  // the staged stores are done before the CTA exits
   }
   tc_fence_before();
-  __syncthreads();
+  sync_settled(gave_up);
   if (warp == 1) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"((u32)(2 * BN)) : "memory");

@@ -225,7 +225,7 @@ extern "C" __global__ void __launch_bounds__(256, 1) tcb_orth_small(const tcb::A
     }
   }
   tc_fence_before();
-  __syncthreads();
+  sync_settled(!ok);
   if (warp == 0) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(512u) : "memory");

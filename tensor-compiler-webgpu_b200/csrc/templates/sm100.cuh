@@ -31,9 +31,6 @@ __device__ __forceinline__ bool mbar_try(u32 bar, u32 parity) {
   return ok != 0;
 }
 // Bounded wait: false (and the error word set) if the barrier phase never completes, or the word is set already.
-// Whoever gives up leaves after 1 ms more: copies and products in flight, which take microseconds, have then ended,
-// and a CTA neither exits nor frees its tensor memory under them.
-constexpr u32 SETTLE_NS = 1000000u;
 __device__ __forceinline__ bool mbar_wait(u32 bar, u32 parity, u32* err, u32 code) {
   if (mbar_try(bar, parity)) return true;
   const u64 t0 = now_ns();
@@ -41,10 +38,16 @@ __device__ __forceinline__ bool mbar_wait(u32 bar, u32 parity, u32* err, u32 cod
     if (mbar_try(bar, parity)) return true;
     if ((it & 255) == 0 && (now_ns() - t0 > WAIT_NS || (err && *(volatile u32*)err))) {
       if (err) atomicCAS(err, 0u, code);
-      for (const u64 t1 = now_ns(); now_ns() - t1 < SETTLE_NS;) { }
       return false;
     }
   }
+}
+
+// The CTA's barrier before it gives up its shared and tensor memory.  Where one of its waits gave up, copies and
+// products of its own may still be in flight: 1 ms, they take microseconds, and they have ended.
+__device__ __forceinline__ void sync_settled(bool gave_up) {
+  if (__syncthreads_or(gave_up))
+    for (const u64 t0 = now_ns(); now_ns() - t0 < 1000000u;) { }
 }
 
 // Shared -> global tensor store of one box (rows outside the tensor are not written); completion is
