@@ -14,11 +14,11 @@
 // of log 2: z2 = log2(e) z is one fma from the sums, its exponential one ex2 (2^-22 relative, as far off as the
 // operands' split).
 // What the backward needs of it is saved in one opaque value (NllSaved): the scales, b log2(e), each
-// row's maximum m and sum s of exponentials below it, and h and W as split for the tensor core, 4 bytes a value.
-// m and s stay two floats: m + log2(s) in one is off by half a step of m, 4e-6 at logits of 100, and so would be
+// row's maximum m and 1 / s of the sum of exponentials below it, and h and W as split for the tensor core, 4 bytes a
+// value.  m and s stay two floats: m + log2(s) in one is off by half a step of m, 4e-6 at logits of 100, and so would be
 // the gradient of a row whose target is all but certain (and that row's dz would not add up to 0).
 // Backward: the vocabulary is walked in pieces (a bounded workspace).  A piece's logits are computed
-// again in the forward's order, turned into dz = (2^(z2 - m) - s [v = t]) g / s in the epilogue -- as fp16 hi / lo, what the two products after it read;
+// again in the forward's order, turned into dz = 2^(z2 - m) g / s - g [v = t] in the epilogue -- as fp16 hi / lo, what the two products after it read;
 // |dz| <= |g_i|, so its scale is known before -- and dh += dz W_piece^T and dW_piece = h^T dz follow.
 // db's column sums are taken in the dz epilogue, and added up there (or by tcb_nll_db) in the same way.
 //
@@ -66,7 +66,7 @@ template <bool BACK> struct Nll {
   }
   __device__ __forceinline__ NllScales* scales() const { return saved<NllScales>(0); }
   __device__ __forceinline__ float* bias2() const { return saved<float>(256); }
-  __device__ __forceinline__ float2* stats() const { return saved<float2>((u64)a.p[8]); }   // m, s of every row
+  __device__ __forceinline__ float2* stats() const { return saved<float2>((u64)a.p[8]); }   // m, 1 / s of every row
   __device__ __forceinline__ float* amax() const { return scratch<float>(0); }
   __device__ __forceinline__ float2* g_scale() const { return scratch<float2>(0); }   // up, down (backward)
 };
@@ -265,7 +265,7 @@ __device__ __forceinline__ void nll_write(const Nll<false>& n, u64 row, float m,
   if (!((u32)a.p[13] & NLL_NO_LOSS))
     reinterpret_cast<float*>(a.p[14] ? (u64)a.p[7] : a.out)[row] =
         nll_loss(m, s, __ldcg(n.scratch<float>((u64)a.p[11]) + row), n.target(row), reinterpret_cast<const float*>(a.in[2]));
-  n.stats()[row] = make_float2(m, s);
+  n.stats()[row] = make_float2(m, 1.0f / s);
 }
 
 // Forward epilogue: a row's maximum and sum of exponentials over the half tile's columns, the target's
@@ -333,7 +333,7 @@ struct NllDz {
   const TmaDesc* map;
   const float* bias2;
   float* part_row;   // where this lane's column sums go
-  float z2, up, down, m, s, g, bias;
+  float z2, up, down, m, g, p, bias;   // p: what an exponential is multiplied by
   int t;
   __device__ __forceinline__ explicit NllDz(const GemmParams& P) : a(P.a), map(&P.maps[2]) {}
   // The cotangent's scale: each CTA's epilogue warps look through all of it behind the first product.
@@ -370,9 +370,10 @@ struct NllDz {
     const Nll<true> n(a);
     const u64 row = e.row < n.R() ? e.row : n.R() - 1;
     t = n.target(row);
-    m = n.stats()[row].x;
-    s = n.stats()[row].y;
-    g = n.cotangent(row) * up / s;
+    const float2 stats = n.stats()[row];
+    m = stats.x;
+    g = n.cotangent(row) * up;
+    p = g * stats.y;
     if (e.row != row) t = -1;
     part_row = n.template scratch<float>((u64)a.p[11]) + ((u64)e.T.m0 / 32 + e.q) * n.V() + (u64)a.p[12] + e.lane;
     bias = bias2[nll_column(e, e.c0)];
@@ -389,12 +390,12 @@ struct NllDz {
       v[j] = ex2(v[j]);
       v[j + 1] = ex2(v[j + 1]);
     }
+#pragma unroll
+    for (int j = 0; j < 32; j += 2) mul2(v[j], v[j + 1], p, p);
     if (__any_sync(0xffffffffu, mine != 0u)) {   // in one block of 8 at 8192 classes
 #pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] = (mine >> j) & 1 ? v[j] - s : v[j];
+      for (int j = 0; j < 32; ++j) v[j] = (mine >> j) & 1 ? v[j] - g : v[j];
     }
-#pragma unroll
-    for (int j = 0; j < 32; j += 2) mul2(v[j], v[j + 1], g, g);
     if (t < 0) {   // not by g = 0: an excluded row's logits may be anything
 #pragma unroll
       for (int j = 0; j < 32; ++j) v[j] = 0.0f;
