@@ -167,7 +167,8 @@ def _check_eps(op, eps):
 
 def linear_nll_saved(R, d, V):
     """The value linearNll saves for its backward: byte offsets of its parts (the scales at 0, the scaled bias
-    at 256; "lse": each row's largest logit and 1 over its sum of exponentials below it) and its size in floats.  h and W are held as fp16 pairs in blocks of 256 columns."""
+    at 256; "lse": each row's largest logit and 1 over its sum of exponentials below it) and its size in floats.
+    h and W are held as fp16 pairs in blocks of 256 columns."""
     def up(n, k):
         return -(-n // k) * k
 

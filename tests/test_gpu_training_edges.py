@@ -121,6 +121,41 @@ def test_nll_mixed_magnitudes(pkg, mods, runner, what):
     check_nll(mods, runner, case)
 
 
+# ---------------------------------------------------------------- pieces and operands of odd shapes
+@pytest.mark.parametrize("bn,ctas", [(64, 1), (128, 1), (128, 2), (256, 2)])
+def test_nll_last_piece_of_one_column(pkg, mods, runner, monkeypatch, bn, ctas):
+    """The vocabulary in five pieces by the forward's tile, the last one column wide: most of its tile lies beyond."""
+    to = importlib.import_module(P + ".training_ops")
+    # (dW's products of one column take the narrowest tile whatever it costs)
+    monkeypatch.setattr(to, "F16_COST", {to.Tile(64, 1): (10 ** 6, 0, 10 ** 9, 0), to.Tile(bn, ctas): (100, 1000, 10 ** 9, 0)})
+    monkeypatch.setattr(to, "DZ_BYTES", 4 * 300 * 256)
+    assert to.nll_pieces(300, 1025) == (256, 5)
+    check_nll(mods, runner, nll_case(pkg, 300, 70, 1025, seed=bn), runs=2)
+
+
+def test_operands_that_are_one_value(pkg, mods, runner):
+    """Rows and weight of a head the same square matrix: its gradient is the sum of both; the gain of a head norm its
+    positions too."""
+    g = pkg.ir.Graph()
+    x = g.input("x", [90, 90])
+    y = g.linear_nll(x, x, None, g.input("t", [90]))
+    G = pkg.autodiff.grad(g, [y], [x])
+    rng = np.random.default_rng(5)
+    v = {"x": f32(rng.standard_normal((90, 90)) / 9), "t": rng.integers(-1, 90, 90).astype(np.float64), "d0": f32(rng.random(90))}
+    loss, dx = run_graph(mods, runner, G.graph, v, [y, G.grads[0]])
+    eloss, eg = ref.nll_bounds(v["x"], v["x"], None, v["t"], v["d0"])
+    within(loss, ref.nll(v["x"], v["x"], None, v["t"])[0], eloss, "loss")
+    want = ref.nll_grad(v["x"], v["x"], None, v["t"], v["d0"])
+    within(dx, want["h"] + want["w"], eg["h"] + eg["w"] + U * (np.abs(want["h"]) + np.abs(want["w"])), "dx")
+    g = pkg.ir.Graph()
+    x, gain = g.input("x", [2, 16, 3, 16]), g.input("gain", [16])
+    y = g.head_norm_rope(x, gain, gain)
+    v = {"x": f32(rng.standard_normal((2, 16, 3, 16))), "gain": f32(1 + 0.1 * rng.standard_normal(16))}
+    a = g.nodes[y].attrs
+    within(run_graph(mods, runner, g, v, [y])[0], ref.head(v["x"], v["gain"], v["gain"], a),
+           ref.head_bounds(v["x"], v["gain"], v["gain"], a, None)["y"], "y")
+
+
 # ---------------------------------------------------------------- memory that other launches left
 def test_one_off_runs_over_what_others_left_in_scratch(pkg, mods, runner):
     """The runner's scratch full of ones' bits (error words, counters, partial sums): a one-off run clears what it
