@@ -32,9 +32,10 @@
 // the even one's warp 1 issues the products of both (cta_group::2).  A stage of 32 K indices of a tile 256 wide
 // takes 768 clocks of products; one SM alone would load 48 KB in them, as many bytes a clock as it takes from L2
 // at best (64, measured with boxes of 16 KB), one of a pair 32 KB: 16384 x 1024 x 131072 with exponentials 10.9
-// ms alone, 9.2 in pairs.  A K step of 16 takes 290 to 305 ns then, 1.5 to 1.6 PFLOP/s of products.  128 wide a
-// pair is as fast as two SMs (166 to 200 ns a step), but draws less power: 4095 x 256 x 8192 forward and backward,
-// run for seconds, 269 us alone and 256 in pairs.  Full barriers are the even CTA's and count both CTAs' bytes,
+// ms alone, 9.2 in pairs.  A K step of 16 takes 290 to 310 ns in long products, the epilogues' share included
+// (1.5 to 1.6 PFLOP/s of products), 320 to 380 when run for seconds.  128 wide a pair is as fast as two SMs (164 to
+// 200 ns a step), but draws less power: 4095 x 256 x 8192 forward and backward, run for seconds, 269 us alone and 261
+// in pairs.  Full barriers are the even CTA's and count both CTAs' bytes,
 // empty and accumulator ones are each CTA's own, and both leave together.
 //
 // Work: where there are as many tiles as SMs or more, they go whole to the CTAs in turn, in grouped raster

@@ -4,7 +4,8 @@
 // Bound by reading W once.  The tensor core would need a pass for its largest magnitude, one that splits it and
 // one that reads it back; here every value of W goes from memory into at most 16 float32 multiply-adds on the CUDA
 // cores: 1 x 64 x 50001 34.6 -> 8.6 us, 4 x 276 x 89420 124 -> 25 us (W alone at the copy rate: 15), 16 x 1024 x
-// 131072 458 -> 228 us (82).  With 32 rows the tensor core's form is ahead: 128 us against 166 at 1024 x 32000.
+// 131072 464 -> 228 us (82), 16 x 64 x 65 12.3 -> 12.3 us.  Up to 4 rows W bounds it, at 16 the multiply-adds; with 32 the
+// tensor core's form is ahead: 128 us against 166 at 1024 x 32000.
 //
 // A block takes 128 columns and a range of the d indices; lanes hold four columns each, warps take every eighth
 // index, eight loads in flight, and h comes from shared memory four rows a load.  Each 32 columns of a row leave

@@ -61,8 +61,8 @@ def f16_tiles(M, N, tile, symmetric):
     return sum(tn - i * rows // tile.bn for i in range(tm)) if symmetric else tm * tn
 
 
-# Nanoseconds of a split-fp16 product by tile, as measured with every SM busy: a K step of 16 of one tile; an
-# epilogue; the exchange of a divided tile's partial sums, at all and for each part.
+# Nanoseconds of a split-fp16 product by tile, as measured in bursts with every SM busy: a K step of 16 of one tile,
+# without its epilogue's share; an epilogue; the exchange of a divided tile's partial sums, at all and for each part.
 F16_COST = {Tile(256, 2): (275, 6600, 3000, 2500), Tile(128, 2): (173, 3600, 1500, 1600),
             Tile(128, 1): (180, 3000, 1500, 1200), Tile(64, 1): (140, 1500, 1000, 700)}
 
@@ -192,7 +192,10 @@ def nll_source(bias, rows=False):
 """
 
 
-NLL_ROWS = 16    # most rows of a loss without a backward that are worth reading W as it is
+# Most rows of a loss without a backward that read W as it is (tcb/nll_rows.cuh) instead of splitting it for the tensor
+# core.  16 rows at d x V, us: 64 x 65 12.3 against 12.3, 256 x 8192 14.3 : 25.8, 1024 x 32000 69.8 : 125.9, 1024 x
+# 131072 228 : 464; 32 rows at 1024 x 32000 166 : 128, and their sums would take twice the registers.
+NLL_ROWS = 16
 
 
 def _nll_rows_launch(graph, node):
