@@ -517,17 +517,22 @@ def _sustained_peaks():
 
 
 def _code_hash(code):
-    """Hash of a launch's source plus the code of every library template it includes (their `//`
-    comments and blank lines left out), so a recorded traffic figure is used only for the exact
+    """Hash of a launch's source plus the code of every library template it includes, those of a template too
+    (their `//` comments and blank lines left out), so a recorded traffic figure is used only for the exact
     kernel it was captured on, and a comment edit does not orphan it."""
     import hashlib
     import re
     h = hashlib.sha256(code.encode())
     tdir = os.path.join(ROOT, "tensor-compiler-webgpu_b200", "csrc", "templates")
-    for name in sorted(set(re.findall(r'#include "tcb/([a-z_]+\.cuh)"', code))):
-        with open(os.path.join(tdir, name)) as f:
-            text = f.read()
-        lines = (ln.rstrip() for ln in re.sub(r"//[^\n]*", "", text).splitlines())
+    texts, found = {}, re.findall(r'#include "tcb/([a-z0-9_]+\.cuh)"', code)
+    while found:
+        name = found.pop()
+        if name not in texts:
+            with open(os.path.join(tdir, name)) as f:
+                texts[name] = re.sub(r"//[^\n]*", "", f.read())
+            found += re.findall(r'#include "tcb/([a-z0-9_]+\.cuh)"', texts[name])
+    for name in sorted(texts):
+        lines = (ln.rstrip() for ln in texts[name].splitlines())
         h.update("\n".join(ln for ln in lines if ln).encode())
     return h.hexdigest()[:16]
 
