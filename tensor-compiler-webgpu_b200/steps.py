@@ -370,7 +370,7 @@ def muon_names(names):
 
 def state_spec(names, shapes, opt=ADAM_3B):
     """The optimizer's state, (name, shape) in order: Adam's moments, or for Muon's matrices a momentum buffer."""
-    if opt["kind"] != "muon":
+    if opt.get("kind") != "muon":
         return adam_state_spec(names, shapes)
     mu = muon_names(names)
     return [(f"{p}.buf", shapes[p]) for p in mu] + adam_state_spec([n for n in names if n not in mu], shapes)
@@ -419,7 +419,7 @@ def build_step3b(V, B, cfg=CONFIG, opt=ADAM_3B, bug=None, rules=None):
     g = G.graph
     grads = {n: G.grads[k] for k, n in enumerate(names)}
     state = {name: g.input(name, shape) for name, shape in state_spec(names, param_shapes(V, cfg), opt)}
-    update = muon_update if opt["kind"] == "muon" else adam_update
+    update = muon_update if opt.get("kind") == "muon" else adam_update
     outputs = update(g, names, f["ids"], grads, state, opt)
     inputs = {**{n: f["ids"][n] for n in names}, "x": f["ids"]["x"], "y": f["ids"]["y"], **state}
     return {"graph": g, "names": names, "stateNames": list(state), "loss": f["loss"], "logits": f["logits"],
@@ -446,7 +446,7 @@ def build_adam_graph(V, cfg=CONFIG, opt=ADAM_3B):
     ids = {n: g.input(n, shapes[n]) for n in names}
     grads = {n: g.input(f"g:{n}", shapes[n]) for n in names}
     state = {name: g.input(name, shape) for name, shape in state_spec(names, shapes, opt)}
-    update = muon_update if opt["kind"] == "muon" else adam_update
+    update = muon_update if opt.get("kind") == "muon" else adam_update
     outputs = update(g, names, ids, grads, state, opt)
     inputs = {**ids, **{f"g:{n}": grads[n] for n in names}, **state}
     return {"graph": g, "names": names, "inputs": inputs, "outputs": outputs}

@@ -224,6 +224,15 @@ def test_muon_scales_by_fan_out_over_fan_in(pkg):
         s.muon_update(g, list(shapes), ids, grads, state, {**opt, "factor": "fan"})
 
 
+def test_optimizer_settings_without_a_kind_are_adams(pkg):
+    """Adam's settings alone, as before there was a second optimizer."""
+    s = pkg.steps
+    cfg = s.make_config(T=4, d=8, H=2, L=1, ff=16)
+    bare = {k: v for k, v in s.ADAM_3B.items() if k != "kind"}
+    for build in (lambda opt: s.build_step3b(7, 1, cfg, opt=opt), lambda opt: s.build_adam_graph(7, cfg, opt)):
+        assert build(bare)["graph"].to_json() == build(s.ADAM_3B)["graph"].to_json()
+
+
 def test_unknown_targets_are_refused(pkg):
     """A word that is neither form of the targets built the one-hot model before."""
     s = pkg.steps
