@@ -66,11 +66,19 @@ class Reader {
 
  private:
   const char* p_;
+  int depth_ = 0;
+  static constexpr int MAX_DEPTH = 256;   // a graph's JSON nests a fused body in a node's attributes: a few levels
+  struct Level {
+    int& d;
+    ~Level() { --d; }
+  };
   [[noreturn]] void fail(const char* what) { throw std::runtime_error(std::string("JSON: ") + what); }
   void ws() {
     while (*p_ == ' ' || *p_ == '\n' || *p_ == '\t' || *p_ == '\r') ++p_;
   }
   Value value() {
+    Level level{++depth_};
+    if (depth_ > MAX_DEPTH) fail("nested too deep");
     ws();
     Value v;
     switch (*p_) {

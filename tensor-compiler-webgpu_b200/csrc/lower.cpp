@@ -107,6 +107,8 @@ static Node node_from_json(const Value& n, int id) {
     if (auto* v = a->find("output")) nd.output = (int)v->as_int();
     if (auto* v = a->find("body")) nd.body = graph_from_json(*v);
   }
+  if (nd.op == "const" && !nd.scalar_value && (i64)nd.values.size() != size_of(nd.shape))
+    throw Error("node " + std::to_string(id) + " (const): " + std::to_string(nd.values.size()) + " values for its shape");
   for (int i : nd.inputs)
     if (i < 0 || i >= id) throw Error("node " + std::to_string(id) + ": input " + std::to_string(i) + " is not an earlier node");
   return nd;

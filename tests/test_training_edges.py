@@ -116,6 +116,30 @@ def test_coefficients_are_float32(pkg):
     assert status == 1 and "coeffs" in message
 
 
+# ---------------------------------------------------------------- graphs that are not well formed
+def test_the_library_refuses_short_constants(pkg):
+    """A constant with fewer values than its shape: refused when lowered (its upload ended the process)."""
+    rt = importlib.import_module(P + ".runtime")
+    g = pkg.ir.Graph()
+    g.add(g.input("x", [5]), g.const([1, 2, 3, 4, 5], [5]))
+    js = g.to_json()
+    assert _lower(rt, js) == (0, "")
+    for value in ([1, 2], [], [1, 2, 3, 4, 5, 6]):
+        js["nodes"][1]["attrs"]["value"] = value
+        status, message = _lower(rt, js)
+        assert status == 1 and "const" in message
+
+
+def test_the_library_refuses_deep_json(pkg):
+    """Brackets without end are an error, not a stack overflow."""
+    import ctypes
+    rt = importlib.import_module(P + ".runtime")
+    out = ctypes.c_void_p()
+    for text in (b'{"nodes":' + b"[" * 200000, b'{"nodes":' * 200000):
+        assert rt.lib().tc_lower_json(text, b"{}", ctypes.byref(out)) == 1
+        assert b"nested" in rt.lib().tc_last_error()
+
+
 # ---------------------------------------------------------------- sizes beyond any device
 def _big(pkg, which):
     g = pkg.ir.Graph()
