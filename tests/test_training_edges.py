@@ -383,3 +383,29 @@ def test_timed_programs_of_launches_with_several_outputs(pkg, monkeypatch):
         for lau in multi:
             for i in lau.nodes:
                 assert made["buffers"][i].ptr in used
+
+
+# ---------------------------------------------------------------- the backward's logits are the forward's
+@pytest.mark.parametrize("R,d,V", [(1, 16, 2), (64, 64, 65), (150, 600, 500), (33, 1030, 300), (40, 3000, 90), (4095, 256, 8192),
+                                   (8192, 1024, 50001), (16384, 17, 131072), (70000, 64, 600), (16, 64, 1 << 24), (200000, 32, 700),
+                                   (2048, 64, 131072), (131073, 8, 257)])
+def test_logits_are_computed_again_by_the_same_tiles(pkg, R, d, V):
+    """dz subtracts the maximum that the forward found, so its logits have to be the forward's bit for bit: the same
+    tile, and where K is divided among CTAs the same division (several pieces are never divided)."""
+    cg, to = importlib.import_module(P + ".codegen"), importlib.import_module(P + ".training_ops")
+    g = pkg.ir.Graph()
+    h, w = g.input("h", [R, d]), g.input("w", [d, V])
+    y = g.linear_nll(h, w, None, g.input("t", [R]))
+    G = pkg.autodiff.grad(g, [y], [h, w]).graph
+    calls = [c for lau in cg.lower(G)["launches"] for c in lau.calls]
+    (logits,) = [c for c in calls if c.name.startswith("tcb_nll_logits")]
+    dz = [c for c in calls if c.name.startswith("tcb_nll_dz")]
+    tile = logits.name.rsplit("_", 1)[1]
+    assert len(dz) == to.nll_pieces(R, V)[1] and all(c.name.rsplit("_", 1)[1] == tile for c in dz)
+    if len(dz) == 1:
+        assert dz[0].grid == logits.grid and dz[0].params[:3] == logits.params[:3]
+    else:
+        ctas = 2 if tile.endswith("x2") else 1
+        for c in (logits, *dz):
+            M, N = c.params[0] & 0xFFFFFFFF, c.params[0] >> 32
+            assert c.params[2] & 0xFFFFFFFF == to.f16_tiles(M, N, to.Tile(int(tile.split("x")[0]), ctas), False)
