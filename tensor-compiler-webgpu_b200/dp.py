@@ -195,7 +195,10 @@ class DPTrainer:
         self.step_device()
         if self.comm is not None and self.comm.world > 1:
             self.comm.wait()
-        return float(self.grad_prog.read(self.loss_id)[0])
+        loss = float(self.grad_prog.read(self.loss_id)[0])
+        self.grad_prog.check_errors()   # a bounded wait that ran out raises: the parameters are then not to be used
+        self.adam_prog.check_errors()
+        return loss
 
     def read(self, names):
         self.runner.sync()

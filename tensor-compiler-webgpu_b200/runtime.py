@@ -970,12 +970,15 @@ class GpuTrainer:
             self.prog.capture()
 
     def train(self, x, y):
-        """One step on batch (x, y); returns the loss from the parameters before the update."""
+        """One step on batch (x, y); returns the loss from the parameters before the update.  A bounded wait that
+        ran out in it raises TcError: the parameters are then not to be used."""
         s = self.step
         self.prog.write(s["inputs"]["x"], x)
         self.prog.write(s["inputs"]["y"], y)
         self.prog.run()
-        return float(self.prog.read(s["loss"])[0])
+        loss = float(self.prog.read(s["loss"])[0])
+        self.prog.check_errors()
+        return loss
 
     def read(self, names):
         return {n: self.prog.read(self.step["inputs"][n]) for n in names}

@@ -309,6 +309,43 @@ def test_replays_leave_the_error_words_alone(pkg, monkeypatch):
     assert kinds >= {("nll", True), ("nll", False), ("orth", True), ("orth", False), ("gemm", True)}
 
 
+def test_trainers_raise_a_step_whose_wait_ran_out(pkg, monkeypatch):
+    """train() reads the error words after its step: a wait that ran out is not a loss like any other."""
+    import ctypes
+    from test_program_plan import Recorder
+    rt, dp = importlib.import_module(P + ".runtime"), importlib.import_module(P + ".dp")
+    words = []
+
+    class Device(Recorder):
+        def tc_download(self, h, host, nbytes, offset):
+            ctypes.memset(host, 0, int(nbytes))
+            if words:
+                ctypes.memmove(host, (ctypes.c_uint32 * 1)(words[0]), 4)
+            return 0
+
+        def tc_memcpy_dtoh(self, ctx, host, src, nbytes):
+            ctypes.memset(host, 0, int(nbytes))
+            return 0
+
+        def tc_plan_run(self, plan):
+            return 0
+    rec = Device(rt.lib())
+    monkeypatch.setattr(rt, "lib", lambda: rec)
+    monkeypatch.setattr(rt.GpuRunner, "pipeline", lambda self, code: rt.Module(hash(code) & 0xFFFF, self))
+    s, cfg, step = _tiny_step(pkg, pkg.steps.MUON)
+    params = s.init_params_normal(11, 0, 0.02, cfg)
+    state = s.initial_state(step["names"], s.param_shapes(11, cfg), s.MUON)
+    runner = rt.GpuRunner(1, 0)
+    x, y = np.zeros(12 * 11), np.zeros(12)
+    for tr in (rt.FusedTrainer(runner, rt.fused_step(step, matmul="tiled"), params, state, capture=False),
+               dp.DPTrainer(runner, 11, 2, cfg, params, opt=s.MUON, capture=False)):
+        words[:] = []
+        assert tr.train(x, y) == 0.0
+        words[:] = [7]
+        with pytest.raises(rt.TcError, match="ran out"):
+            tr.train(x, y)
+
+
 @pytest.fixture(scope="module")
 def check_program(pkg, tmp_path_factory):
     import os
